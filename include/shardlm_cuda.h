@@ -249,6 +249,67 @@ int shd_attn_decode(shd_ctx* ctx, const float* q, const float* k_cache, const fl
 int shd_attn_prefill(shd_ctx* ctx, const float* q, const float* k_cache, const float* v_cache,
                      int kv_capacity, int H, int Hkv, int head_dim, int pos0, int M, int variant,
                      const float* mask, float* out_c, float* out_s);
+/* ----------------------------------------------------------------------------------------------
+ * 4-bit key/value cache (no counterpart in the reference, which keeps its reconstructed cache in f32,
+ * crates/v2/server/src/routes/secure_inference.rs:2452-2471): quantised as rows are written, read
+ * back, and attended to with an optional sliding window whose first tokens stay visible.
+ *
+ * A row is one position of one kv head: head_dim (64 or 128) channels in groups of 32. A group holds
+ * a scale s and a minimum z (f16) and 32 codes c in 0..15 and stands for fma(s, c, z):
+ *   z = f16(min x),  s = f16(max(max x - z, 0) * (1/15)),  c = clamp(rint((x - z) * (1/s)), 0, 15)
+ * evaluated in f32 (c = 0 where s = 0), x = client + server share: 5 bits a value with the parameters.
+ * Memory is the caller's:
+ *   k_codes, v_codes   uint8 [slots][n_kv_heads][capacity][head_dim / 2], two codes a byte, low first
+ *   k_params, v_params f16   [slots][n_kv_heads][capacity][2][head_dim / 32], scales then minima
+ * Keys keep 32-bit words of 8 channels: word t (channels 8 t .. + 7) of group g is word
+ * t * (head_dim / 32) + g of the row; values 16-bit half words of 4 channels: half word u of group g
+ * is half word u * (head_dim / 32) + g.
+ *
+ * Position p is in row p while p < capacity; past that, rows [sinks, capacity) are a ring and
+ * position p is in row sinks + (p - sinks) mod (capacity - sinks). A query at position p sees the
+ * positions t <= p with t < sinks or t > p - window; window 0 means all t <= p. Once positions have
+ * passed the capacity, the window must lie within the ring. Rows that were never written may hold
+ * anything. All pointers 16-byte aligned, capacity a multiple of 16, 0 <= sinks < capacity. The
+ * calls are asynchronous on the context's stream; they use no memory that is kept between calls
+ * except context scratch, so calls on one context are ordered by one stream at a time.
+ * -------------------------------------------------------------------------------------------- */
+typedef struct shd_kv4_cache {
+  uint8_t* k_codes;
+  uint16_t* k_params;
+  uint8_t* v_codes;
+  uint16_t* v_params;
+  int slots, n_kv_heads, capacity, head_dim;
+  int sinks; /* first positions whose rows are never reused; visible under every window */
+} shd_kv4_cache;
+
+/* Quantise M rows of reconstructed K and V (client + server shares, [M][ld], n_kv_heads * head_dim
+ * used; ks and vs null: kc and vc hold the values) into the cache. Row m goes to position pos[m] of
+ * slot[m] (device arrays; pos[m] < 0 skips the row; a slot outside the cache -> SHD_ERR_ARG at
+ * shd_sync, row skipped), or, with both null, to position pos0 + m of slot0. Two rows of one call
+ * must not go to the same cache row. k_val, v_val ([M][n_kv_heads * head_dim], nullable) receive the
+ * values that the written rows stand for (0 for skipped rows). A value that f16 cannot hold is
+ * clamped to +-65504, NaN is taken as 0, and either is reported as SHD_ERR_NUMERIC at shd_sync. */
+int shd_kv4_write(shd_ctx* ctx, const shd_kv4_cache* cache, const float* kc, const float* ks,
+                  const float* vc, const float* vs, int ld, const int32_t* slot, const int32_t* pos,
+                  int slot0, int pos0, int M, float* k_val, float* v_val);
+/* Positions [pos0, pos0 + n) of a slot as f32 rows [n][n_kv_heads * head_dim] (either output may be
+ * null), in the layout shd_model_read_kv and shd_attn_* use. */
+int shd_kv4_read(shd_ctx* ctx, const shd_kv4_cache* cache, int slot, int pos0, int n, float* k_out,
+                 float* v_out);
+/* Attention of one token for each of M sequences: q [M][ldq] reconstructed, H heads; row m is position
+ * pos[m] of slot[m] (device arrays) and its own K/V row is already written. The softmax is exact (no
+ * clamp of the scores). pos[m] < 0 sees nothing and gives 0; a slot outside the cache, or a position
+ * past the capacity whose window the ring does not hold, gives 0 and SHD_ERR_ARG at shd_sync. Output
+ * [M][H * head_dim], reshared (attn - mask, mask); mask null: (attn, 0). */
+int shd_kv4_attn_decode(shd_ctx* ctx, const shd_kv4_cache* cache, const float* q, int ldq, int H,
+                        const int32_t* slot, const int32_t* pos, int M, int window,
+                        const float* mask, float* out_c, float* out_s);
+/* The same attention for M consecutive positions pos0 .. pos0 + M - 1 of one slot, all of whose K/V
+ * rows are written; past the capacity the ring must hold window + M - 1 positions. */
+int shd_kv4_attn_prefill(shd_ctx* ctx, const shd_kv4_cache* cache, const float* q, int ldq, int H,
+                         int slot, int pos0, int M, int window, const float* mask, float* out_c,
+                         float* out_s);
+
 /* Server-side embedding share generation (get_embeddings_direct, crates/v2/server/src/routes/
  * secure_inference.rs:387-460): e = bf16 table row, server share uniform [0,1) (24-bit, rand's
  * Standard f32 construction) from Philox(seed, counter + m), client share e - s. */

@@ -71,6 +71,10 @@ SIGNATURES: dict[str, tuple] = {
     "shd_attn_decode": (I32, [P, P, P, P, I32, I32, I32, I32, P, I32, I32, P, P, P]),
     "shd_embed_shares": (I32, [P, P, I32, I32, P, I32, U64, U64, P, P]),
     "shd_attn_prefill": (I32, [P, P, P, P, I32, I32, I32, I32, I32, I32, I32, P, P, P]),
+    "shd_kv4_write": (I32, [P, P, P, P, P, P, I32, P, P, I32, I32, I32, P, P]),
+    "shd_kv4_read": (I32, [P, P, I32, I32, I32, P, P]),
+    "shd_kv4_attn_decode": (I32, [P, P, P, I32, I32, P, P, I32, I32, P, P, P]),
+    "shd_kv4_attn_prefill": (I32, [P, P, P, I32, I32, I32, I32, I32, I32, P, P, P]),
     "shd_model_prefill_hidden": (I32, [P, I32, P, P, I32, P, P, P, P, P]),
     "shd_model_read_kv": (I32, [P, I32, I32, I32, P, P]),
     "shd_model_forward_host_hidden": (I32, [P, I32, P, P, P, P, P, P]),
@@ -129,6 +133,15 @@ class ShardInfoC(C.Structure):
         ("kv_head_begin", I32), ("kv_head_count", I32),
         ("inter_begin", I32), ("inter_count", I32),
         ("vocab_begin", I32), ("vocab_count", I32),
+    ]
+
+
+class Kv4CacheC(C.Structure):
+    """shd_kv4_cache of include/shardlm_cuda.h."""
+    _fields_ = [
+        ("k_codes", P), ("k_params", P), ("v_codes", P), ("v_params", P),
+        ("slots", I32), ("n_kv_heads", I32), ("capacity", I32), ("head_dim", I32),
+        ("sinks", I32),
     ]
 
 _lib = None

@@ -1,0 +1,122 @@
+// The 4-bit key/value cache: format, addressing and visibility shared by its kernels (shd_kv4.cu,
+// shd_kv4_decode.cu, shd_kv4_prefill.cu).
+//
+// A row is one position of one kv head: head_dim channels in groups of 32, a group being 32 codes
+// c in 0..15 with a scale s and a minimum z in f16 and standing for s * c + z. Stored orders, chosen
+// so that one thread's share of a tensor-core fragment is contiguous:
+//   keys    32-bit word (t, g), t = 0..3 of group g, holds channels 32 g + 8 t .. + 7 and is word
+//           t * NG + g of the row: thread t of a quad reads its words of all NG groups at once
+//   values  16-bit half word (u, g), u = 0..7, holds channels 32 g + 4 u .. + 3 and is half word
+//           u * NG + g of the row
+//   params  [2][NG] f16 a row: the NG scales, then the NG minima
+// nibble n of a word is its n-th channel, lowest first.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "shd_common.cuh"
+
+namespace shd {
+
+constexpr int kKv4Group = 32;
+constexpr int kKv4Chunk = 16;  // rows the kernels take together; capacity is a multiple of it
+
+struct Kv4View {
+  uint8_t* kc;   // [slots][heads][capacity][HD / 2]
+  __half* kp;    // [slots][heads][capacity][2][HD / 32]
+  uint8_t* vc;
+  __half* vp;
+  int slots, heads, capacity, head_dim, sinks;
+};
+
+// Row of the cache that holds position p >= 0: itself up to the capacity, then a ring over the rows
+// behind the sinks.
+__host__ __device__ __forceinline__ int kv4_row(const Kv4View& c, int p) {
+  return p < c.capacity ? p : c.sinks + (p - c.sinks) % (c.capacity - c.sinks);
+}
+
+// First row of (slot, head): 64-bit, a long cache passes 2^31 bytes.
+__host__ __device__ __forceinline__ size_t kv4_base(const Kv4View& c, int slot, int head) {
+  return ((size_t)slot * c.heads + head) * (size_t)c.capacity;
+}
+
+// Whether queries at positions up to `last` can be served with the newest position being `last`:
+// past the capacity only what the ring still holds for the oldest query may be visible.
+__host__ __device__ __forceinline__ bool kv4_in_reach(const Kv4View& c, int last, int window, int extra) {
+  return last < c.capacity || (window > 0 && (int64_t)window + extra <= (int64_t)c.capacity - c.sinks);
+}
+
+// The rows that queries at positions [lo, hi] see, when `hi` is the newest position written, as up to
+// three intervals of 16-row chunks in increasing order (the sinks; the ring's two parts, or the one
+// run of positions). Every visible row is in exactly one of them.
+struct Kv4Spans {
+  int begin[3], end[3];
+  int total;
+};
+
+__host__ __device__ __forceinline__ Kv4Spans kv4_spans(const Kv4View& c, int lo, int hi, int window) {
+  Kv4Spans s;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) s.begin[i] = s.end[i] = 0;
+  s.total = 0;
+  if (hi < 0) return s;
+  const int64_t far = (int64_t)lo - window + 1;
+  if (window <= 0 || far <= c.sinks) {
+    // everything from position 0, in place unless the sequence has passed the capacity
+    const int rows = hi < c.capacity ? hi + 1 : c.capacity;
+    s.end[0] = (rows + kKv4Chunk - 1) / kKv4Chunk;
+  } else {
+    s.end[0] = (c.sinks + kKv4Chunk - 1) / kKv4Chunk;
+    const int first = kv4_row(c, (int)far), last = kv4_row(c, hi);
+    // the ring has been gone round between the two positions
+    const bool wrapped = hi >= c.capacity && first > last;
+    const int b1 = wrapped ? c.sinks : first, e1 = last + 1;
+    s.begin[1] = max(b1 / kKv4Chunk, s.end[0]);
+    s.end[1] = max((e1 + kKv4Chunk - 1) / kKv4Chunk, s.begin[1]);
+    if (wrapped) {
+      s.begin[2] = max(first / kKv4Chunk, s.end[1]);
+      s.end[2] = max((c.capacity + kKv4Chunk - 1) / kKv4Chunk, s.begin[2]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) s.total += s.end[i] - s.begin[i];
+  return s;
+}
+
+// i-th chunk of the spans, 0 <= i < total.
+__host__ __device__ __forceinline__ int kv4_span_chunk(const Kv4Spans& s, int i) {
+  const int n0 = s.end[0] - s.begin[0], n1 = s.end[1] - s.begin[1];
+  if (i < n0) return s.begin[0] + i;
+  if (i < n0 + n1) return s.begin[1] + (i - n0);
+  return s.begin[2] + (i - n0 - n1);
+}
+
+// Position held by row r when `last` is the newest position written (negative, or below the sinks for
+// a row behind them: none).
+__host__ __device__ __forceinline__ int kv4_held(const Kv4View& c, int r, int last) {
+  if (r < c.sinks || last < c.capacity) return r;
+  const int ring = c.capacity - c.sinks;
+  int back = (last - r) % ring;
+  return last - back;
+}
+
+// Whether a query at position p sees the row r that holds position t.
+__host__ __device__ __forceinline__ bool kv4_sees(const Kv4View& c, int p, int r, int t, int window) {
+  return t <= p && (window <= 0 || r < c.sinks || (int64_t)t > (int64_t)p - window);
+}
+
+// Attention over the cache: rows of several sequences (slot, pos) or consecutive positions of one.
+struct Kv4AttnArgs {
+  Kv4View c;
+  const float* q;  // reconstructed queries [M][ldq], H heads
+  int ldq, H, M;
+  const int32_t *slot, *pos;  // [M] device; null: row m is position pos0 + m of slot0
+  int slot0, pos0;
+  int window;   // 0: every earlier position
+  float scale;  // 1 / sqrt(head_dim)
+  const float* mask;       // [M][H * head_dim], nullable
+  float *out_c, *out_s;    // [M][H * head_dim]
+  int* err;
+};
+
+}  // namespace shd

@@ -1,0 +1,170 @@
+"""A key/value cache held in 4 bits, and the attention that reads it (shd_kv4_* of
+include/shardlm_cuda.h, which states the format and the rules of visibility).
+
+Against the f32 cache of the model loop (the reference's, crates/v2/server/src/routes/
+secure_inference.rs:2452-2471) a position takes 5/32 of the memory. Rows are quantised as they are
+written, straight from the K and V shares; queries may be limited to a sliding window, the first
+`sinks` positions staying visible, and a cache smaller than its sequences is then used as a ring.
+
+Device tensors in, device tensors out, asynchronous on torch's current stream; errors that only the
+device sees (a slot outside the cache, values that the format cannot hold) surface at Context.sync().
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import Kv4CacheC, check, lib
+from .runtime import Context
+from .sharing import SharingError
+
+GROUP = 32
+CHUNK = 16
+
+
+class Kv4Cache:
+    """`slots` sequences of up to `capacity` rows (rounded up to a multiple of 16) of n_kv_heads heads."""
+
+    def __init__(self, ctx: Context, slots: int, n_kv_heads: int, capacity: int, head_dim: int, sinks: int = 0):
+        if slots <= 0 or n_kv_heads <= 0 or capacity <= 0:
+            raise SharingError("a cache needs at least one slot, head and row")
+        if head_dim not in (64, 128):
+            raise SharingError("head_dim must be 64 or 128")
+        capacity = -(-capacity // CHUNK) * CHUNK
+        shape = (slots, n_kv_heads, capacity)
+        codes = [ctx.empty(*shape, head_dim // 2, dtype=torch.uint8) for _ in range(2)]
+        params = [ctx.empty(*shape, 2, head_dim // GROUP, dtype=torch.float16) for _ in range(2)]
+        self._bind(ctx, codes[0], params[0], codes[1], params[1], sinks)
+
+    @classmethod
+    def from_tensors(cls, ctx: Context, k_codes: torch.Tensor, k_params: torch.Tensor, v_codes: torch.Tensor,
+                     v_params: torch.Tensor, sinks: int = 0) -> "Kv4Cache":
+        """A cache over tensors that the caller holds (uint8 codes and float16 params in the format's layout)."""
+        self = cls.__new__(cls)
+        self._bind(ctx, k_codes, k_params, v_codes, v_params, sinks)
+        return self
+
+    def _bind(self, ctx, k_codes, k_params, v_codes, v_params, sinks):
+        if k_codes.dim() != 4:
+            raise SharingError("ShapeMismatch: codes are [slots, n_kv_heads, capacity, head_dim / 2]")
+        slots, heads, cap, half = k_codes.shape
+        for t, shape, dtype in ((k_codes, (slots, heads, cap, half), torch.uint8),
+                                (v_codes, (slots, heads, cap, half), torch.uint8),
+                                (k_params, (slots, heads, cap, 2, half // 16), torch.float16),
+                                (v_params, (slots, heads, cap, 2, half // 16), torch.float16)):
+            if t.dtype != dtype or t.device != ctx.torch_device or not t.is_contiguous():
+                raise SharingError(f"expected a contiguous {dtype} tensor on {ctx.torch_device}")
+            if tuple(t.shape) != shape:
+                raise SharingError(f"ShapeMismatch: expected {list(shape)}, got {list(t.shape)}")
+        if half not in (32, 64):
+            raise SharingError("head_dim must be 64 or 128")
+        if cap % CHUNK or not 0 <= sinks < cap:
+            raise SharingError("capacity must be a multiple of 16 and above the sinks")
+        self.ctx = ctx
+        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
+        self.slots, self.n_kv_heads, self.capacity, self.head_dim, self.sinks = slots, heads, cap, 2 * half, sinks
+        self.kv_dim = heads * 2 * half
+        self._c = Kv4CacheC(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), slots,
+                            heads, cap, 2 * half, sinks)
+        self._ref = C.byref(self._c)
+
+    @property
+    def device_bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_params, self.v_codes, self.v_params))
+
+    # -- argument checks -----------------------------------------------------------------------
+    def _rows(self, t: torch.Tensor, width: int, name: str) -> torch.Tensor:
+        """f32 [rows, width] on the cache's device whose rows the kernels can read: unit column stride,
+        16-byte aligned rows (anything else is copied)."""
+        if t.dtype != torch.float32 or t.device != self.ctx.torch_device:
+            raise SharingError(f"{name}: expected a float32 tensor on {self.ctx.torch_device}")
+        if t.dim() != 2 or t.shape[1] != width or t.shape[0] == 0:
+            raise SharingError(f"ShapeMismatch: {name}: expected [rows, {width}], got {list(t.shape)}")
+        ld = t.stride(0)
+        if t.stride(1) != 1 or ld < width or ld % 4 or ld > 0x7FFFFFFF or t.data_ptr() % 16:
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t
+
+    def _index(self, t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
+        if t.dtype != torch.int32 or t.device != self.ctx.torch_device or not t.is_contiguous():
+            raise SharingError(f"{name}: expected a contiguous int32 tensor on {self.ctx.torch_device}")
+        if t.numel() != rows:
+            raise SharingError(f"ShapeMismatch: {name}: expected [{rows}], got {list(t.shape)}")
+        return t
+
+    def _call(self, name: str, *args) -> None:
+        ctx = self.ctx
+        ctx.bind_stream()
+        check(getattr(lib(), name)(ctx.ptr, self._ref, *args), ctx.ptr)
+
+    # -- writing and reading -------------------------------------------------------------------
+    def _write(self, k_client, k_server, v_client, v_server, slot, pos, slot0, pos0, values):
+        if (k_server is None) != (v_server is None):
+            raise SharingError("server shares are given for K and V or for neither")
+        t = [None if x is None else self._rows(x, self.kv_dim, n) for x, n in
+             ((k_client, "k_client"), (k_server, "k_server"), (v_client, "v_client"), (v_server, "v_server"))]
+        rows = t[0].shape[0]
+        if any(x is not None and x.shape[0] != rows for x in t):
+            raise SharingError("ShapeMismatch: K and V shares differ in rows")
+        ld = t[0].stride(0) if rows > 1 else self.kv_dim
+        if rows > 1 and any(x is not None and x.stride(0) != ld for x in t):
+            t = [None if x is None else x.contiguous() for x in t]
+            ld = self.kv_dim
+        out = torch.empty(2, rows, self.kv_dim, dtype=torch.float32, device=self.ctx.torch_device) if values else None
+        if pos is not None:
+            slot, pos = self._index(slot, rows, "slot").data_ptr(), self._index(pos, rows, "pos").data_ptr()
+        self._call("shd_kv4_write", t[0].data_ptr(), None if t[1] is None else t[1].data_ptr(), t[2].data_ptr(),
+                   None if t[3] is None else t[3].data_ptr(), ld, slot, pos, slot0, pos0, rows,
+                   out[0].data_ptr() if values else None, out[1].data_ptr() if values else None)
+        return (out[0], out[1]) if values else None
+
+    def write(self, k_client, k_server, v_client, v_server, *, slot: torch.Tensor, pos: torch.Tensor, values: bool = False):
+        """Quantise one row for each sequence: row m goes to position pos[m] of slot[m] (device int32;
+        pos[m] < 0 skips the row). Server shares None: the client's hold the values. With `values`
+        returns (K, V), f32 [M, kv_dim]: what the written rows stand for."""
+        return self._write(k_client, k_server, v_client, v_server, slot, pos, 0, 0, values)
+
+    def write_prompt(self, k_client, k_server, v_client, v_server, *, slot: int, pos0: int, values: bool = False):
+        """Quantise consecutive positions pos0, pos0 + 1, .. of one slot."""
+        return self._write(k_client, k_server, v_client, v_server, None, None, slot, pos0, values)
+
+    def read(self, slot: int, pos0: int, n: int):
+        """Positions [pos0, pos0 + n) of a slot as (K, V), f32 [n, kv_dim]."""
+        if n <= 0:
+            raise SharingError("read: n must be positive")
+        out = torch.empty(2, n, self.kv_dim, dtype=torch.float32, device=self.ctx.torch_device)
+        self._call("shd_kv4_read", slot, pos0, n, out[0].data_ptr(), out[1].data_ptr())
+        return out[0], out[1]
+
+    # -- attention -----------------------------------------------------------------------------
+    def _attn_args(self, q, mask):
+        if q.dim() != 2 or q.shape[1] % self.kv_dim:
+            raise SharingError(f"ShapeMismatch: q: expected [rows, heads * {self.head_dim}] with heads a multiple of "
+                               f"{self.n_kv_heads}, got {list(q.shape)}")
+        q = self._rows(q, q.shape[1], "q")
+        rows, width = q.shape
+        if mask is not None:
+            mask = self._rows(mask, width, "mask")
+            if mask.shape[0] != rows:
+                raise SharingError("ShapeMismatch: mask and q differ in rows")
+            mask = mask.contiguous()
+        out = torch.empty(2, rows, width, dtype=torch.float32, device=self.ctx.torch_device)
+        return q, (q.stride(0) if rows > 1 else width), width // self.head_dim, mask, out
+
+    def attend(self, q: torch.Tensor, *, slot: torch.Tensor, pos: torch.Tensor, window: int = 0, mask: torch.Tensor | None = None):
+        """One token for each sequence: q [M, heads * head_dim] reconstructed, row m at position pos[m] of
+        slot[m] (device int32), whose K/V row is written. Output shares (attn - mask, mask), or (attn, 0)."""
+        q, ldq, heads, mask, out = self._attn_args(q, mask)
+        rows = q.shape[0]
+        self._call("shd_kv4_attn_decode", q.data_ptr(), ldq, heads, self._index(slot, rows, "slot").data_ptr(),
+                   self._index(pos, rows, "pos").data_ptr(), rows, window, None if mask is None else mask.data_ptr(),
+                   out[0].data_ptr(), out[1].data_ptr())
+        return out[0], out[1]
+
+    def attend_prompt(self, q: torch.Tensor, *, slot: int, pos0: int, window: int = 0, mask: torch.Tensor | None = None):
+        """Consecutive positions pos0, pos0 + 1, .. of one slot, all of whose K/V rows are written."""
+        q, ldq, heads, mask, out = self._attn_args(q, mask)
+        self._call("shd_kv4_attn_prefill", q.data_ptr(), ldq, heads, slot, pos0, q.shape[0], window,
+                   None if mask is None else mask.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
+        return out[0], out[1]
