@@ -5,6 +5,7 @@
 #include <vector>
 
 #include "shd_gemv.cuh"
+#include "shd_kv4.cuh"
 #include "shd_tc.cuh"
 
 using namespace shd;
@@ -50,6 +51,7 @@ extern "C" int shd_init(int device, shd_ctx** out) {
   if ((e = cudaMalloc(&ctx->d_err, 16)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMalloc(&ctx->d_partials, ctx->partial_floats * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMalloc(&ctx->d_counters, (size_t)ctx->n_counters * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
+  if ((e = cudaMalloc(&ctx->d_kv4, kv4_scratch_floats(ctx->num_sms) * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMemset(ctx->d_err, 0, 16)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMemset(ctx->d_counters, 0, (size_t)ctx->n_counters * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaDeviceSynchronize()) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
@@ -78,6 +80,7 @@ extern "C" int shd_destroy(shd_ctx* ctx) {
   cudaFree(ctx->d_err);
   cudaFree(ctx->d_partials);
   cudaFree(ctx->d_counters);
+  cudaFree(ctx->d_kv4);
   cudaFree(ctx->d_scratch64);
   cudaFree(ctx->d_stage);
   cudaFree(ctx->d_rope_cos);

@@ -316,7 +316,7 @@ extern "C" int shd_kv4_attn_decode(shd_ctx* ctx, const shd_kv4_cache* cache, con
   SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
   a.slot = slot;
   a.pos = pos;
-  return launch_attn(ctx, a);
+  return launch_kv4_decode(ctx, a);
 }
 
 extern "C" int shd_kv4_attn_prefill(shd_ctx* ctx, const shd_kv4_cache* cache, const float* q, int ldq, int H, int slot,

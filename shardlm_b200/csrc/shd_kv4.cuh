@@ -14,6 +14,8 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "shd_common.cuh"
 
 namespace shd {
@@ -118,5 +120,11 @@ struct Kv4AttnArgs {
   float *out_c, *out_s;    // [M][H * head_dim]
   int* err;
 };
+
+// Single-token attention (shd_kv4_decode.cu): CTAs of a launch, and the context scratch they leave the
+// parts of cut items in, two a CTA.
+inline int kv4_decode_ctas(int num_sms) { return 2 * num_sms; }
+inline size_t kv4_scratch_floats(int num_sms) { return (size_t)kv4_decode_ctas(num_sms) * 2 * (8 * 128 + 16); }
+int launch_kv4_decode(shd_ctx* ctx, const Kv4AttnArgs& a);
 
 }  // namespace shd

@@ -61,7 +61,7 @@ class Kv4Cache:
             raise SharingError("head_dim must be 64 or 128")
         if cap % CHUNK or not 0 <= sinks < cap:
             raise SharingError("capacity must be a multiple of 16 and above the sinks")
-        self.ctx = ctx
+        self.ctx, self._device = ctx, ctx.torch_device
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
         self.slots, self.n_kv_heads, self.capacity, self.head_dim, self.sinks = slots, heads, cap, 2 * half, sinks
         self.kv_dim = heads * 2 * half
@@ -77,47 +77,63 @@ class Kv4Cache:
     def _rows(self, t: torch.Tensor, width: int, name: str) -> torch.Tensor:
         """f32 [rows, width] on the cache's device whose rows the kernels can read: unit column stride,
         16-byte aligned rows (anything else is copied)."""
-        if t.dtype != torch.float32 or t.device != self.ctx.torch_device:
-            raise SharingError(f"{name}: expected a float32 tensor on {self.ctx.torch_device}")
-        if t.dim() != 2 or t.shape[1] != width or t.shape[0] == 0:
-            raise SharingError(f"ShapeMismatch: {name}: expected [rows, {width}], got {list(t.shape)}")
-        ld = t.stride(0)
-        if t.stride(1) != 1 or ld < width or ld % 4 or ld > 0x7FFFFFFF or t.data_ptr() % 16:
+        if t.dtype is not torch.float32 or t.device != self._device:
+            raise SharingError(f"{name}: expected a float32 tensor on {self._device}")
+        shape = t.shape
+        if len(shape) != 2 or shape[1] != width or shape[0] == 0:
+            raise SharingError(f"ShapeMismatch: {name}: expected [rows, {width}], got {list(shape)}")
+        ld, step = t.stride()
+        if step != 1 or ld < width or ld % 4 or ld > 0x7FFFFFFF or t.data_ptr() % 16:
             t = t.clone(memory_format=torch.contiguous_format)
         return t
 
-    def _index(self, t: torch.Tensor, rows: int, name: str) -> torch.Tensor:
-        if t.dtype != torch.int32 or t.device != self.ctx.torch_device or not t.is_contiguous():
-            raise SharingError(f"{name}: expected a contiguous int32 tensor on {self.ctx.torch_device}")
+    def _index(self, t: torch.Tensor, rows: int, name: str) -> int:
+        """Address of `rows` device int32."""
+        if t.dtype is not torch.int32 or t.device != self._device or not t.is_contiguous():
+            raise SharingError(f"{name}: expected a contiguous int32 tensor on {self._device}")
         if t.numel() != rows:
             raise SharingError(f"ShapeMismatch: {name}: expected [{rows}], got {list(t.shape)}")
-        return t
+        return t.data_ptr()
 
     def _call(self, name: str, *args) -> None:
         ctx = self.ctx
         ctx.bind_stream()
-        check(getattr(lib(), name)(ctx.ptr, self._ref, *args), ctx.ptr)
+        rc = getattr(lib(), name)(ctx.ptr, self._ref, *args)
+        if rc:
+            check(rc, ctx.ptr)
+
+    def _pair(self, rows: int, width: int):
+        """Two f32 [rows, width] outputs and their addresses."""
+        out = torch.empty((2, rows, width), dtype=torch.float32, device=self._device)
+        at = out.data_ptr()
+        return out.unbind(0), at, at + 4 * rows * width
 
     # -- writing and reading -------------------------------------------------------------------
     def _write(self, k_client, k_server, v_client, v_server, slot, pos, slot0, pos0, values):
+        width = self.kv_dim
+        kc, vc = self._rows(k_client, width, "k_client"), self._rows(v_client, width, "v_client")
         if (k_server is None) != (v_server is None):
             raise SharingError("server shares are given for K and V or for neither")
-        t = [None if x is None else self._rows(x, self.kv_dim, n) for x, n in
-             ((k_client, "k_client"), (k_server, "k_server"), (v_client, "v_client"), (v_server, "v_server"))]
-        rows = t[0].shape[0]
-        if any(x is not None and x.shape[0] != rows for x in t):
-            raise SharingError("ShapeMismatch: K and V shares differ in rows")
-        ld = t[0].stride(0) if rows > 1 else self.kv_dim
-        if rows > 1 and any(x is not None and x.stride(0) != ld for x in t):
-            t = [None if x is None else x.contiguous() for x in t]
-            ld = self.kv_dim
-        out = torch.empty(2, rows, self.kv_dim, dtype=torch.float32, device=self.ctx.torch_device) if values else None
+        ks = vs = None
+        if k_server is not None:
+            ks, vs = self._rows(k_server, width, "k_server"), self._rows(v_server, width, "v_server")
+        t = (kc, vc) if ks is None else (kc, vc, ks, vs)
+        rows = kc.shape[0]
+        for x in t:
+            if x.shape[0] != rows:
+                raise SharingError("ShapeMismatch: K and V shares differ in rows")
+        ld = kc.stride(0) if rows > 1 else width
+        for x in t:
+            if rows > 1 and x.stride(0) != ld:
+                kc, vc, ks, vs = (None if y is None else y.contiguous() for y in (kc, vc, ks, vs))
+                ld = width
+                break
         if pos is not None:
-            slot, pos = self._index(slot, rows, "slot").data_ptr(), self._index(pos, rows, "pos").data_ptr()
-        self._call("shd_kv4_write", t[0].data_ptr(), None if t[1] is None else t[1].data_ptr(), t[2].data_ptr(),
-                   None if t[3] is None else t[3].data_ptr(), ld, slot, pos, slot0, pos0, rows,
-                   out[0].data_ptr() if values else None, out[1].data_ptr() if values else None)
-        return (out[0], out[1]) if values else None
+            slot, pos = self._index(slot, rows, "slot"), self._index(pos, rows, "pos")
+        out, k_at, v_at = self._pair(rows, width) if values else (None, None, None)
+        self._call("shd_kv4_write", kc.data_ptr(), None if ks is None else ks.data_ptr(), vc.data_ptr(),
+                   None if vs is None else vs.data_ptr(), ld, slot, pos, slot0, pos0, rows, k_at, v_at)
+        return out
 
     def write(self, k_client, k_server, v_client, v_server, *, slot: torch.Tensor, pos: torch.Tensor, values: bool = False):
         """Quantise one row for each sequence: row m goes to position pos[m] of slot[m] (device int32;
@@ -133,38 +149,37 @@ class Kv4Cache:
         """Positions [pos0, pos0 + n) of a slot as (K, V), f32 [n, kv_dim]."""
         if n <= 0:
             raise SharingError("read: n must be positive")
-        out = torch.empty(2, n, self.kv_dim, dtype=torch.float32, device=self.ctx.torch_device)
-        self._call("shd_kv4_read", slot, pos0, n, out[0].data_ptr(), out[1].data_ptr())
-        return out[0], out[1]
+        out, k_at, v_at = self._pair(n, self.kv_dim)
+        self._call("shd_kv4_read", slot, pos0, n, k_at, v_at)
+        return out
 
     # -- attention -----------------------------------------------------------------------------
-    def _attn_args(self, q, mask):
+    def _queries(self, q, mask):
         if q.dim() != 2 or q.shape[1] % self.kv_dim:
             raise SharingError(f"ShapeMismatch: q: expected [rows, heads * {self.head_dim}] with heads a multiple of "
                                f"{self.n_kv_heads}, got {list(q.shape)}")
-        q = self._rows(q, q.shape[1], "q")
         rows, width = q.shape
+        q = self._rows(q, width, "q")
         if mask is not None:
-            mask = self._rows(mask, width, "mask")
+            mask = self._rows(mask, width, "mask").contiguous()
             if mask.shape[0] != rows:
                 raise SharingError("ShapeMismatch: mask and q differ in rows")
-            mask = mask.contiguous()
-        out = torch.empty(2, rows, width, dtype=torch.float32, device=self.ctx.torch_device)
-        return q, (q.stride(0) if rows > 1 else width), width // self.head_dim, mask, out
+        return q, (q.stride(0) if rows > 1 else width), rows, width, mask
 
     def attend(self, q: torch.Tensor, *, slot: torch.Tensor, pos: torch.Tensor, window: int = 0, mask: torch.Tensor | None = None):
         """One token for each sequence: q [M, heads * head_dim] reconstructed, row m at position pos[m] of
         slot[m] (device int32), whose K/V row is written. Output shares (attn - mask, mask), or (attn, 0)."""
-        q, ldq, heads, mask, out = self._attn_args(q, mask)
-        rows = q.shape[0]
-        self._call("shd_kv4_attn_decode", q.data_ptr(), ldq, heads, self._index(slot, rows, "slot").data_ptr(),
-                   self._index(pos, rows, "pos").data_ptr(), rows, window, None if mask is None else mask.data_ptr(),
-                   out[0].data_ptr(), out[1].data_ptr())
-        return out[0], out[1]
+        q, ldq, rows, width, mask = self._queries(q, mask)
+        slot_at, pos_at = self._index(slot, rows, "slot"), self._index(pos, rows, "pos")
+        out, c_at, s_at = self._pair(rows, width)
+        self._call("shd_kv4_attn_decode", q.data_ptr(), ldq, width // self.head_dim, slot_at, pos_at, rows, window,
+                   None if mask is None else mask.data_ptr(), c_at, s_at)
+        return out
 
     def attend_prompt(self, q: torch.Tensor, *, slot: int, pos0: int, window: int = 0, mask: torch.Tensor | None = None):
         """Consecutive positions pos0, pos0 + 1, .. of one slot, all of whose K/V rows are written."""
-        q, ldq, heads, mask, out = self._attn_args(q, mask)
-        self._call("shd_kv4_attn_prefill", q.data_ptr(), ldq, heads, slot, pos0, q.shape[0], window,
-                   None if mask is None else mask.data_ptr(), out[0].data_ptr(), out[1].data_ptr())
-        return out[0], out[1]
+        q, ldq, rows, width, mask = self._queries(q, mask)
+        out, c_at, s_at = self._pair(rows, width)
+        self._call("shd_kv4_attn_prefill", q.data_ptr(), ldq, width // self.head_dim, slot, pos0, rows, window,
+                   None if mask is None else mask.data_ptr(), c_at, s_at)
+        return out
