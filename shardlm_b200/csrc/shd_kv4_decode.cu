@@ -31,19 +31,23 @@ namespace {
 
 constexpr int kDWarps = 8;
 constexpr int kDThreads = 32 * kDWarps;
-constexpr int kDStages = 4;
+constexpr int kDStages = 2;       // of a warp's ring, two chunks each
 constexpr int kDRows = 1024;      // query rows of one launch (their chunk counts are in shared memory)
-constexpr int kDMinShare = 16;    // fewest chunks worth a CTA
+constexpr int kDItem = 8;         // what an item costs a CTA besides its chunks, in chunks
+constexpr int kDMinShare = 16 + kDItem;  // least cost worth a CTA
+constexpr float kNever = -3.0e38f;  // running maximum before any row
 
 template <int HD>
 struct DecodeShape {
   static constexpr int NG = HD / kKv4Group;
   static constexpr int CODE = kKv4Chunk * HD / 2;      // bytes of a chunk's codes (K or V)
   static constexpr int PAR = kKv4Chunk * 4 * NG;       // bytes of a chunk's parameters
-  static constexpr int STAGE = 2 * (CODE + PAR);
+  static constexpr int CHUNK = 2 * (CODE + PAR);
+  static constexpr int STAGE = 2 * CHUNK;
   static constexpr int PART = HD + 4;                  // of one head: running max, sum, 2 unused, weighted V
   static constexpr int LEFT = 8 * HD + 16;             // of a cut item: weighted V of 8 heads, maxima, sums
-  static constexpr int RING = kDWarps * kDStages * STAGE;
+  static constexpr int ROWS = 3 * 32 * NG * 4;         // f32 parameters of a stage's 32 rows, see Rows
+  static constexpr int RING = kDWarps * (kDStages * STAGE + ROWS);
   static constexpr int JOIN = kDWarps * 8 * PART * 4;  // per warp and head, over the rings
   static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + kDRows * 8 + 8 * 8 * 4 * 2 + 256;
 };
@@ -54,6 +58,47 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the same with nothing to add to
+__device__ __forceinline__ void mma_f16_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_f16_k8_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5}, {%6}, {%7, %7, %7, %7};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
+}
+
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -80,6 +125,16 @@ __device__ __forceinline__ uint32_t centre(uint32_t codes, __half2 up) {
   return *reinterpret_cast<const uint32_t*>(&y);
 }
 
+// two weights times their rows' scales, as two f16 terms
+__device__ __forceinline__ void split_weights(uint64_t w, uint64_t s, uint32_t& hi, uint32_t& lo) {
+  const uint64_t y = mul2(w, s);
+  const float2 f = unpair(y);
+  hi = pack_f16(f.x, f.y);
+  const float2 h = unpack_f16(hi);
+  const float2 r = unpair(fma2(pair(h.x, h.y), pair(-1.0f, -1.0f), y));
+  lo = pack_f16(r.x, r.y);
+}
+
 // 2^e as f32, -126 <= e <= 127
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -87,41 +142,55 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 // NaN as the greatest (the scaled value is then not finite either).
 __device__ __forceinline__ int ceil_exp2(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 126; }
 
+// Asynchronous copies of a chunk: this lane's source addresses for row 0 of the (slot, head) and its
+// places within a stage.
 template <int HD>
-__device__ __forceinline__ void issue_chunk(const Kv4View& c, size_t row0, uint8_t* st, int lane) {
+struct Feed {
   using S = DecodeShape<HD>;
-  constexpr int CPR = HD / 32;           // 16-byte pieces of a row of codes
-  constexpr int NC = kKv4Chunk * CPR;    // pieces of a chunk's codes: 64 or 32
-  const uint8_t* kc = c.kc + row0 * (HD / 2);
-  const uint8_t* vc = c.vc + row0 * (HD / 2);
-#pragma unroll
-  for (int i = 0; i < NC / 32; ++i) {
-    const int p = lane + 32 * i, r = p / CPR, q = p % CPR;
-    // keys: row sigma(n) of each 8 stored as n-th, so that a quad's 8 neighbours are contiguous
-    const int n = (r & 8) | ((r & 4) ? 2 * (r & 3) + 1 : 2 * (r & 3));
-    cp_async16(st + (n * CPR + q) * 16, kc + p * 16, 16);
-    // values: rows 2, 3 (mod 4) with their halves exchanged
-    const int x = HD == 128 ? q ^ (r & 2) : q;
-    cp_async16(st + S::CODE + (r * CPR + x) * 16, vc + p * 16, 16);
-  }
-  constexpr int NP = S::PAR / 16;  // 16 or 8
-  if (lane < 2 * NP) {
-    const bool v = lane >= NP;
-    const int p = v ? lane - NP : lane;
-    cp_async16(st + 2 * S::CODE + (v ? S::PAR : 0) + p * 16,
-               reinterpret_cast<const uint8_t*>(v ? c.vp : c.kp) + row0 * (4 * S::NG) + p * 16, 16);
-  }
-}
+  static constexpr int CPR = HD / 32;         // 16-byte pieces of a row of codes
+  static constexpr int NC = kKv4Chunk * CPR;  // pieces of a chunk's codes: 64 or 32
+  static constexpr int NP = S::PAR / 16;      // pieces of a chunk's parameters: 16 or 8
+  const uint8_t *k, *v, *p;
+  uint32_t dk[NC / 32], dv[NC / 32], dp;
 
-// NG scales and NG minima of a row
+  __device__ __forceinline__ void places(int lane) {
+#pragma unroll
+    for (int i = 0; i < NC / 32; ++i) {
+      const int x = lane + 32 * i, r = x / CPR, q = x % CPR;
+      // keys: row sigma(n) of each 8 stored as n-th, so that a quad's 8 neighbours are contiguous
+      const int n = (r & 8) | ((r & 4) ? 2 * (r & 3) + 1 : 2 * (r & 3));
+      dk[i] = (n * CPR + q) * 16;
+      // values: rows 2, 3 (mod 4) with their halves exchanged
+      dv[i] = S::CODE + (r * CPR + (HD == 128 ? q ^ (r & 2) : q)) * 16;
+    }
+    dp = 2 * S::CODE + min(lane, 2 * NP - 1) * 16;
+  }
+  __device__ __forceinline__ void source(const Kv4View& c, size_t base, int lane) {
+    k = c.kc + base * (HD / 2) + lane * 16;
+    v = c.vc + base * (HD / 2) + lane * 16;
+    p = reinterpret_cast<const uint8_t*>(lane < NP ? c.kp : c.vp) + base * (4 * S::NG) + (lane & (NP - 1)) * 16;
+  }
+  __device__ __forceinline__ void chunk(int i, uint32_t st, int lane) const {
+#pragma unroll
+    for (int j = 0; j < NC / 32; ++j) {
+      copy(st + dk[j], k + (size_t)i * S::CODE + j * 512);
+      copy(st + dv[j], v + (size_t)i * S::CODE + j * 512);
+    }
+    if (lane < 2 * NP) copy(st + dp, p + (size_t)i * S::PAR);
+  }
+  static __device__ __forceinline__ void copy(uint32_t dst, const uint8_t* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  }
+};
+
+// f32 pairs (rows sigma(2 tig), sigma(2 tig + 1)) of NG groups
 template <int NG>
-__device__ __forceinline__ void load_params(const uint8_t* p, uint32_t (&s)[NG / 2], uint32_t (&z)[NG / 2]) {
-  if constexpr (NG == 4) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    s[0] = v.x; s[1] = v.y; z[0] = v.z; z[1] = v.w;
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    s[0] = v.x; z[0] = v.y;
+__device__ __forceinline__ void load_pairs(const float* p, uint64_t (&v)[NG]) {
+#pragma unroll
+  for (int g = 0; g < NG; g += 2) {
+    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(p + 2 * g);
+    v[g] = x.x;
+    v[g + 1] = x.y;
   }
 }
 
@@ -132,12 +201,6 @@ struct Seen {
   __device__ __forceinline__ bool row(int r) const {
     const int t = r <= edge ? r + up : r + down;
     return r < sinks ? r <= p : (t >= lowest && t <= p);
-  }
-  // every row of the 16 from r0
-  __device__ __forceinline__ bool chunk(int r0) const {
-    const bool below = r0 + kKv4Chunk - 1 <= edge;
-    const int t = below ? r0 + up : r0 + down;
-    return r0 >= sinks && (below || r0 > edge) && t >= lowest && t + kKv4Chunk - 1 <= p;
   }
 };
 
@@ -193,11 +256,13 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   int64_t* scan = reinterpret_cast<int64_t*>(total + 32);               // [8] warp sums
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   const Kv4View& c = a.c;
+  Feed<HD> feed;
+  feed.places(lane);
   const __half2 low_up = __floats2half2_rn(32768.0f, 32768.0f), high_up = __floats2half2_rn(2048.0f, 2048.0f);
   pdl_trigger();
   pdl_wait();
 
-  // chunk counts of the rows, summed up to each (a row that sees nothing counts one, for its output)
+  // costs of the rows in chunks, summed up to each (a row that sees nothing counts one, for its output)
   const int G = a.H / c.heads, nsub = (G + 7) / 8, HS = c.heads * nsub;
   int64_t sum = 0;
   for (int m0 = 0; m0 < a.M; m0 += kDThreads) {
@@ -207,7 +272,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
       const int p = a.pos[m], sl = a.slot[m];
       const bool ok = p >= 0 && sl >= 0 && sl < c.slots && kv4_in_reach(c, p, a.window, 0);
       if (p >= 0 && !ok && blockIdx.x == 0) atomicOr(a.err, SHD_DEVERR_ARG);
-      n = ok ? max(kv4_spans(c, p, p, a.window).total, 1) : 1;
+      n = (ok ? max(kv4_spans(c, p, p, a.window).total, 1) : 1) + kDItem;
     }
     int64_t x = n;
 #pragma unroll
@@ -230,7 +295,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   const int64_t t_begin = blockIdx.x * per, t_end = min(T, t_begin + per);
 
   for (int64_t t = t_begin; t < t_end;) {
-    // the item that chunk t belongs to
+    // the item that t falls into: kDItem for its start and end, then its chunks
     int lo = 0, hi = a.M - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -238,10 +303,15 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     }
     const int m = lo;
     const int64_t row_t = pre[m] * HS;
-    const int n = (int)((m + 1 < a.M ? pre[m + 1] : sum) - pre[m]);
-    const int hs = (int)((t - row_t) / n);
-    const int64_t item_t = row_t + (int64_t)hs * n;
-    const int c0 = (int)(t - item_t), c1 = (int)min((int64_t)n, t_end - item_t);
+    const int cost = (int)((m + 1 < a.M ? pre[m + 1] : sum) - pre[m]), n = cost - kDItem;
+    const int hs = (int)((t - row_t) / cost);
+    const int64_t item_t = row_t + (int64_t)hs * cost;
+    const int64_t done = min(t_end, item_t + cost);
+    const int c0 = max((int)(t - item_t) - kDItem, 0), c1 = (int)(done - item_t) - kDItem;
+    if (c1 <= c0) {  // none of its chunks
+      t = done;
+      continue;
+    }
     const int kvh = hs / nsub, h0 = kvh * G + (hs % nsub) * 8, nh = min(8, kvh * G + G - h0);
     int p = a.pos[m], sl = a.slot[m];
     if (!(p >= 0 && sl >= 0 && sl < c.slots && kv4_in_reach(c, p, a.window, 0))) p = -1;
@@ -249,22 +319,37 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     const Seen seen = make_seen(c, p, a.window);
     const size_t base = p >= 0 ? kv4_base(c, sl, kvh) : 0;
 
-    // this warp's chunks: c0 + warp, + 8, ..
-    const int first = c0 + warp;
-    const int mine = p >= 0 && first < min(c1, sp.total) ? (min(c1, sp.total) - first + kDWarps - 1) / kDWarps : 0;
-    uint8_t* ring = smem + warp * (kDStages * SH::STAGE);
-#pragma unroll
-    for (int i = 0; i < kDStages - 1; ++i) {
-      if (i < mine) issue_chunk<HD>(c, base + (size_t)kv4_span_chunk(sp, first + i * kDWarps) * kKv4Chunk, ring + i * SH::STAGE, lane);
-      cp_async_commit();
-    }
+    // this warp's chunk pairs: c0 + 2 warp, + 16, ..
+    const int first = c0 + 2 * warp, stop = p >= 0 ? min(c1, sp.total) : 0;
+    const int mine = first < stop ? (stop - first + 2 * kDWarps - 1) / (2 * kDWarps) : 0;
+    uint8_t* ring = smem + warp * (kDStages * SH::STAGE + SH::ROWS);
+    const uint32_t ring_at = smem_u32(ring);
+    feed.source(c, base, lane);
+    float* rows_f32 = reinterpret_cast<float*>(ring + kDStages * SH::STAGE);
+    int row0 = 0, row1 = 0, next0 = 0, next1 = 0;  // first rows of the chunks at work, and of those on their way
+    auto issue = [&](int i) {
+      const int x = first + i * 2 * kDWarps;
+      const uint32_t st = ring_at + (i % kDStages) * SH::STAGE;
+      const int a0 = kv4_span_chunk(sp, x);
+      feed.chunk(a0, st, lane);
+      next0 = a0 * kKv4Chunk;
+      if (x + 1 < stop) {
+        const int a1 = kv4_span_chunk(sp, x + 1);
+        feed.chunk(a1, st + SH::CHUNK, lane);
+        next1 = a1 * kKv4Chunk;
+      }
+    };
+    if (mine > 0) issue(0);
+    cp_async_commit();
+    row0 = next0;
+    row1 = next1;
 
     // queries of head gid: two f16 terms of q * 2^k, in the order of the masked code words
-    uint32_t qh[NG][4], ql[NG][4];
-    float qs[NG], factor;
+    uint32_t qh[NG][4], ql[NG][4], zh, zl;
+    float factor, zfactor;
     {
       const float* q = a.q + (size_t)m * a.ldq + (size_t)(h0 + min(gid, nh - 1)) * HD + 8 * tig;
-      float x[NG][8], top = 0.0f;
+      float x[NG][8], qs[NG], top = 0.0f, ztop = 0.0f;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float4 u = *reinterpret_cast<const float4*>(q + 32 * g), v = *reinterpret_cast<const float4*>(q + 32 * g + 4);
@@ -287,12 +372,22 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         qs[g] = __fadd_rn(qs[g], __shfl_xor_sync(0xffffffffu, qs[g], 1));
-        qs[g] = __fadd_rn(qs[g], __shfl_xor_sync(0xffffffffu, qs[g], 2)) * sc;
+        qs[g] = __fadd_rn(qs[g], __shfl_xor_sync(0xffffffffu, qs[g], 2));
+        ztop = fmaxf(ztop, fabsf(qs[g]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           split_f16(x[g][i] * up, x[g][i + 4] * up, qh[g][i], ql[g][i]);  // channel pairs (i, i + 4)
         }
       }
+      // the query sums against a row's parameters (scales, then minima): word tig of the row
+      const int kz = max(min(12 - ceil_exp2(ztop), 100), -100);  // 7.5 |sum| 2^kz < 2^15
+      zfactor = sc * pow2i(-kz);
+      const float zup = pow2i(kz) * (tig < NG / 2 ? 7.5f : (tig < NG ? 1.0f : 0.0f));
+      float za = qs[0], zb = qs[1];
+      if constexpr (NG == 4) {
+        if (tig & 1) { za = qs[2]; zb = qs[3]; }
+      }
+      split_f16(za * zup, zb * zup, zh, zl);
     }
 
     float o[HD / 16][4];  // [2 g + e]: channels 32 g + 4 gid + 2 e (+ 1: third and fourth), heads 2 tig, + 1
@@ -300,164 +395,182 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-    float oz[NG], mx = -INFINITY, l = 0.0f;
+    uint64_t oz[NG];  // head gid's minima, even and odd rows
 #pragma unroll
-    for (int g = 0; g < NG; ++g) oz[g] = 0.0f;
-    // the weights are scaled by 2^(13 - ev); every value scale so far is <= evf = 2^ev, or 0
-    int ev = -100;
-    float evf = 0.0f;
+    for (int g = 0; g < NG; ++g) oz[g] = pair(0.0f, 0.0f);
+    // weights are 2^(score - ref), ref = running maximum - (13 - ev): every value scale so far (the
+    // largest is vbound, f16 bits) is below 2^ev, so that weight times scale is at most 2^13
+    float mx = kNever, ref = kNever, l = 0.0f;
+    uint32_t vbound = 0u;
+    int ev = 0;
 
     for (int i = 0; i < mine; ++i) {
-      cp_async_wait<kDStages - 2>();
+      cp_async_wait<0>();
       __syncwarp();
-      {
-        const int nx = i + kDStages - 1;
-        if (nx < mine)
-          issue_chunk<HD>(c, base + (size_t)kv4_span_chunk(sp, first + nx * kDWarps) * kKv4Chunk,
-                          ring + (nx % kDStages) * SH::STAGE, lane);
-        cp_async_commit();
-      }
       const uint8_t* st = ring + (i % kDStages) * SH::STAGE;
-      const int r0 = kv4_span_chunk(sp, first + i * kDWarps) * kKv4Chunk;
-
-      // scores of head gid with rows 8 j + tig and 8 j + tig + 4 (log2 units)
-      float s[2][2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        uint32_t kw[NG];
+      // row `lane` of the 32: whether it is seen, and its parameters in f32 for the 8 heads' lanes; a
+      // row out of sight has them 0, whatever its memory holds
+      uint32_t sight, vtop;
+      {
+        const int u = lane >> 4, r = lane & 15;
+        const bool ok = (u == 0 || first + i * 2 * kDWarps + 1 < stop) && seen.row((u ? row1 : row0) + r);
+        sight = __ballot_sync(0xffffffffu, ok);
+        uint8_t* kp = ring + (i % kDStages) * SH::STAGE + u * SH::CHUNK + 2 * SH::CODE + r * (4 * NG);
+        const uint8_t* vp = kp + SH::PAR;
+        uint32_t ks[NG / 2], vs[NG / 2], vz[NG / 2];
         if constexpr (NG == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(st + (8 * j + gid) * (HD / 2) + 16 * tig);
-          kw[0] = v.x; kw[1] = v.y; kw[2] = v.z; kw[3] = v.w;
+          const uint2 x = *reinterpret_cast<const uint2*>(kp);
+          const uint4 y = *reinterpret_cast<const uint4*>(vp);
+          ks[0] = x.x; ks[1] = x.y; vs[0] = y.x; vs[1] = y.y; vz[0] = y.z; vz[1] = y.w;
         } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(st + (8 * j + gid) * (HD / 2) + 8 * tig);
-          kw[0] = v.x; kw[1] = v.y;
+          const uint2 y = *reinterpret_cast<const uint2*>(vp);
+          ks[0] = *reinterpret_cast<const uint32_t*>(kp);
+          vs[0] = y.x; vz[0] = y.y;
         }
-        const uint8_t* kp = st + 2 * SH::CODE;
-        uint32_t s0[NG / 2], z0[NG / 2], s1[NG / 2], z1[NG / 2];
-        load_params<NG>(kp + (8 * j + tig) * (4 * NG), s0, z0);
-        load_params<NG>(kp + (8 * j + tig + 4) * (4 * NG), s1, z1);
-        float d0 = 0.0f, d1 = 0.0f, e0 = 0.0f, e1 = 0.0f;
+        if (!ok) {
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const uint32_t w = kw[g], w8 = w >> 8;
-          mma_f16(acc, qh[g][0], ql[g][0], qh[g][1], ql[g][1], centre(w & 0x000f000fu, low_up), centre(w & 0x00f000f0u, high_up));
-          mma_f16(acc, qh[g][2], ql[g][2], qh[g][3], ql[g][3], centre(w8 & 0x000f000fu, low_up), centre(w8 & 0x00f000f0u, high_up));
-          const float2 sa = unpack_f16(s0[g / 2]), sb = unpack_f16(s1[g / 2]);
-          const float2 za = unpack_f16(z0[g / 2]), zb = unpack_f16(z1[g / 2]);
-          const float s_a = (g & 1) ? sa.y : sa.x, s_b = (g & 1) ? sb.y : sb.x;
-          d0 = fmaf(s_a, acc[0] + acc[2], d0);
-          d1 = fmaf(s_b, acc[1] + acc[3], d1);
-          e0 = fmaf(fmaf(7.5f, s_a, (g & 1) ? za.y : za.x), qs[g], e0);
-          e1 = fmaf(fmaf(7.5f, s_b, (g & 1) ? zb.y : zb.x), qs[g], e1);
-        }
-        s[j][0] = fmaf(d0, factor, e0);
-        s[j][1] = fmaf(d1, factor, e1);
-      }
-
-      // value parameters of the same rows; rows out of sight weigh 0 and their parameters are not used
-      uint32_t vs[4][NG / 2], vz[4][NG / 2];
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        load_params<NG>(st + 2 * SH::CODE + SH::PAR + (8 * (x >> 1) + 4 * (x & 1) + tig) * (4 * NG), vs[x], vz[x]);
-      if (!seen.chunk(r0)) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (!seen.row(r0 + 8 * (x >> 1) + 4 * (x & 1) + tig)) {
-            s[x >> 1][x & 1] = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < NG / 2; ++g) vs[x][g] = vz[x][g] = 0u;
+          for (int g = 0; g < NG / 2; ++g) {
+            ks[g] = vs[g] = vz[g] = 0u;
+            *reinterpret_cast<uint2*>(kp + 8 * g) = make_uint2(0u, 0u);
           }
         }
+        // [chunk][half of the chunk][tig][group][row sigma(2 tig), sigma(2 tig + 1)]
+        float* out = rows_f32 + (((lane >> 3) * 4 + (lane & 3)) * NG) * 2 + ((lane >> 2) & 1);
+        vtop = 0u;
+#pragma unroll
+        for (int g = 0; g < NG / 2; ++g) {
+          const float2 k = unpack_f16(ks[g]), v = unpack_f16(vs[g]), z = unpack_f16(vz[g]);
+          out[4 * g] = k.x;
+          out[4 * g + 2] = k.y;
+          out[32 * NG + 4 * g] = v.x;
+          out[32 * NG + 4 * g + 2] = v.y;
+          out[64 * NG + 4 * g] = fmaf(7.5f, v.x, z.x);
+          out[64 * NG + 4 * g + 2] = fmaf(7.5f, v.y, z.y);
+          vtop = max(vtop, max(vs[g] & 0xffffu, vs[g] >> 16));  // positive f16 order as integers
+        }
+        vtop = __reduce_max_sync(0xffffffffu, vtop);
       }
+      __syncwarp();
+      if (i + 1 < mine) issue(i + 1);
+      cp_async_commit();
 
-      // running maximum of the head and running bound of the value scales: rescale when either grows
-      float tm = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+      // scores (log2 units) of head gid with row 8 j + tig (and + 4) of chunk u: s[4 u + 2 j (+ 1)]
+      float s[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* kc = st + u * SH::CHUNK;
+          const uint8_t* kp = kc + 2 * SH::CODE;
+          uint32_t kw[NG];
+          if constexpr (NG == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(kc + (8 * j + gid) * (HD / 2) + 16 * tig);
+            kw[0] = v.x; kw[1] = v.y; kw[2] = v.z; kw[3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(kc + (8 * j + gid) * (HD / 2) + 8 * tig);
+            kw[0] = v.x; kw[1] = v.y;
+          }
+          uint64_t sc[NG];
+          load_pairs<NG>(rows_f32 + ((2 * u + j) * 4 + tig) * NG * 2, sc);
+          // the minima's part: all parameters of row sigma(gid) times (7.5 and 1) x the groups' query sums
+          float z[4];
+          const int zr = 8 * j + (gid >> 1) + 4 * (gid & 1);
+          mma_f16_k8_new(z, zh, zl, *reinterpret_cast<const uint32_t*>(kp + zr * (4 * NG) + 4 * (NG == 4 ? tig : (tig & 1))));
+          uint64_t d = pair(0.0f, 0.0f);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            float acc[4];
+            const uint32_t w = kw[g], w8 = w >> 8;
+            mma_f16_new(acc, qh[g][0], ql[g][0], qh[g][1], ql[g][1], centre(w & 0x000f000fu, low_up), centre(w & 0x00f000f0u, high_up));
+            mma_f16(acc, qh[g][2], ql[g][2], qh[g][3], ql[g][3], centre(w8 & 0x000f000fu, low_up), centre(w8 & 0x00f000f0u, high_up));
+            d = fma2(sc[g], add2(pair(acc[0], acc[1]), pair(acc[2], acc[3])), d);
+          }
+          const float2 y = unpair(fma2(d, pair(factor, factor), mul2(add2(pair(z[0], z[1]), pair(z[2], z[3])), pair(zfactor, zfactor))));
+          s[4 * u + 2 * j] = y.x;
+          s[4 * u + 2 * j + 1] = y.y;
+        }
+      }
+      if (sight != 0xffffffffu) {
+        const uint32_t at = sight >> tig;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (!(at >> (4 * x) & 1u)) s[x] = -INFINITY;
+      }
+      float tm = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
-      __half2 hm = *reinterpret_cast<const __half2*>(&vs[0][0]);
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-#pragma unroll
-        for (int g = 0; g < NG / 2; ++g) hm = __hmax2(hm, *reinterpret_cast<const __half2*>(&vs[x][g]));
-      float vm = fmaxf(__low2float(hm), __high2float(hm));
-      vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 1));
-      vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, 2));
-      if (__any_sync(0xffffffffu, tm > mx || vm > evf)) {
-        const float mn = fmaxf(mx, tm);
-        const float al = mx == -INFINITY ? 0.0f : exp2_fast(mx - mn);
-        mx = mn;
+
+      // rescale when the head's maximum or the bound of the value scales grows
+      if (__any_sync(0xffffffffu, tm > mx || vtop > vbound)) {
+        mx = fmaxf(mx, tm);
+        if (vtop > vbound) {  // the same in every lane
+          ev = ceil_exp2(__half2float(__ushort_as_half((unsigned short)vtop))) + 1;
+          vbound = vtop;
+        }
+        const float now = mx == kNever ? kNever : mx - (float)(13 - ev);
+        const float al = exp2_fast(ref - now);
+        ref = now;
         l *= al;
 #pragma unroll
-        for (int g = 0; g < NG; ++g) oz[g] *= al;
-        float down = 1.0f;
-        if (vm > evf) {  // the same in every lane
-          const int e = ceil_exp2(vm) + 1;
-          down = evf == 0.0f ? 0.0f : pow2i(ev - e);
-          ev = e;
-          evf = pow2i(e);
-        }
-        const float al0 = __shfl_sync(0xffffffffu, al, 8 * tig) * down, al1 = __shfl_sync(0xffffffffu, al, 8 * tig + 4) * down;
+        for (int g = 0; g < NG; ++g) oz[g] = mul2(oz[g], pair(al, al));
+        const float al0 = __shfl_sync(0xffffffffu, al, 8 * tig), al1 = __shfl_sync(0xffffffffu, al, 8 * tig + 4);
 #pragma unroll
         for (int x = 0; x < HD / 16; ++x) {
           o[x][0] *= al0; o[x][1] *= al1; o[x][2] *= al0; o[x][3] *= al1;
         }
       }
 
-      // weights: plain for the sum and the minima, times scale and as two f16 terms for the codes
-      float w[4];
-      const float wup = pow2i(13 - ev);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float sx = s[x >> 1][x & 1];
-        w[x] = sx == -INFINITY ? 0.0f : exp2_fast(sx - mx);
-        l += w[x];
-      }
-      uint32_t wh[NG][2], wl[NG][2];
-#pragma unroll
-      for (int g = 0; g < NG / 2; ++g) {
-        float2 sv[4];
+      for (int u = 0; u < 2; ++u) {
+        // weights: plain for the sum and the minima, times scale and as two f16 terms for the codes
+        float w[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          sv[x] = unpack_f16(vs[x][g]);
-          const float2 zv = unpack_f16(vz[x][g]);
-          oz[2 * g] = fmaf(w[x], fmaf(7.5f, sv[x].x, zv.x), oz[2 * g]);
-          oz[2 * g + 1] = fmaf(w[x], fmaf(7.5f, sv[x].y, zv.y), oz[2 * g + 1]);
+          w[x] = exp2_fast(s[4 * u + x] - ref);
+          l += w[x];
         }
+        uint32_t wh[NG][2], wl[NG][2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float wa = w[2 * j] * wup, wb = w[2 * j + 1] * wup;
-          split_f16(wa * sv[2 * j].x, wb * sv[2 * j + 1].x, wh[2 * g][j], wl[2 * g][j]);
-          split_f16(wa * sv[2 * j].y, wb * sv[2 * j + 1].y, wh[2 * g + 1][j], wl[2 * g + 1][j]);
+          const uint64_t ww = pair(w[2 * j], w[2 * j + 1]);
+          uint64_t sc[NG], mid[NG];
+          load_pairs<NG>(rows_f32 + 32 * NG + ((2 * u + j) * 4 + tig) * NG * 2, sc);
+          load_pairs<NG>(rows_f32 + 64 * NG + ((2 * u + j) * 4 + tig) * NG * 2, mid);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            oz[g] = fma2(ww, mid[g], oz[g]);
+            split_weights(ww, sc[g], wh[g][j], wl[g][j]);
+          }
+        }
+        // value codes of unit gid, rows in the same order
+        uint32_t vw[4][NG / 2];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int r = 8 * (x >> 1) + 4 * (x & 1) + tig;
+          const uint8_t* v = st + u * SH::CHUNK + SH::CODE + r * (HD / 2);
+          if constexpr (NG == 4) {
+            const uint2 y = *reinterpret_cast<const uint2*>(v + 16 * ((gid >> 1) ^ (r & 2)) + 8 * (gid & 1));
+            vw[x][0] = y.x; vw[x][1] = y.y;
+          } else {
+            vw[x][0] = *reinterpret_cast<const uint32_t*>(v + 4 * gid);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const uint32_t t0 = __byte_perm(vw[0][g / 2], vw[1][g / 2], (g & 1) ? 0x7632 : 0x5410);
+          const uint32_t t1 = __byte_perm(vw[2][g / 2], vw[3][g / 2], (g & 1) ? 0x7632 : 0x5410);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t u0 = e ? t0 >> 8 : t0, u1 = e ? t1 >> 8 : t1;
+            const uint32_t a0 = centre(u0 & 0x000f000fu, low_up), a1 = centre(u0 & 0x00f000f0u, high_up);
+            const uint32_t a2 = centre(u1 & 0x000f000fu, low_up), a3 = centre(u1 & 0x00f000f0u, high_up);
+            mma_f16(o[2 * g + e], a0, a1, a2, a3, wh[g][0], wh[g][1]);
+            mma_f16(o[2 * g + e], a0, a1, a2, a3, wl[g][0], wl[g][1]);
+          }
         }
       }
-
-      // value codes of unit gid, rows in the same order
-      uint32_t vw[4][NG / 2];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int r = 8 * (x >> 1) + 4 * (x & 1) + tig;
-        const uint8_t* v = st + SH::CODE + r * (HD / 2);
-        if constexpr (NG == 4) {
-          const uint2 y = *reinterpret_cast<const uint2*>(v + 16 * ((gid >> 1) ^ (r & 2)) + 8 * (gid & 1));
-          vw[x][0] = y.x; vw[x][1] = y.y;
-        } else {
-          vw[x][0] = *reinterpret_cast<const uint32_t*>(v + 4 * gid);
-        }
-      }
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const uint32_t t0 = __byte_perm(vw[0][g / 2], vw[1][g / 2], (g & 1) ? 0x7632 : 0x5410);
-        const uint32_t t1 = __byte_perm(vw[2][g / 2], vw[3][g / 2], (g & 1) ? 0x7632 : 0x5410);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t u0 = e ? t0 >> 8 : t0, u1 = e ? t1 >> 8 : t1;
-          const uint32_t a0 = centre(u0 & 0x000f000fu, low_up), a1 = centre(u0 & 0x00f000f0u, high_up);
-          const uint32_t a2 = centre(u1 & 0x000f000fu, low_up), a3 = centre(u1 & 0x00f000f0u, high_up);
-          mma_f16(o[2 * g + e], a0, a1, a2, a3, wh[g][0], wh[g][1]);
-          mma_f16(o[2 * g + e], a0, a1, a2, a3, wl[g][0], wl[g][1]);
-        }
-      }
+      row0 = next0;
+      row1 = next1;
     }
     cp_async_wait<0>();
 
@@ -466,23 +579,25 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     __syncthreads();  // every ring is done with
     float* part = reinterpret_cast<float*>(smem);
-    const float f0 = evf * 0.0625f;  // 2^(ev - 13) * 2^9
+    float ozf[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      oz[g] += __shfl_xor_sync(0xffffffffu, oz[g], 1);
-      oz[g] += __shfl_xor_sync(0xffffffffu, oz[g], 2);
-      const float za = __shfl_sync(0xffffffffu, oz[g], 8 * tig), zb = __shfl_sync(0xffffffffu, oz[g], 8 * tig + 4);
+      const float2 y = unpair(oz[g]);
+      ozf[g] = y.x + y.y;
+      ozf[g] += __shfl_xor_sync(0xffffffffu, ozf[g], 1);
+      ozf[g] += __shfl_xor_sync(0xffffffffu, ozf[g], 2);
+      const float za = __shfl_sync(0xffffffffu, ozf[g], 8 * tig), zb = __shfl_sync(0xffffffffu, ozf[g], 8 * tig + 4);
       float* pa = part + (warp * 8 + 2 * tig) * PART + 4 + 32 * g + 4 * gid;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        pa[2 * e] = fmaf(o[2 * g + e][0], f0, za);
-        pa[2 * e + 1] = fmaf(o[2 * g + e][2], f0, za);
-        pa[PART + 2 * e] = fmaf(o[2 * g + e][1], f0, zb);
-        pa[PART + 2 * e + 1] = fmaf(o[2 * g + e][3], f0, zb);
+        pa[2 * e] = fmaf(o[2 * g + e][0], 512.0f, za);  // codes were (c - 7.5) 2^-9
+        pa[2 * e + 1] = fmaf(o[2 * g + e][2], 512.0f, za);
+        pa[PART + 2 * e] = fmaf(o[2 * g + e][1], 512.0f, zb);
+        pa[PART + 2 * e + 1] = fmaf(o[2 * g + e][3], 512.0f, zb);
       }
     }
     if (tig == 0) {
-      part[(warp * 8 + gid) * PART] = mx;
+      part[(warp * 8 + gid) * PART] = ref == kNever ? -INFINITY : ref;
       part[(warp * 8 + gid) * PART + 1] = l;
     }
     __syncthreads();
@@ -518,7 +633,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     }
     if (!whole) {
       // the last CTA of the item joins the parts in CTA order
-      const int w0 = (int)(item_t / per), parts = (int)((item_t + n - 1) / per) - w0 + 1;
+      const int w0 = (int)((item_t + kDItem) / per), parts = (int)((item_t + cost - 1) / per) - w0 + 1;
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -570,7 +685,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
       }
     }
     __syncthreads();  // the shared memory is used again
-    t += c1 - c0;
+    t = done;
   }
 }
 
