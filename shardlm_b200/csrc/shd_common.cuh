@@ -30,7 +30,8 @@ struct shd_ctx {
   size_t partial_floats = 0;
   int* d_counters = nullptr;     // per-tile arrival counters, left zero by every kernel
   int n_counters = 0;
-  float* d_kv4 = nullptr;        // partial results of attention over the 4-bit cache
+  float* d_kv4 = nullptr;        // partial results of attention over the 4-bit cache: single tokens
+  float* d_kv4_parts = nullptr;  // and blocks of positions (allocated by the first such call)
   unsigned long long* d_scratch64 = nullptr;  // one word for synchronous result checks (encoders)
   void* d_stage = nullptr;  // staging of the synchronous per-call entry points (metadata, OT queries)
   size_t stage_bytes = 0;

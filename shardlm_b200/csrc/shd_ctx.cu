@@ -81,6 +81,7 @@ extern "C" int shd_destroy(shd_ctx* ctx) {
   cudaFree(ctx->d_partials);
   cudaFree(ctx->d_counters);
   cudaFree(ctx->d_kv4);
+  cudaFree(ctx->d_kv4_parts);
   cudaFree(ctx->d_scratch64);
   cudaFree(ctx->d_stage);
   cudaFree(ctx->d_rope_cos);

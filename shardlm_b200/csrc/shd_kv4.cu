@@ -332,5 +332,5 @@ extern "C" int shd_kv4_attn_prefill(shd_ctx* ctx, const shd_kv4_cache* cache, co
   SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
   a.slot0 = slot;
   a.pos0 = pos0;
-  return launch_attn(ctx, a);
+  return launch_kv4_prefill(ctx, a);
 }

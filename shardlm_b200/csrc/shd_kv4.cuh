@@ -48,9 +48,9 @@ __host__ __device__ __forceinline__ bool kv4_in_reach(const Kv4View& c, int last
   return last < c.capacity || (window > 0 && (int64_t)window + extra <= (int64_t)c.capacity - c.sinks);
 }
 
-// The rows that queries at positions [lo, hi] see, when `hi` is the newest position written, as up to
-// three intervals of 16-row chunks in increasing order (the sinks; the ring's two parts, or the one
-// run of positions). Every visible row is in exactly one of them.
+// The rows that queries at positions [lo, hi] see as up to three intervals of 16-row chunks in
+// increasing order (the sinks; the ring's two parts, or the one run of positions). Every visible row is
+// in exactly one of them. Call only where kv4_in_reach holds.
 struct Kv4Spans {
   int begin[3], end[3];
   int total;
@@ -64,20 +64,18 @@ __host__ __device__ __forceinline__ Kv4Spans kv4_spans(const Kv4View& c, int lo,
   if (hi < 0) return s;
   const int64_t far = (int64_t)lo - window + 1;
   if (window <= 0 || far <= c.sinks) {
-    // everything from position 0, in place unless the sequence has passed the capacity
-    const int rows = hi < c.capacity ? hi + 1 : c.capacity;
-    s.end[0] = (rows + kKv4Chunk - 1) / kKv4Chunk;
+    // everything from position 0: the sequence is within the capacity
+    s.end[0] = ((hi < c.capacity ? hi + 1 : c.capacity) + kKv4Chunk - 1) / kKv4Chunk;
   } else {
     s.end[0] = (c.sinks + kKv4Chunk - 1) / kKv4Chunk;
     const int first = kv4_row(c, (int)far), last = kv4_row(c, hi);
-    // the ring has been gone round between the two positions
-    const bool wrapped = hi >= c.capacity && first > last;
+    const bool wrapped = first > last;  // the ring's end lies between the two
     const int b1 = wrapped ? c.sinks : first, e1 = last + 1;
     s.begin[1] = max(b1 / kKv4Chunk, s.end[0]);
     s.end[1] = max((e1 + kKv4Chunk - 1) / kKv4Chunk, s.begin[1]);
     if (wrapped) {
       s.begin[2] = max(first / kKv4Chunk, s.end[1]);
-      s.end[2] = max((c.capacity + kKv4Chunk - 1) / kKv4Chunk, s.begin[2]);
+      s.end[2] = max(c.capacity / kKv4Chunk, s.begin[2]);
     }
   }
 #pragma unroll
@@ -126,5 +124,7 @@ struct Kv4AttnArgs {
 inline int kv4_decode_ctas(int num_sms) { return 2 * num_sms; }
 inline size_t kv4_scratch_floats(int num_sms) { return (size_t)kv4_decode_ctas(num_sms) * 2 * (8 * 128 + 16); }
 int launch_kv4_decode(shd_ctx* ctx, const Kv4AttnArgs& a);
+// Blocks of positions (shd_kv4_prefill.cu).
+int launch_kv4_prefill(shd_ctx* ctx, const Kv4AttnArgs& a);
 
 }  // namespace shd
