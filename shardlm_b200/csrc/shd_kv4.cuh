@@ -105,6 +105,73 @@ __host__ __device__ __forceinline__ bool kv4_sees(const Kv4View& c, int p, int r
   return t <= p && (window <= 0 || r < c.sinks || (int64_t)t > (int64_t)p - window);
 }
 
+#ifdef __CUDACC__
+// ------------------------------------------------------------------------------------------------
+// Arithmetic of the attention kernels
+// ------------------------------------------------------------------------------------------------
+constexpr float kKv4Never = -3.0e38f;  // running maximum before any row
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e as f32, -126 <= e <= 127
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+// an e with |x| < 2^e <= 2 |x|: 0 and denormals as the least, inf and NaN as the greatest
+__device__ __forceinline__ int ceil_exp2(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 126; }
+
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) { return as_u32(__floats2half2_rn(lo, hi)); }
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(as_half2(v)); }
+
+// two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+// a pair of values as two f16 terms each
+__device__ __forceinline__ void split_pair(uint64_t y, uint32_t& hi, uint32_t& lo) {
+  const float2 f = unpair(y);
+  hi = pack_f16(f.x, f.y);
+  const float2 h = unpack_f16(hi);
+  const float2 r = unpair(fma2(pair(h.x, h.y), pair(-1.0f, -1.0f), y));
+  lo = pack_f16(r.x, r.y);
+}
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) { split_pair(pair(a, b), hi, lo); }
+
+// two codes under a mask, c * 2^-24 (low nibbles of a half word: up = 2^15) or c * 2^-20 (the next: up =
+// 2^11), as (c - 7.5) * 2^-9, exactly
+__device__ __forceinline__ __half2 centre(uint32_t codes, __half2 up) {
+  return __hfma2(as_half2(codes), up, __floats2half2_rn(-7.5f / 512, -7.5f / 512));
+}
+__device__ __forceinline__ __half2 centre_low(uint32_t w) { return centre(w & 0x000f000fu, __floats2half2_rn(32768.0f, 32768.0f)); }
+__device__ __forceinline__ __half2 centre_high(uint32_t w) { return centre(w & 0x00f000f0u, __floats2half2_rn(2048.0f, 2048.0f)); }
+#endif
+
 // Attention over the cache: rows of several sequences (slot, pos) or consecutive positions of one.
 struct Kv4AttnArgs {
   Kv4View c;

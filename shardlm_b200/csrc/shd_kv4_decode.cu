@@ -35,7 +35,6 @@ constexpr int kDStages = 2;       // of a warp's ring, two chunks each
 constexpr int kDRows = 1024;      // query rows of one launch (their chunk counts are in shared memory)
 constexpr int kDItem = 8;         // what an item costs a CTA besides its chunks, in chunks
 constexpr int kDMinShare = 16 + kDItem;  // least cost worth a CTA
-constexpr float kNever = -3.0e38f;  // running maximum before any row
 
 template <int HD>
 struct DecodeShape {
@@ -73,74 +72,6 @@ __device__ __forceinline__ void mma_f16_k8_new(float (&d)[4], uint32_t a0, uint3
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a0), "r"(a1), "r"(b0), "f"(0.0f));
 }
-
-// two f32 operations in one instruction
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-  return v;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-// two values as two f16 terms each
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_f16(a, b);
-  const float2 h = unpack_f16(hi);
-  lo = pack_f16(__fsub_rn(a, h.x), __fsub_rn(b, h.y));
-}
-
-// two codes under a mask, c * 2^-24 (up = 2^15) or c * 2^-20 (up = 2^11), as (c - 7.5) * 2^-9
-__device__ __forceinline__ uint32_t centre(uint32_t codes, __half2 up) {
-  const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&codes), up, __floats2half2_rn(-7.5f / 512, -7.5f / 512));
-  return *reinterpret_cast<const uint32_t*>(&y);
-}
-
-// two weights times their rows' scales, as two f16 terms
-__device__ __forceinline__ void split_weights(uint64_t w, uint64_t s, uint32_t& hi, uint32_t& lo) {
-  const uint64_t y = mul2(w, s);
-  const float2 f = unpair(y);
-  hi = pack_f16(f.x, f.y);
-  const float2 h = unpack_f16(hi);
-  const float2 r = unpair(fma2(pair(h.x, h.y), pair(-1.0f, -1.0f), y));
-  lo = pack_f16(r.x, r.y);
-}
-
-// 2^e as f32, -126 <= e <= 127
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-
-// Exponent that scales |x| <= 2^e: biased exponent arithmetic, 0 and denormals as the least, inf and
-// NaN as the greatest (the scaled value is then not finite either).
-__device__ __forceinline__ int ceil_exp2(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 126; }
 
 // Asynchronous copies of a chunk: this lane's source addresses for row 0 of the (slot, head) and its
 // places within a stage.
@@ -258,7 +189,6 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   const Kv4View& c = a.c;
   Feed<HD> feed;
   feed.places(lane);
-  const __half2 low_up = __floats2half2_rn(32768.0f, 32768.0f), high_up = __floats2half2_rn(2048.0f, 2048.0f);
   pdl_trigger();
   pdl_wait();
 
@@ -400,7 +330,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     for (int g = 0; g < NG; ++g) oz[g] = pair(0.0f, 0.0f);
     // weights are 2^(score - ref), ref = running maximum - (13 - ev): every value scale so far (the
     // largest is vbound, f16 bits) is below 2^ev, so that weight times scale is at most 2^13
-    float mx = kNever, ref = kNever, l = 0.0f;
+    float mx = kKv4Never, ref = kKv4Never, l = 0.0f;
     uint32_t vbound = 0u;
     int ev = 0;
 
@@ -481,8 +411,8 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
           for (int g = 0; g < NG; ++g) {
             float acc[4];
             const uint32_t w = kw[g], w8 = w >> 8;
-            mma_f16_new(acc, qh[g][0], ql[g][0], qh[g][1], ql[g][1], centre(w & 0x000f000fu, low_up), centre(w & 0x00f000f0u, high_up));
-            mma_f16(acc, qh[g][2], ql[g][2], qh[g][3], ql[g][3], centre(w8 & 0x000f000fu, low_up), centre(w8 & 0x00f000f0u, high_up));
+            mma_f16_new(acc, qh[g][0], ql[g][0], qh[g][1], ql[g][1], as_u32(centre_low(w)), as_u32(centre_high(w)));
+            mma_f16(acc, qh[g][2], ql[g][2], qh[g][3], ql[g][3], as_u32(centre_low(w8)), as_u32(centre_high(w8)));
             d = fma2(sc[g], add2(pair(acc[0], acc[1]), pair(acc[2], acc[3])), d);
           }
           const float2 y = unpair(fma2(d, pair(factor, factor), mul2(add2(pair(z[0], z[1]), pair(z[2], z[3])), pair(zfactor, zfactor))));
@@ -507,7 +437,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
           ev = ceil_exp2(__half2float(__ushort_as_half((unsigned short)vtop))) + 1;
           vbound = vtop;
         }
-        const float now = mx == kNever ? kNever : mx - (float)(13 - ev);
+        const float now = mx == kKv4Never ? kKv4Never : mx - (float)(13 - ev);
         const float al = exp2_fast(ref - now);
         ref = now;
         l *= al;
@@ -539,7 +469,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
             oz[g] = fma2(ww, mid[g], oz[g]);
-            split_weights(ww, sc[g], wh[g][j], wl[g][j]);
+            split_pair(mul2(ww, sc[g]), wh[g][j], wl[g][j]);
           }
         }
         // value codes of unit gid, rows in the same order
@@ -562,8 +492,8 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const uint32_t u0 = e ? t0 >> 8 : t0, u1 = e ? t1 >> 8 : t1;
-            const uint32_t a0 = centre(u0 & 0x000f000fu, low_up), a1 = centre(u0 & 0x00f000f0u, high_up);
-            const uint32_t a2 = centre(u1 & 0x000f000fu, low_up), a3 = centre(u1 & 0x00f000f0u, high_up);
+            const uint32_t a0 = as_u32(centre_low(u0)), a1 = as_u32(centre_high(u0));
+            const uint32_t a2 = as_u32(centre_low(u1)), a3 = as_u32(centre_high(u1));
             mma_f16(o[2 * g + e], a0, a1, a2, a3, wh[g][0], wh[g][1]);
             mma_f16(o[2 * g + e], a0, a1, a2, a3, wl[g][0], wl[g][1]);
           }
@@ -597,7 +527,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
       }
     }
     if (tig == 0) {
-      part[(warp * 8 + gid) * PART] = ref == kNever ? -INFINITY : ref;
+      part[(warp * 8 + gid) * PART] = ref == kKv4Never ? -INFINITY : ref;
       part[(warp * 8 + gid) * PART + 1] = l;
     }
     __syncthreads();

@@ -15,10 +15,16 @@
 // product overflows f16 whatever the scales of the rows, and the softmax's sum takes 2^-e back out.
 //
 // Warps: 0-3 softmax (a thread owns a row: its 64 scores come from tensor memory, its weights go back
-// there as the second product's A operand), 4-7 unpack keys and values into shared memory, 8 issues
-// the MMAs. Scores, weights, keys and values are double-buffered, so that S of the next 64 rows and O of
-// the last run while the softmax works. O stays in tensor memory; it is rescaled only when a row's
-// reference has to grow by more than 2^8, which the f16 range of the weights leaves room for.
+// to the same columns as the second product's A operand), 4-7 unpack keys and values into shared
+// memory, 8 issues the MMAs. Scores, keys and values are double-buffered, so that S of the next 64 rows
+// and O of the last run while the softmax works; the queries' high terms are an A operand in tensor
+// memory too, which spares shared memory most of the first product's reads. O stays in tensor memory; it
+// is rescaled only when a row's reference has to grow by more than 2^8, which the f16 range of the
+// weights leaves room for. The tensor core's f32 sums round toward 0, so every kPDrain steps the softmax
+// threads add O to a second accumulator, rounding to nearest, and the MMAs start afresh: without it the
+// error grows with the length (2.3e-5 of the result at 8700 positions; the exact values need 1e-6).
+// The roles' inner loops stay rolled at 16 columns: unrolled, four of five cycles went to instruction
+// fetches (four kinds of warps run different code).
 //
 // Work: the 64-row steps of all (tile, kv head) items, laid end to end, are cut into equal shares, one
 // persistent CTA an SM; an item that is cut leaves its parts (weighted values, reference, sum) in
@@ -35,7 +41,7 @@ constexpr int kPRows = 128;    // (position, head) pairs of a tile
 constexpr int kPKV = 64;       // cache rows of a step
 constexpr int kPThreads = 288;
 constexpr int kPTiles = 2048;  // tiles a launch (their step counts are in shared memory)
-constexpr float kNever = -3.0e38f;
+constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
 constexpr float kRoom = 8.0f, kHead = 6.0f;  // weights are 2^(score' - ref + 6), score' - ref <= 8
 
 template <int HD>
@@ -43,15 +49,21 @@ struct PromptShape {
   static constexpr int NG = HD / kKv4Group;
   static constexpr int KB = HD / 64;            // 64-channel blocks of the first product's depth
   static constexpr int NV = HD + 16;            // width of the second product
-  static constexpr uint32_t Q = 0;              // [2 terms][KB][128 rows][128 B]
-  static constexpr uint32_t QX = Q + 2 * KB * kPRows * 128;    // [128 rows][32 B]: query sums
-  static constexpr uint32_t K = QX + kPRows * 32;              // [2 buffers][2 terms][KB][64 rows][128 B]
+  static constexpr uint32_t QL = 0;             // [KB][128 rows][128 B]: low terms of the queries
+  static constexpr uint32_t K = QL + KB * kPRows * 128;        // [2 buffers][2 terms][KB][64 rows][128 B]
   static constexpr uint32_t KBUF = 2 * KB * kPKV * 128;
   static constexpr uint32_t V = K + 2 * KBUF;                  // [2 buffers][2 terms][NV rows][128 B]
   static constexpr uint32_t VBUF = 2 * NV * 128;
-  static constexpr uint32_t KX = V + 2 * VBUF;                 // [2 buffers][64 rows][32 B]: parameters
+  static constexpr uint32_t QX = V + 2 * VBUF;                 // [128 rows][32 B]: query sums
+  static constexpr uint32_t KX = QX + kPRows * 32;             // [2 buffers][64 rows][32 B]: parameters
   static constexpr uint32_t KXBUF = kPKV * 32;
-  static constexpr uint32_t ROW = KX + 2 * KXBUF;              // [4][5][64]: key scale, e, 2^-e, position, out of sight from
+  static constexpr uint32_t RAW = KX + 2 * KXBUF;              // [2 buffers] keys, values, their parameters as stored
+  static constexpr uint32_t RAWC = kPKV * HD / 2, RAWP = kPKV * 4 * NG;
+  static constexpr uint32_t RAWBUF = 2 * (RAWC + RAWP);
+  static constexpr uint32_t KS = RAW + 2 * RAWBUF;             // [64 rows][NG] f16: scaled key scales
+  static constexpr uint32_t VS = KS + kPKV * NG * 2;           // [NG][64 rows] f16: scaled value scales
+  static constexpr uint32_t VM = VS + kPKV * NG * 2;           // [2 terms][NG][64 rows] f16: scaled middles
+  static constexpr uint32_t ROW = VM + 2 * kPKV * NG * 2;      // [4][5][64]: key scale, e, 2^-e, position, out of sight from
   static constexpr uint32_t ROWBUF = 5 * kPKV * 4;
   static constexpr uint32_t FULL = ROW + 4 * ROWBUF;           // [4][2]: every query sees all of 32 rows
   static constexpr uint32_t BAR = FULL + 32;
@@ -60,8 +72,8 @@ struct PromptShape {
   static constexpr int PART = HD + 4;                          // of a row: reference, sum, 2 unused, weighted values
 };
 
-// tensor memory columns
-constexpr uint32_t kColS = 0, kColO = 128, kColP = 288, kCols = 512;
+// Tensor memory columns. Of each 16 columns of scores, 8 take the weights' high terms and 8 the low ones.
+constexpr uint32_t kColS = 0, kColO = 128, kColSum = 272, kColQ = 416, kCols = 512;
 
 enum Bar { B_QFULL = 0, B_KFULL = 1, B_KFREE = 3, B_VFULL = 5, B_VFREE = 7, B_SFULL = 9, B_PFULL = 11, B_PDONE = 13, B_END = 15 };
 
@@ -86,20 +98,12 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "f"(v[0]),
-               "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
-               : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -108,41 +112,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint4& r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // no use of the loaded values moves above the wait before this
-__device__ __forceinline__ void tmem_loaded32(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_loaded16(uint32_t (&r)[16]) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8)
+  for (int i = 0; i < 16; i += 8)
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_f16(a, b);
-  const float2 h = unpack_f16(hi);
-  lo = pack_f16(__fsub_rn(a, h.x), __fsub_rn(b, h.y));
-}
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-// least e with |x| <= 2^e, or one more (x a power of two); 0 and denormals as the least
-__device__ __forceinline__ int ceil_exp2(float x) { return (int)((__float_as_uint(x) >> 23) & 255u) - 126; }
-
-__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
-
-// The four pairs of codes of a word under the two masks, times their scales: (c - 7.5) 2^-9 is exact, and
-// so is its product with an f16 scale in two terms.
-__device__ __forceinline__ void unpack_pair(uint32_t w, bool high, __half2 s, uint32_t& hi, uint32_t& lo) {
-  const __half2 up = high ? __floats2half2_rn(2048.0f, 2048.0f) : __floats2half2_rn(32768.0f, 32768.0f);
-  const __half2 c = __hfma2(as_half2(w & (high ? 0x00f000f0u : 0x000f000fu)), up, __floats2half2_rn(-7.5f / 512, -7.5f / 512));
+// Two centred codes times their scales: the product is exact in two f16 terms.
+__device__ __forceinline__ void scale_pair(__half2 c, __half2 s, uint32_t& hi, uint32_t& lo) {
   const __half2 h = __hmul2(s, c);
   hi = as_u32(h);
   lo = as_u32(__hfma2(s, c, __hneg2(h)));
@@ -168,17 +151,6 @@ struct RowParams {
     e = max(ceil_exp2(top), -40) - 9;
   }
 };
-
-template <int NG>
-__device__ __forceinline__ void load_row_params(const __half* p, bool ok, uint32_t (&w)[NG]) {
-  if constexpr (NG == 4) {
-    const uint4 v = ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0u, 0u, 0u, 0u);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else {
-    const uint2 v = ok ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0u, 0u);
-    w[0] = v.x; w[1] = v.y;
-  }
-}
 
 struct PromptArgs {
   Kv4AttnArgs a;
@@ -316,7 +288,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       const bool live = r < (int64_t)a.M * G;
       const int m = live ? (int)(r / G) : a.M - 1, hq = sg.head * G + (live ? (int)(r % G) : 0);
       const int p = a.pos0 + m;
-      // the row's queries as two terms of q * 2^k, |q| 2^k <= 2^7, channels in the order of the key words
+      // the row's queries as two terms of q * 2^k, |q| 2^k < 2^7, channels in the order of the key words
       float rowf;
       {
         const float* q = a.q + (size_t)m * a.ldq + (size_t)hq * HD;
@@ -334,7 +306,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         const int k = max(min(7 - ceil_exp2(top), 100), -100);
         const float up = live ? pow2i(k) : 0.0f;
         rowf = a.scale * 1.44269504088896341f * pow2i(-k);
-#pragma unroll
+#pragma unroll 2
         for (int x = 0; x < HD / 8; ++x) {
           const float4 u = *reinterpret_cast<const float4*>(q + 8 * x), v = *reinterpret_cast<const float4*>(q + 8 * x + 4);
           uint4 hi, lo;
@@ -342,13 +314,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           split_f16(u.y * up, v.y * up, hi.y, lo.y);
           split_f16(u.z * up, v.z * up, hi.z, lo.z);
           split_f16(u.w * up, v.w * up, hi.w, lo.w);
-          const uint32_t at = SH::Q + (x >> 3) * (kPRows * 128) + sw128_offset(row, (x & 7) * 8);
-          *reinterpret_cast<uint4*>(smem + at) = hi;
-          *reinterpret_cast<uint4*>(smem + at + KB * kPRows * 128) = lo;
+          tmem_st4(t_row + kColQ + 4 * x, hi);
+          *reinterpret_cast<uint4*>(smem + SH::QL + (x >> 3) * (kPRows * 128) + sw128_offset(row, (x & 7) * 8)) = lo;
         }
-        uint32_t h[8], l[8];  // 7.5 x and 1 x the groups' sums
+        uint32_t h[4], l[4];  // 7.5 x and 1 x the groups' sums
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = l[i] = 0u;
+        for (int i = 0; i < 4; ++i) h[i] = l[i] = 0u;
 #pragma unroll
         for (int g = 0; g < NG; g += 2) {
           split_f16(qs[g] * up * 7.5f, qs[g + 1] * up * 7.5f, h[g / 2], l[g / 2]);
@@ -357,11 +328,16 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(row, 0)) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(row, 1)) = make_uint4(l[0], l[1], l[2], l[3]);
       }
+      tmem_wait_st();
+      tc_fence_before();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar + B_QFULL);
 
-      float ref = kNever, l = 0.0f;
+      const uint64_t rowf2 = pair(rowf, rowf);
+      float ref = kKv4Never;
+      uint64_t l2 = pair(0.0f, 0.0f);
+      bool summed = false;  // the second accumulator holds something
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
         const int b = it & 1;
         if (!(ok = wait(B_SFULL + b, (it >> 1) & 1))) break;
@@ -369,74 +345,97 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         const float* rp = reinterpret_cast<const float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF);
         const int* full = reinterpret_cast<const int*>(smem + SH::FULL) + (it & 3) * 2;
         const bool masked = !(full[0] && full[1]);
-        float x[kPKV];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t v[32];
-          tmem_ld32(t_row + kColS + b * kPKV + 32 * h, v);
+        const uint32_t t_s = t_row + kColS + b * kPKV;
+        // score + e in log2 units, back to the same columns, and the row's maximum
+        float top = -INFINITY;
+#pragma unroll 1
+        for (int i = 0; i < kPKV; i += 16) {
+          uint32_t v[16];
+          tmem_ld16(t_s + i, v);
           tmem_wait_ld();
-          tmem_loaded32(v);
+          tmem_loaded16(v);
+          float x[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 kf = *reinterpret_cast<const float4*>(rp + 32 * h + i), ve = *reinterpret_cast<const float4*>(rp + 64 + 32 * h + i);
-            x[32 * h + i] = fmaf(__uint_as_float(v[i]) * rowf, kf.x, ve.x);
-            x[32 * h + i + 1] = fmaf(__uint_as_float(v[i + 1]) * rowf, kf.y, ve.y);
-            x[32 * h + i + 2] = fmaf(__uint_as_float(v[i + 2]) * rowf, kf.z, ve.z);
-            x[32 * h + i + 3] = fmaf(__uint_as_float(v[i + 3]) * rowf, kf.w, ve.w);
+          for (int y = 0; y < 16; y += 4) {
+            const ulonglong2 kf = *reinterpret_cast<const ulonglong2*>(rp + i + y), ve = *reinterpret_cast<const ulonglong2*>(rp + 64 + i + y);
+            const float2 x0 = unpair(fma2(mul2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), rowf2), kf.x, ve.x));
+            const float2 x1 = unpair(fma2(mul2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), rowf2), kf.y, ve.y));
+            x[y] = x0.x; x[y + 1] = x0.y; x[y + 2] = x1.x; x[y + 3] = x1.y;
           }
-        }
-        if (masked) {
-          const int* at = reinterpret_cast<const int*>(rp + 3 * kPKV);
+          if (masked) {
+            const int* at = reinterpret_cast<const int*>(rp + 3 * kPKV) + i;
 #pragma unroll
-          for (int i = 0; i < kPKV; ++i)
-            if (!(at[i] <= p && p < at[kPKV + i])) x[i] = -INFINITY;
-        }
-        float top = x[0];
+            for (int y = 0; y < 16; ++y)
+              if (!(at[y] <= p && p < at[kPKV + y])) x[y] = -INFINITY;
+          }
 #pragma unroll
-        for (int i = 1; i < kPKV; ++i) top = fmaxf(top, x[i]);
-        if (__any_sync(0xffffffffu, top > ref + kRoom)) {
-          const float now = fmaxf(ref, top), al = exp2_fast(ref - now);
+          for (int y = 0; y < 16; y += 2) top = fmaxf(top, fmaxf(x[y], x[y + 1]));
+#pragma unroll
+          for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(x[y]);
+          tmem_st16(t_s + i, v);
+        }
+        float al = 1.0f;
+        const bool grow = __any_sync(0xffffffffu, top > ref + kRoom);
+        if (grow) {
+          const float now = fmaxf(ref, top);
+          al = exp2_fast(ref - now);
           ref = now;
-          l *= al;
-          if (j > sg.begin) {  // O holds the sums of the steps before: the last of them has to be complete
-            if (!(ok = wait(B_PDONE + (b ^ 1), ((it - 1) >> 1) & 1))) break;
-            tc_fence_after();
-#pragma unroll
-            for (int h = 0; h < SH::NV / 16; ++h) {
-              float v[2][8];
-              tmem_ld8(t_row + kColO + 16 * h, v[0]);
-              tmem_ld8(t_row + kColO + 16 * h + 8, v[1]);
-              tmem_wait_ld();
-              tmem_loaded(v[0]);
-              tmem_loaded(v[1]);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i / 8][i % 8] *= al;
-              tmem_st8(t_row + kColO + 16 * h, v[0]);
-              tmem_st8(t_row + kColO + 16 * h + 8, v[1]);
-            }
-          }
+          l2 = mul2(l2, pair(al, al));
         }
-        // the weights' buffer was last read by the step before the last
-        if (j >= sg.begin + 2 && !(ok = wait(B_PDONE + b, ((it - 2) >> 1) & 1))) break;
-        const float shift = kHead - ref;
+        tmem_wait_st();
+        // weights as two f16 terms, over the scores; their sum without the rows' powers of two
+        const uint64_t shift = pair(kHead - ref, kHead - ref);
+#pragma unroll 1
+        for (int i = 0; i < kPKV; i += 16) {
+          uint32_t v[16], w[16];
+          tmem_ld16(t_s + i, v);
+          tmem_wait_ld();
+          tmem_loaded16(v);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 ie = *reinterpret_cast<const float4*>(rp + 128 + 32 * h + i);
-            float w[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) w[y] = exp2_fast(x[32 * h + i + y] + shift);
-            l = fmaf(w[0], ie.x, l);
-            l = fmaf(w[1], ie.y, l);
-            l = fmaf(w[2], ie.z, l);
-            l = fmaf(w[3], ie.w, l);
-            split_f16(w[0], w[1], hi[i / 2], lo[i / 2]);
-            split_f16(w[2], w[3], hi[i / 2 + 1], lo[i / 2 + 1]);
+          for (int y = 0; y < 16; y += 4) {
+            const ulonglong2 ie = *reinterpret_cast<const ulonglong2*>(rp + 128 + i + y);
+            const float2 x0 = unpair(add2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), shift));
+            const float2 x1 = unpair(add2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), shift));
+            const uint64_t w0 = pair(exp2_fast(x0.x), exp2_fast(x0.y)), w1 = pair(exp2_fast(x1.x), exp2_fast(x1.y));
+            l2 = fma2(w0, ie.x, l2);
+            l2 = fma2(w1, ie.y, l2);
+            split_pair(w0, w[y / 2], w[8 + y / 2]);
+            split_pair(w1, w[y / 2 + 1], w[8 + y / 2 + 1]);
           }
-          tmem_st16(t_row + kColP + b * 64 + 16 * h, hi);
-          tmem_st16(t_row + kColP + b * 64 + 32 + 16 * h, lo);
+          tmem_st16(t_s + i, w);
+        }
+        // every kPDrain steps the sums so far go to the second accumulator; both follow the reference
+        const int step = j - sg.begin;
+        const bool drain = step > 0 && step % kPDrain == 0;
+        if (step > 0 && (drain || grow)) {
+          if (!(ok = wait(B_PDONE + (b ^ 1), ((it - 1) >> 1) & 1))) break;
+          tc_fence_after();
+          const uint64_t al2 = pair(al, al);
+#pragma unroll 1
+          for (int i = 0; i < SH::NV; i += 16) {
+            uint32_t o[16], s[16];
+            tmem_ld16(t_row + kColO + i, o);
+            if (summed) tmem_ld16(t_row + kColSum + i, s);
+            tmem_wait_ld();
+            tmem_loaded16(o);
+            if (summed) {
+              tmem_loaded16(s);
+            } else {
+#pragma unroll
+              for (int y = 0; y < 16; ++y) s[y] = 0u;
+            }
+#pragma unroll
+            for (int y = 0; y < 16; y += 2) {
+              uint64_t ov = pair(__uint_as_float(o[y]), __uint_as_float(o[y + 1])), sv = pair(__uint_as_float(s[y]), __uint_as_float(s[y + 1]));
+              if (drain) sv = add2(sv, ov);
+              const float2 so = unpair(mul2(sv, al2)), oo = unpair(mul2(ov, al2));
+              s[y] = __float_as_uint(so.x); s[y + 1] = __float_as_uint(so.y);
+              o[y] = __float_as_uint(oo.x); o[y + 1] = __float_as_uint(oo.y);
+            }
+            if (summed || drain) tmem_st16(t_row + kColSum + i, s);
+            if (!drain) tmem_st16(t_row + kColO + i, o);
+          }
+          summed |= drain;
         }
         tmem_wait_st();
         tc_fence_before();
@@ -448,207 +447,274 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       // the row's result, or its part
       if (!(ok = wait(B_PDONE + ((it - 1) & 1), ((it - 1) >> 1) & 1))) break;
       tc_fence_after();
-      float zv[8];
-      tmem_ld8(t_row + kColO + HD, zv);
-      tmem_wait_ld();
-      tmem_loaded(zv);
+      const float2 lv = unpair(l2);
+      const float l = lv.x + lv.y, D = l == 0.0f ? 1.0f : l;
+      float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       const bool whole = sg.begin == 0 && sg.end == sg.steps;
       float* part = pa.parts + (((size_t)blockIdx.x * 2 + (t == t_begin ? 0 : 1)) * kPRows + row) * SH::PART;
       const size_t out_at = (size_t)m * a.H * HD + (size_t)hq * HD;
-      const float D = l == 0.0f ? 1.0f : l;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        uint32_t v[32];
-        tmem_ld32(t_row + kColO + 32 * g, v);
+#pragma unroll 1
+      for (int x = SH::NV / 16 - 1; x >= 0; --x) {  // the minima's columns first
+        const int i = 16 * x;
+        uint32_t o[16], s[16];
+        tmem_ld16(t_row + kColO + i, o);
+        if (summed) tmem_ld16(t_row + kColSum + i, s);
         tmem_wait_ld();
-        tmem_loaded32(v);
-        if (!live) continue;
+        tmem_loaded16(o);
+        float y[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 y = make_float4(__uint_as_float(v[i]) + zv[g], __uint_as_float(v[i + 1]) + zv[g],
-                                 __uint_as_float(v[i + 2]) + zv[g], __uint_as_float(v[i + 3]) + zv[g]);
+        for (int n = 0; n < 16; ++n) y[n] = __uint_as_float(o[n]);
+        if (summed) {
+          tmem_loaded16(s);
+#pragma unroll
+          for (int n = 0; n < 16; ++n) y[n] += __uint_as_float(s[n]);
+        }
+        if (i == HD) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) z[n] = y[n];
+          continue;
+        }
+        if (!live) continue;
+        const int g = i / 32;
+        const float zg = g == 0 ? z[0] : g == 1 ? z[1] : g == 2 ? z[2] : z[3];
+#pragma unroll
+        for (int n = 0; n < 16; n += 4) {
+          const float4 f = make_float4(y[n] + zg, y[n + 1] + zg, y[n + 2] + zg, y[n + 3] + zg);
           if (whole) {
-            const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + out_at + 32 * g + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(a.out_c + out_at + 32 * g + i) =
-                make_float4(__fsub_rn(__fdiv_rn(y.x, D), mk.x), __fsub_rn(__fdiv_rn(y.y, D), mk.y),
-                            __fsub_rn(__fdiv_rn(y.z, D), mk.z), __fsub_rn(__fdiv_rn(y.w, D), mk.w));
-            *reinterpret_cast<float4*>(a.out_s + out_at + 32 * g + i) = mk;
+            const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + out_at + i + n) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(a.out_c + out_at + i + n) =
+                make_float4(__fsub_rn(__fdiv_rn(f.x, D), mk.x), __fsub_rn(__fdiv_rn(f.y, D), mk.y),
+                            __fsub_rn(__fdiv_rn(f.z, D), mk.z), __fsub_rn(__fdiv_rn(f.w, D), mk.w));
+            *reinterpret_cast<float4*>(a.out_s + out_at + i + n) = mk;
           } else {
-            *reinterpret_cast<float4*>(part + 4 + 32 * g + i) = y;
+            *reinterpret_cast<float4*>(part + 4 + i + n) = f;
           }
         }
       }
-      if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(ref == kNever ? -INFINITY : ref, l);
+      if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(ref == kKv4Never ? -INFINITY : ref, l);
       tc_fence_before();
       t += sg.end - sg.begin;
     }
   } else if (warp < 8) {
     // ---- unpacking ----------------------------------------------------------------------------
     const int th = tid - 128, w4 = warp - 4;
-    int it = 0;
-    bool ok = true;
-    for (int64_t t = t_begin; ok && t < t_end;) {
-      const Segment sg = find_segment(pre, pa.tiles, sum, c.heads, t, t_end);
-      int lo, hi;
-      tile_positions(a, sg.tile, G, lo, hi);
-      const Kv4Spans sp = kv4_spans(c, lo, hi, a.window);
-      const size_t base = kv4_base(c, a.slot0, sg.head);
-      // what row r of step j holds: its cache row, whether any query of the tile sees it, from which
-      // position on and until which
-      auto locate = [&](int j, int r, int& row, int& from, int& until) -> bool {
-        const int x = j * (kPKV / kKv4Chunk) + r / kKv4Chunk;
-        row = 0;
-        from = 0x7fffffff;
-        until = 0;
-        if (x >= sp.total) return false;
-        row = kv4_span_chunk(sp, x) * kKv4Chunk + r % kKv4Chunk;
-        const int at = kv4_held(c, row, last);
-        if (row >= c.sinks && at < c.sinks) return false;
-        const int64_t end = a.window > 0 && row >= c.sinks ? (int64_t)at + a.window : 0x7fffffff;
-        if (at > hi || end <= lo) return false;
-        from = at;
-        until = (int)min(end, (int64_t)0x7fffffff);
-        return true;
-      };
-      // keys: thread -> row th % 64, words 2 (th / 64), + 1 of every group
-      const int kr = th & 63, kh = th >> 6;
-      uint32_t kw[2 * NG], kpw[NG], kvw[NG];
-      int kfrom, kuntil;
-      auto load_keys = [&](int j) {
-        int row;
-        const bool in = locate(j, kr, row, kfrom, kuntil);
-        const uint8_t* src = c.kc + (base + row) * (HD / 2) + kh * (HD / 4);
-        if constexpr (NG == 4) {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(src)), y = __ldg(reinterpret_cast<const uint4*>(src) + 1);
-          kw[0] = x.x; kw[1] = x.y; kw[2] = x.z; kw[3] = x.w;
-          kw[4] = y.x; kw[5] = y.y; kw[6] = y.z; kw[7] = y.w;
-        } else {
-          const uint4 x = __ldg(reinterpret_cast<const uint4*>(src));
-          kw[0] = x.x; kw[1] = x.y; kw[2] = x.z; kw[3] = x.w;
+    // a walk over the CTA's steps
+    struct Walk {
+      int64_t t;
+      Segment sg;
+      Kv4Spans sp;
+      size_t base;
+      int lo, hi, j;
+    };
+    auto enter = [&](Walk& w) {
+      if (w.t >= t_end) return;
+      w.sg = find_segment(pre, pa.tiles, sum, c.heads, w.t, t_end);
+      tile_positions(a, w.sg.tile, G, w.lo, w.hi);
+      w.sp = kv4_spans(c, w.lo, w.hi, a.window);
+      w.base = kv4_base(c, a.slot0, w.sg.head);
+      w.j = w.sg.begin;
+    };
+    auto advance = [&](Walk& w) {
+      ++w.t;
+      if (++w.j == w.sg.end) enter(w);
+    };
+    // asynchronous copies of a step's rows as they are stored: warp w4 copies its w4-th chunk
+    constexpr int CPR = HD / 32, NC = kKv4Chunk * CPR, NP = kKv4Chunk * 4 * NG / 16;
+    auto fetch = [&](const Walk& w, int buf) {
+      const int x = w.j * (kPKV / kKv4Chunk) + w4;
+      if (w.t < t_end && x < w.sp.total) {
+        const size_t row0 = w.base + (size_t)kv4_span_chunk(w.sp, x) * kKv4Chunk;
+        uint8_t* raw = smem + SH::RAW + buf * SH::RAWBUF;
+#pragma unroll
+        for (int i = 0; i < NC / 32; ++i) {
+          const int y = lane + 32 * i, r = w4 * kKv4Chunk + y / CPR, q = y % CPR;
+          const uint32_t at = (uint32_t)(r * CPR + (HD == 128 ? q ^ ((r >> 1) & 3) : q)) * 16;
+          cp_async16(raw + at, c.kc + row0 * (HD / 2) + y * 16, 16);
+          cp_async16(raw + SH::RAWC + at, c.vc + row0 * (HD / 2) + y * 16, 16);
         }
-        load_row_params<NG>(c.kp + (base + row) * (2 * NG), in, kpw);
-        load_row_params<NG>(c.vp + (base + row) * (2 * NG), in, kvw);
-      };
-      // values: thread -> rows 2 lane, + 1, units 2 w4, + 1
-      uint32_t vw[2][NG], vpw[2][NG];
-      auto load_values = [&](int j) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          int row, from, until;
-          const bool in = locate(j, 2 * lane + x, row, from, until);
-          const uint8_t* src = c.vc + (base + row) * (HD / 2) + w4 * (HD / 8);
-          if constexpr (NG == 4) {
-            const uint4 y = __ldg(reinterpret_cast<const uint4*>(src));
-            vw[x][0] = y.x; vw[x][1] = y.y; vw[x][2] = y.z; vw[x][3] = y.w;
-          } else {
-            const uint2 y = __ldg(reinterpret_cast<const uint2*>(src));
-            vw[x][0] = y.x; vw[x][1] = y.y;
-          }
-          load_row_params<NG>(c.vp + (base + row) * (2 * NG), in, vpw[x]);
+        if (lane < 2 * NP) {
+          const bool v = lane >= NP;
+          const int y = v ? lane - NP : lane;
+          cp_async16(raw + 2 * SH::RAWC + (v ? SH::RAWP : 0) + w4 * (kKv4Chunk * 4 * NG) + y * 16,
+                     reinterpret_cast<const uint8_t*>(v ? c.vp : c.kp) + row0 * (4 * NG) + y * 16, 16);
         }
-      };
-      load_keys(sg.begin);
-      for (int j = sg.begin; j < sg.end; ++j, ++it) {
-        const int b = it & 1;
-        load_values(j);
-        // keys
-        if (it >= 2 && !(ok = wait(B_KFREE + b, ((it - 2) >> 1) & 1))) break;
-        {
-          RowParams<NG> k;
-          k.set(kpw, false);
-          const float down = pow2i(-k.e);
-          uint8_t* kb = smem + SH::K + b * SH::KBUF;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const __half2 s = __half2half2(__float2half_rn(k.s[g] * down * 512.0f));
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint32_t w = kw[x * NG + g], w8 = w >> 8;
-              uint4 h, l;
-              unpack_pair(w, false, s, h.x, l.x);
-              unpack_pair(w, true, s, h.y, l.y);
-              unpack_pair(w8, false, s, h.z, l.z);
-              unpack_pair(w8, true, s, h.w, l.w);
-              const uint32_t at = (g >> 1) * (kPKV * 128) + sw128_offset(kr, (g & 1) * 32 + (2 * kh + x) * 8);
-              *reinterpret_cast<uint4*>(kb + at) = h;
-              *reinterpret_cast<uint4*>(kb + KB * kPKV * 128 + at) = l;
-            }
-          }
-          if (kh == 0) {
-            uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int g = 0; g < NG; g += 2) {
-              w[g / 2] = pack_f16(k.s[g] * down, k.s[g + 1] * down);
-              w[NG / 2 + g / 2] = pack_f16(k.z[g] * down, k.z[g + 1] * down);
-            }
-            uint8_t* kx = smem + SH::KX + b * SH::KXBUF;
-            *reinterpret_cast<uint4*>(kx + plain16_offset(kr, 0)) = make_uint4(w[0], w[1], w[2], w[3]);
-            *reinterpret_cast<uint4*>(kx + plain16_offset(kr, 1)) = make_uint4(w[0], w[1], w[2], w[3]);
-            RowParams<NG> v;
-            v.set(kvw, true);
-            float* rp = reinterpret_cast<float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF);
-            rp[kr] = pow2i(k.e);
-            rp[64 + kr] = (float)v.e;
-            rp[128 + kr] = pow2i(-v.e);
-            reinterpret_cast<int*>(rp)[192 + kr] = kfrom;
-            reinterpret_cast<int*>(rp)[256 + kr] = kuntil;
-            const int full = __all_sync(0xffffffffu, kfrom <= lo && hi < kuntil);
-            if (lane == 0) reinterpret_cast<int*>(smem + SH::FULL)[(it & 3) * 2 + w4] = full;
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar + B_KFULL + b);
-        if (j + 1 < sg.end) load_keys(j + 1);
-        // values
-        if (it >= 2 && !(ok = wait(B_VFREE + b, ((it - 2) >> 1) & 1))) break;
-        {
-          RowParams<NG> v0, v1;
-          v0.set(vpw[0], true);
-          v1.set(vpw[1], true);
-          const float d0 = pow2i(-v0.e), d1 = pow2i(-v1.e);
-          uint8_t* vb = smem + SH::V + b * SH::VBUF;
-          const uint32_t col = (uint32_t)(lane >> 2) , in = (uint32_t)(lane & 3) * 4;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const __half2 s = __floats2half2_rn(v0.s[g] * d0 * 512.0f, v1.s[g] * d1 * 512.0f);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {  // unit 2 w4 + x: half word x NG + g of this warp's share
-              const int hw = x * NG + g;
-              const uint32_t w = __byte_perm(vw[0][hw / 2], vw[1][hw / 2], (hw & 1) ? 0x7632 : 0x5410), w8 = w >> 8;
-              const int ch = 32 * g + 4 * (2 * w4 + x);
-              uint32_t h[4], l[4];
-              unpack_pair(w, false, s, h[0], l[0]);
-              unpack_pair(w, true, s, h[1], l[1]);
-              unpack_pair(w8, false, s, h[2], l[2]);
-              unpack_pair(w8, true, s, h[3], l[3]);
-#pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                const uint32_t at = (uint32_t)((ch + n) >> 3) * 1024u + (uint32_t)((ch + n) & 7) * 128u + ((col ^ (uint32_t)((ch + n) & 7)) << 4) + in;
-                *reinterpret_cast<uint32_t*>(vb + at) = h[n];
-                *reinterpret_cast<uint32_t*>(vb + SH::NV * 128 + at) = l[n];
-              }
-            }
-          }
-          if (w4 < NG) {  // the minima: column HD + w4
-            float m0 = v0.z[0], m1 = v1.z[0];
-#pragma unroll
-            for (int g = 1; g < NG; ++g)
-              if (w4 == g) { m0 = v0.z[g]; m1 = v1.z[g]; }
-            uint32_t h, l;
-            split_f16(m0 * d0, m1 * d1, h, l);
-            const int ch = HD + w4;
-            const uint32_t at = (uint32_t)(ch >> 3) * 1024u + (uint32_t)(ch & 7) * 128u + ((col ^ (uint32_t)(ch & 7)) << 4) + in;
-            *reinterpret_cast<uint32_t*>(vb + at) = h;
-            *reinterpret_cast<uint32_t*>(vb + SH::NV * 128 + at) = l;
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar + B_VFULL + b);
       }
-      t += sg.end - sg.begin;
+      cp_async_commit();
+    };
+    bool ok = true;
+    Walk at{}, ahead{};
+    at.t = ahead.t = t_begin;
+    enter(at);
+    enter(ahead);
+    if (t_begin < t_end) {
+      fetch(ahead, 0);
+      advance(ahead);
     }
+    for (int it = 0; at.t < t_end; ++it) {
+      const int b = it & 1;
+      const uint8_t* raw = smem + SH::RAW + b * SH::RAWBUF;
+      cp_async_wait<0>();
+      named_bar_sync(1, 128);  // this step's rows have landed, and nobody reads the last step's
+      fetch(ahead, b ^ 1);
+      advance(ahead);
+      // after a wait that ran out the walk goes on without waiting: the four warps meet at their barriers
+      ok = ok && (it < 2 || wait(B_KFREE + b, ((it - 2) >> 1) & 1));
+      // one row a thread: keys 0-63, values 64-127
+      {
+        const int r = th & 63;
+        const bool vals = th >= 64;
+        // whether any query of the tile sees the row: at positions [from, until)
+        int from = 0x7fffffff, until = 0;
+        const int x = at.j * (kPKV / kKv4Chunk) + r / kKv4Chunk;
+        if (x < at.sp.total) {
+          const int row = kv4_span_chunk(at.sp, x) * kKv4Chunk + r % kKv4Chunk;
+          const int held = kv4_held(c, row, last);
+          const int64_t end = a.window > 0 && row >= c.sinks ? (int64_t)held + a.window : 0x7fffffff;
+          if ((row < c.sinks || held >= c.sinks) && held <= at.hi && end > at.lo) {
+            from = held;
+            until = (int)min(end, (int64_t)0x7fffffff);
+          }
+        }
+        uint32_t w[NG];
+        const uint8_t* src = raw + 2 * SH::RAWC + (vals ? SH::RAWP : 0) + r * (4 * NG);
+        if constexpr (NG == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(src);
+          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(src);
+          w[0] = v.x; w[1] = v.y;
+        }
+        if (until == 0) {
+#pragma unroll
+          for (int g = 0; g < NG; ++g) w[g] = 0u;
+        }
+        RowParams<NG> q;
+        q.set(w, vals);
+        const float down = pow2i(-q.e), up9 = down * 512.0f;
+        float* rp = reinterpret_cast<float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF);
+        if (!vals) {
+          uint32_t s[NG / 2], y[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int g = 0; g < NG; g += 2) {
+            s[g / 2] = pack_f16(q.s[g] * up9, q.s[g + 1] * up9);
+            y[g / 2] = pack_f16(q.s[g] * down, q.s[g + 1] * down);
+            y[NG / 2 + g / 2] = pack_f16(q.z[g] * down, q.z[g + 1] * down);
+          }
+          if constexpr (NG == 4)
+            *reinterpret_cast<uint2*>(smem + SH::KS + r * 8) = make_uint2(s[0], s[1]);
+          else
+            *reinterpret_cast<uint32_t*>(smem + SH::KS + r * 4) = s[0];
+          uint8_t* kx = smem + SH::KX + b * SH::KXBUF;
+          *reinterpret_cast<uint4*>(kx + plain16_offset(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(kx + plain16_offset(r, 1)) = make_uint4(y[0], y[1], y[2], y[3]);
+          rp[r] = pow2i(q.e);
+          reinterpret_cast<int*>(rp)[192 + r] = from;
+          reinterpret_cast<int*>(rp)[256 + r] = until;
+          const int full = __all_sync(0xffffffffu, from <= at.lo && at.hi < until);
+          if (lane == 0) reinterpret_cast<int*>(smem + SH::FULL)[(it & 3) * 2 + w4] = full;
+        } else {
+          rp[64 + r] = (float)q.e;
+          rp[128 + r] = pow2i(-q.e);
+          __half *vs = reinterpret_cast<__half*>(smem + SH::VS), *vm = reinterpret_cast<__half*>(smem + SH::VM);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            vs[g * kPKV + r] = __float2half_rn(q.s[g] * up9);
+            const float y = q.z[g] * down;
+            const __half h = __float2half_rn(y);
+            vm[g * kPKV + r] = h;
+            vm[(NG + g) * kPKV + r] = __float2half_rn(__fsub_rn(y, __half2float(h)));
+          }
+        }
+      }
+      named_bar_sync(1, 128);
+      // keys: thread -> row th % 64, words 2 (th / 64), + 1 of every group
+      {
+        const int r = th & 63, kh = th >> 6;
+        uint8_t* kb = smem + SH::K + b * SH::KBUF;
+        uint32_t s[NG / 2];
+        if constexpr (NG == 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(smem + SH::KS + r * 8);
+          s[0] = v.x; s[1] = v.y;
+        } else {
+          s[0] = *reinterpret_cast<const uint32_t*>(smem + SH::KS + r * 4);
+        }
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+          const int u = 2 * kh + x;
+          uint32_t kw[NG];
+          if constexpr (NG == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
+            kw[0] = v.x; kw[1] = v.y; kw[2] = v.z; kw[3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(raw + r * 32 + u * 8);
+            kw[0] = v.x; kw[1] = v.y;
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const __half2 sv = (g & 1) ? __high2half2(as_half2(s[g / 2])) : __low2half2(as_half2(s[g / 2]));
+            const uint32_t w = kw[g], w8 = w >> 8;
+            uint4 h, l;
+            scale_pair(centre_low(w), sv, h.x, l.x);
+            scale_pair(centre_high(w), sv, h.y, l.y);
+            scale_pair(centre_low(w8), sv, h.z, l.z);
+            scale_pair(centre_high(w8), sv, h.w, l.w);
+            uint8_t* to = kb + (g >> 1) * (kPKV * 128) + sw128_offset(r, (g & 1) * 32 + u * 8);
+            *reinterpret_cast<uint4*>(to) = h;
+            *reinterpret_cast<uint4*>(to + KB * kPKV * 128) = l;
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar + B_KFULL + b);
+      ok = ok && (it < 2 || wait(B_VFREE + b, ((it - 2) >> 1) & 1));
+      // values, transposed: thread -> rows 2 lane, + 1, units 2 w4, + 1
+      {
+        uint8_t* vb = smem + SH::V + b * SH::VBUF;
+        const uint32_t col = (uint32_t)(lane >> 2), in = (uint32_t)(lane & 3) * 4;
+        const uint8_t* rv = raw + SH::RAWC;
+#pragma unroll 1
+        for (int x = 0; x < 2; ++x) {
+          const int u = 2 * w4 + x;
+          uint32_t va[NG / 2], vc[NG / 2];
+          if constexpr (NG == 4) {
+            const uint8_t* y = rv + lane * 128 + ((w4 ^ (lane & 3)) << 4) + x * 8;
+            const uint2 y0 = *reinterpret_cast<const uint2*>(y), y1 = *reinterpret_cast<const uint2*>(y + 64);
+            va[0] = y0.x; va[1] = y0.y; vc[0] = y1.x; vc[1] = y1.y;
+          } else {
+            va[0] = *reinterpret_cast<const uint32_t*>(rv + lane * 64 + u * 4);
+            vc[0] = *reinterpret_cast<const uint32_t*>(rv + lane * 64 + 32 + u * 4);
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const __half2 sv = *reinterpret_cast<const __half2*>(smem + SH::VS + g * (kPKV * 2) + lane * 4);
+            const uint32_t w = __byte_perm(va[g / 2], vc[g / 2], (g & 1) ? 0x7632 : 0x5410), w8 = w >> 8;
+            uint32_t h[4], l[4];
+            scale_pair(centre_low(w), sv, h[0], l[0]);
+            scale_pair(centre_high(w), sv, h[1], l[1]);
+            scale_pair(centre_low(w8), sv, h[2], l[2]);
+            scale_pair(centre_high(w8), sv, h[3], l[3]);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const int ch = 32 * g + 4 * u + n;  // its row in the swizzled tile; (ch & 7) = 4 x + n
+              uint8_t* to = vb + (uint32_t)(ch >> 3) * 1024u + (uint32_t)(4 * x + n) * 128u + ((col ^ (uint32_t)(4 * x + n)) << 4) + in;
+              *reinterpret_cast<uint32_t*>(to) = h[n];
+              *reinterpret_cast<uint32_t*>(to + SH::NV * 128) = l[n];
+            }
+          }
+        }
+        if (w4 < NG) {  // the middles of group w4
+          uint8_t* to = vb + (HD >> 3) * 1024 + w4 * 128 + ((col ^ (uint32_t)w4) << 4) + in;
+          *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(smem + SH::VM + w4 * (kPKV * 2) + lane * 4);
+          *reinterpret_cast<uint32_t*>(to + SH::NV * 128) = *reinterpret_cast<const uint32_t*>(smem + SH::VM + (NG + w4) * (kPKV * 2) + lane * 4);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar + B_VFULL + b);
+      advance(at);
+    }
+    cp_async_wait<0>();
   } else if (lane == 0) {
     // ---- MMAs -----------------------------------------------------------------------------------
     constexpr uint32_t ids = idesc_f16_f32(kPRows, kPKV), idv = idesc_f16_f32(kPRows, SH::NV);
@@ -660,18 +726,26 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       tc_fence_after();
       const uint32_t d = tbase + kColS + b * kPKV;
       const uint8_t* kb = smem + SH::K + b * SH::KBUF;
+      // small terms first: low high, high low, then the parameters and high high
 #pragma unroll
-      for (int p = 0; p < 3; ++p) {  // high high, high low, low high
-        const uint8_t* qa = smem + SH::Q + (p == 2 ? KB * kPRows * 128 : 0);
-        const uint8_t* ka = kb + (p == 1 ? KB * kPKV * 128 : 0);
+      for (int x = 0; x < KB; ++x) {
+        const uint64_t ad = smem_desc_sw128(smem + SH::QL + x * kPRows * 128), bd = smem_desc_sw128(kb + x * kPKV * 128);
 #pragma unroll
-        for (int x = 0; x < KB; ++x) {
-          const uint64_t ad = smem_desc_sw128(qa + x * kPRows * 128), bd = smem_desc_sw128(ka + x * kPKV * 128);
+        for (int k = 0; k < 4; ++k) tc_mma(d, ad + 2 * k, bd + 2 * k, ids, (x > 0 || k > 0) ? 1u : 0u);
+      }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma(d, ad + 2 * k, bd + 2 * k, ids, (p > 0 || x > 0 || k > 0) ? 1u : 0u);
-        }
+      for (int x = 0; x < KB; ++x) {
+        const uint64_t bd = smem_desc_sw128(kb + (KB + x) * kPKV * 128);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_ts(d, tbase + kColQ + 8 * (4 * x + k), bd + 2 * k, ids, 1u);
       }
       tc_mma(d, smem_desc_plain16(smem + SH::QX), smem_desc_plain16(smem + SH::KX + b * SH::KXBUF), ids, 1u);
+#pragma unroll
+      for (int x = 0; x < KB; ++x) {
+        const uint64_t bd = smem_desc_sw128(kb + x * kPKV * 128);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_ts(d, tbase + kColQ + 8 * (4 * x + k), bd + 2 * k, ids, 1u);
+      }
       tc_commit(bar + B_KFREE + b);
       tc_commit(bar + B_SFULL + b);
       return true;
@@ -688,13 +762,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         if (!(ok = wait_one(B_PFULL + b, (it >> 1) & 1))) break;
         tc_fence_after();
         const uint8_t* vb = smem + SH::V + b * SH::VBUF;
-        const uint32_t pcol = tbase + kColP + b * 64;
+        const uint32_t pcol = tbase + kColS + b * kPKV;
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
+        for (int p = 0; p < 3; ++p) {  // low high, high low, high high
           const uint64_t bd = smem_desc_sw128(vb + (p == 1 ? SH::NV * 128 : 0));
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            tc_mma_ts(tbase + kColO, pcol + (p == 2 ? 32 : 0) + 8 * k, bd + 2 * k, idv, (j > 0 || p > 0 || k > 0) ? 1u : 0u);
+            tc_mma_ts(tbase + kColO, pcol + (p == 0 ? 8 : 0) + 16 * k, bd + 2 * k, idv, (j % kPDrain > 0 || p > 0 || k > 0) ? 1u : 0u);
         }
         tc_commit(bar + B_VFREE + b);
         tc_commit(bar + B_PDONE + b);
