@@ -14,20 +14,20 @@
 // its own too, and its weight is 2^(score + e - ref): the running reference follows score + e, so no
 // product overflows f16 whatever the scales of the rows, and the softmax's sum takes 2^-e back out.
 //
-// Warps: 0-3 softmax (a thread owns a row: its 64 scores come from tensor memory, its weights go back
-// to the same columns as the second product's A operand), 4-7 unpack keys and values into shared
-// memory, 8 issues the MMAs. Scores, keys and values are double-buffered, so that S of the next 64 rows
-// and O of the last run while the softmax works; the queries' high terms are an A operand in tensor
-// memory too, which spares shared memory most of the first product's reads. O stays in tensor memory; it
-// is rescaled only when a row's reference has to grow by more than 2^8, which the f16 range of the
-// weights leaves room for. The tensor core's f32 sums round toward 0, so every kPDrain steps the softmax
-// threads add O to a second accumulator, rounding to nearest, and the MMAs start afresh: without it the
-// error grows with the length (2.3e-5 of the result at 8700 positions; the exact values need 1e-6).
-// The roles' inner loops stay rolled at 16 columns: unrolled, four of five cycles went to instruction
-// fetches (four kinds of warps run different code).
+// Warps: 0-7 softmax (two threads share a row, half of its 64 scores each: scores come from tensor
+// memory, weights go back to the same columns as the second product's A operand), 8-11 unpack keys and
+// 12-15 values into shared memory, 16 issues the MMAs. Scores, keys and values are double-buffered, so
+// that S of the next 64 rows and O of the last run while the softmax works; the queries' high terms are
+// an A operand in tensor memory too, which spares shared memory most of the first product's reads. A
+// value row is unpacked as it lies (the second product's B operand is the wide dimension's major). O
+// stays in tensor memory; it is rescaled only when a row's reference has to grow by more than 2^8, which
+// the f16 range of the weights leaves room for. The tensor core's f32 sums round toward 0, so every
+// kPDrain steps the softmax threads add O to a second accumulator, rounding to nearest, and the MMAs
+// start afresh: without it the error grows with the length (2.3e-5 of the result at 8700 positions; a
+// plain f32 evaluation is 1.9e-6 off).
 //
-// Work: the 64-row steps of all (tile, kv head) items, laid end to end, are cut into equal shares, one
-// persistent CTA an SM; an item that is cut leaves its parts (weighted values, reference, sum) in
+// Work: the 64-row steps of all (tile, kv head) items and kPItem for an item's start and end, laid end to
+// end, are cut into equal shares, one persistent CTA an SM; an item that is cut leaves its parts (weighted values, reference, sum) in
 // context scratch and a second kernel joins them.
 #include <cmath>
 
@@ -39,55 +39,69 @@ namespace {
 
 constexpr int kPRows = 128;    // (position, head) pairs of a tile
 constexpr int kPKV = 64;       // cache rows of a step
-constexpr int kPThreads = 288;
+constexpr int kPThreads = 544;
 constexpr int kPTiles = 2048;  // tiles a launch (their step counts are in shared memory)
+constexpr int kPItem = 3;      // cost of an item's queries and results, in steps
 constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
 constexpr float kRoom = 8.0f, kHead = 6.0f;  // weights are 2^(score' - ref + 6), score' - ref <= 8
 
 template <int HD>
 struct PromptShape {
   static constexpr int NG = HD / kKv4Group;
-  static constexpr int KB = HD / 64;            // 64-channel blocks of the first product's depth
-  static constexpr int NV = HD + 16;            // width of the second product
+  static constexpr int KB = HD / 64;            // 64-channel blocks
+  static constexpr int NV = HD + 16;            // columns of O: channels (see o_channel) and minima
   static constexpr uint32_t QL = 0;             // [KB][128 rows][128 B]: low terms of the queries
-  static constexpr uint32_t K = QL + KB * kPRows * 128;        // [2 buffers][2 terms][KB][64 rows][128 B]
-  static constexpr uint32_t KBUF = 2 * KB * kPKV * 128;
-  static constexpr uint32_t V = K + 2 * KBUF;                  // [2 buffers][2 terms][NV rows][128 B]
-  static constexpr uint32_t VBUF = 2 * NV * 128;
-  static constexpr uint32_t QX = V + 2 * VBUF;                 // [128 rows][32 B]: query sums
-  static constexpr uint32_t KX = QX + kPRows * 32;             // [2 buffers][64 rows][32 B]: parameters
+  static constexpr uint32_t QX = QL + KB * kPRows * 128;       // [128 rows][32 B]: query sums
+  static constexpr uint32_t K = QX + kPRows * 32;              // [2 buffers][2 terms][KB][64 rows][128 B]
+  static constexpr uint32_t BUF = 2 * KB * kPKV * 128;
+  static constexpr uint32_t V = K + 2 * BUF;                   // the same
+  static constexpr uint32_t KX = V + 2 * BUF;                  // [2 buffers][64 rows][32 B]: key parameters
   static constexpr uint32_t KXBUF = kPKV * 32;
-  static constexpr uint32_t RAW = KX + 2 * KXBUF;              // [2 buffers] keys, values, their parameters as stored
-  static constexpr uint32_t RAWC = kPKV * HD / 2, RAWP = kPKV * 4 * NG;
-  static constexpr uint32_t RAWBUF = 2 * (RAWC + RAWP);
-  static constexpr uint32_t KS = RAW + 2 * RAWBUF;             // [64 rows][NG] f16: scaled key scales
-  static constexpr uint32_t VS = KS + kPKV * NG * 2;           // [NG][64 rows] f16: scaled value scales
-  static constexpr uint32_t VM = VS + kPKV * NG * 2;           // [2 terms][NG][64 rows] f16: scaled middles
-  static constexpr uint32_t ROW = VM + 2 * kPKV * NG * 2;      // [4][5][64]: key scale, e, 2^-e, position, out of sight from
+  static constexpr uint32_t VX = KX + 2 * KXBUF;               // [2 buffers][64 rows / 8][16 columns][16 B]: value middles
+  static constexpr uint32_t VXBUF = kPKV * 32;
+  static constexpr uint32_t RAW = VX + 2 * VXBUF;              // [2 kinds][2 buffers] codes and parameters as stored
+  static constexpr uint32_t RAWC = kPKV * HD / 2, RAWBUF = RAWC + kPKV * 4 * NG;
+  static constexpr uint32_t ROW = RAW + 4 * RAWBUF;            // [4][5][64]: key scale, e, 2^-e, position, out of sight from
   static constexpr uint32_t ROWBUF = 5 * kPKV * 4;
   static constexpr uint32_t FULL = ROW + 4 * ROWBUF;           // [4][2]: every query sees all of 32 rows
-  static constexpr uint32_t BAR = FULL + 32;
-  static constexpr uint32_t PRE = BAR + 128;                   // [kPTiles] steps of the tiles before
+  static constexpr uint32_t RED = FULL + 32;                   // [3][2 halves][128]: maxima of even and odd steps, sums
+  static constexpr uint32_t RFAC = RED + 6 * kPRows * 4;       // [128] queries' scale
+  static constexpr uint32_t BAR = RFAC + kPRows * 4;
+  static constexpr uint32_t PRE = BAR + 256;                   // [kPTiles] cost of the tiles before
   static constexpr size_t SMEM = PRE + kPTiles * 4 + 1024;     // + alignment slack
   static constexpr int PART = HD + 4;                          // of a row: reference, sum, 2 unused, weighted values
+  static constexpr int SC = HD / 4;                            // channels of a row staged together on the way out
 };
 
 // Tensor memory columns. Of each 16 columns of scores, 8 take the weights' high terms and 8 the low ones.
 constexpr uint32_t kColS = 0, kColO = 128, kColSum = 272, kColQ = 416, kCols = 512;
 
-enum Bar { B_QFULL = 0, B_KFULL = 1, B_KFREE = 3, B_VFULL = 5, B_VFREE = 7, B_SFULL = 9, B_PFULL = 11, B_PDONE = 13, B_END = 15 };
+enum Bar { B_QFULL = 0, B_KFULL = 1, B_KFREE = 3, B_VFULL = 5, B_VFREE = 7, B_SFULL = 9, B_PFULL = 11, B_PDONE = 13, B_EFULL = 15, B_END = 19 };
 
 // D f32, A and B f16, both K-major
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// 16 columns (32 B a row) without swizzle: 8-row x 16-byte pieces of 128 bytes, the two of a row group
-// next to each other
-__device__ __forceinline__ uint64_t smem_desc_plain16(const void* p) {
-  return ((uint64_t)(smem_u32(p) & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 16) | ((uint64_t)(256 >> 4) << 32) | (1ull << 46);
+constexpr uint32_t kBWide = 1u << 16;  // B has its N dimension contiguous
+// Without swizzle, 8-row x 16-byte pieces of 128 bytes: `k` bytes from one 16 B of depth to the next, `n`
+// from one row group to the next.
+__device__ __forceinline__ uint64_t smem_desc_plain(const void* p, uint32_t k, uint32_t n) {
+  return ((uint64_t)(smem_u32(p) & 0x3FFFFu) >> 4) | ((uint64_t)(k >> 4) << 16) | ((uint64_t)(n >> 4) << 32) | (1ull << 46);
 }
+// 32 B of depth a row, the two pieces of a row group next to each other
 __device__ __forceinline__ uint32_t plain16_offset(int r, int half) { return (uint32_t)(r >> 3) * 256u + half * 128u + (r & 7) * 16u; }
+// N-contiguous operand with the 128-byte swizzle: rows of depth of 64 N elements, 8-row atoms 1024 bytes
+// apart, the next 64 N elements `n` bytes on
+__device__ __forceinline__ uint64_t smem_desc_wide128(const void* p, uint32_t n) {
+  return ((uint64_t)(smem_u32(p) & 0x3FFFFu) >> 4) | ((uint64_t)(n >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
 
+// One thread of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // D[tmem] (+)= A[tmem] * B[smem]^T
 __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -111,10 +125,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint4& r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
-               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // no use of the loaded values moves above the wait before this
@@ -164,19 +174,19 @@ __device__ __forceinline__ void tile_positions(const Kv4AttnArgs& a, int tile, i
   lo = a.pos0 + (int)((int64_t)tile * kPRows / G);
   hi = a.pos0 + min((int)(((int64_t)tile * kPRows + kPRows - 1) / G), a.M - 1);
 }
-__device__ __forceinline__ int tile_steps(const Kv4AttnArgs& a, int tile, int G) {
+__device__ __forceinline__ int tile_cost(const Kv4AttnArgs& a, int tile, int G) {
   int lo, hi;
   tile_positions(a, tile, G, lo, hi);
-  return (kv4_spans(a.c, lo, hi, a.window).total * kKv4Chunk + kPKV - 1) / kPKV;
+  return (kv4_spans(a.c, lo, hi, a.window).total * kKv4Chunk + kPKV - 1) / kPKV + kPItem;
 }
 
-// Steps of the tiles before each into pre[0 .. tiles), their sum returned; all threads of the block.
+// Costs of the tiles before each into pre[0 .. tiles), their sum returned; all threads of the block.
 __device__ __forceinline__ int plan_tiles(const Kv4AttnArgs& a, int tiles, int G, int* pre, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = blockDim.x, warps = n / 32;
   int sum = 0;
   for (int t0 = 0; t0 < tiles; t0 += n) {
     const int t = t0 + tid;
-    const int v = t < tiles ? tile_steps(a, t, G) : 0;
+    const int v = t < tiles ? tile_cost(a, t, G) : 0;
     int x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -196,9 +206,10 @@ __device__ __forceinline__ int plan_tiles(const Kv4AttnArgs& a, int tiles, int G
   return sum;
 }
 
-// A CTA's next stretch of one item.
+// A CTA's next stretch of one item: steps [begin, end) of its `steps` (maybe none), up to cost `next`.
 struct Segment {
-  int tile, head, begin, end, steps;  // steps [begin, end) of the item's `steps`
+  int tile, head, begin, end, steps;
+  int64_t item, next;
 };
 __device__ __forceinline__ Segment find_segment(const int* pre, int tiles, int sum, int heads, int64_t t, int64_t t_end) {
   int lo = 0, hi = tiles - 1;
@@ -208,13 +219,27 @@ __device__ __forceinline__ Segment find_segment(const int* pre, int tiles, int s
   }
   Segment s;
   s.tile = lo;
-  s.steps = (lo + 1 < tiles ? pre[lo + 1] : sum) - pre[lo];
-  const int64_t in = t - (int64_t)pre[lo] * heads;
-  s.head = (int)(in / s.steps);
-  s.begin = (int)(in - (int64_t)s.head * s.steps);
-  s.end = (int)min((int64_t)s.steps, s.begin + (t_end - t));
+  const int cost = (lo + 1 < tiles ? pre[lo + 1] : sum) - pre[lo], in = (int)(t - (int64_t)pre[lo] * heads);
+  s.steps = cost - kPItem;
+  s.head = in / cost;
+  s.item = (int64_t)pre[lo] * heads + (int64_t)s.head * cost;
+  s.next = min(s.item + cost, t_end);
+  s.begin = max((int)(t - s.item) - kPItem, 0);
+  s.end = max((int)(s.next - s.item) - kPItem, s.begin);
   return s;
 }
+// The first stretch from t on that has steps; false: none before t_end.
+__device__ __forceinline__ bool next_segment(Segment& s, const int* pre, int tiles, int sum, int heads, int64_t& t, int64_t t_end) {
+  while (t < t_end) {
+    s = find_segment(pre, tiles, sum, heads, t, t_end);
+    if (s.end > s.begin) return true;
+    t = s.next;
+  }
+  return false;
+}
+
+// O's columns: 8 u + 2 n + (g & 1) of block g / 2 is channel 32 g + 4 u + n, the order in which a word of
+// stored values unpacks.
 
 template <int HD>
 __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_constant__ PromptArgs pa) {
@@ -226,24 +251,25 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + SH::BAR);
   int* pre = reinterpret_cast<int*>(smem + SH::PRE);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   __shared__ uint32_t tmem_base;
   __shared__ int abort_word;
-  __shared__ int scratch[16];
+  __shared__ int scratch[32];
   volatile int* abort_flag = &abort_word;
 
   if (tid == 0) {
     abort_word = 0;
     for (int i = 0; i <= B_END; ++i) {
-      const bool four = i == B_QFULL || i == B_KFULL || i == B_KFULL + 1 || i == B_VFULL || i == B_VFULL + 1 || i == B_PFULL || i == B_PFULL + 1;
-      mbar_init(bar + i, four ? 4 : 1);
+      const bool eight = i == B_QFULL || i == B_PFULL || i == B_PFULL + 1;
+      const bool four = i == B_KFULL || i == B_KFULL + 1 || i == B_VFULL || i == B_VFULL + 1 || (i >= B_EFULL && i < B_EFULL + 4);
+      mbar_init(bar + i, eight ? 8 : four ? 4 : 1);
     }
     mbar_fence_init();
   }
-  if (warp == 8) tmem_alloc(&tmem_base, kCols);
-  // the columns of V past the minima are never written again
-  for (int i = tid; i < 4 * 16 * 128 / 16; i += kPThreads)
-    *reinterpret_cast<uint4*>(smem + SH::V + (i / 128) * (SH::NV * 128) + HD * 128 + (i % 128) * 16) = make_uint4(0u, 0u, 0u, 0u);
+  if (warp == 16) tmem_alloc(&tmem_base, kCols);
+  // the middles' columns past 2 NG are never written again
+  for (int i = tid; i < 2 * SH::VXBUF / 16; i += kPThreads)
+    *reinterpret_cast<uint4*>(smem + SH::VX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
   fence_proxy_async_smem();
   pdl_trigger();
   pdl_wait();
@@ -276,143 +302,166 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
   // The same for a whole warp.
   auto wait = [&](int b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait_one(b, parity)); };
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ---- softmax ------------------------------------------------------------------------------
-    const int row = tid;
-    const uint32_t t_row = tbase + ((uint32_t)(warp * 32) << 16);
+    // After a wait that ran out the walk goes on without waiting: the warps meet at their barriers.
+    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const uint32_t t_row = tbase + ((uint32_t)((warp & 3) * 32) << 16);
+    float* red = reinterpret_cast<float*>(smem + SH::RED);
+    float* rfac = reinterpret_cast<float*>(smem + SH::RFAC);
     int it = 0;
     bool ok = true;
-    for (int64_t t = t_begin; ok && t < t_end;) {
-      const Segment sg = find_segment(pre, pa.tiles, sum, c.heads, t, t_end);
-      const int64_t r = (int64_t)sg.tile * kPRows + row;
-      const bool live = r < (int64_t)a.M * G;
-      const int m = live ? (int)(r / G) : a.M - 1, hq = sg.head * G + (live ? (int)(r % G) : 0);
-      const int p = a.pos0 + m;
-      // the row's queries as two terms of q * 2^k, |q| 2^k < 2^7, channels in the order of the key words
-      float rowf;
-      {
-        const float* q = a.q + (size_t)m * a.ldq + (size_t)hq * HD;
-        float top = 0.0f, qs[NG];
+    Segment sg;
+    for (int64_t t = t_begin; next_segment(sg, pre, pa.tiles, sum, c.heads, t, t_end); t = sg.next) {
+      const int64_t r0 = (int64_t)sg.tile * kPRows, rows = (int64_t)a.M * G;
+      // queries as two terms of q * 2^k, |q| 2^k < 2^7, channels in the order of the key words: a warp
+      // takes 16 rows, HD / 4 lanes a row; the high terms go to tensor memory by way of the low terms' place
+#pragma unroll 1
+      for (int term = 0; term < 2; ++term) {
+        constexpr int LPR = HD / 4, RPW = 32 / LPR;
+        const int ql = lane % LPR;
+#pragma unroll 4
+        for (int i = 0; i < 16; i += RPW) {
+          const int y = warp * 16 + i + lane / LPR;
+          const int64_t r = r0 + y;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (r < rows)
+            v = *reinterpret_cast<const float4*>(a.q + (size_t)(r / G) * a.ldq + (size_t)(sg.head * G + (int)(r % G)) * HD + 4 * ql);
+          float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+          float qs = __fadd_rn(__fadd_rn(v.x, v.y), __fadd_rn(v.z, v.w));
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          qs[g] = 0.0f;
+          for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(q + 32 * g + i);
-            top = fmaxf(fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-            qs[g] = __fadd_rn(qs[g], __fadd_rn(__fadd_rn(v.x, v.y), __fadd_rn(v.z, v.w)));
+          for (int o = 1; o < 8; o <<= 1) qs = __fadd_rn(qs, __shfl_xor_sync(0xffffffffu, qs, o));
+          const int k = max(min(7 - ceil_exp2(top), 100), -100);
+          const float up = pow2i(k);
+          // of 8 channels the even lane makes pairs (0, 4), (1, 5), the odd one (2, 6), (3, 7)
+          const bool odd = lane & 1;
+          const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.z, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v.y : v.w, 1);
+          uint2 hi, lo;
+          split_f16((odd ? s0 : v.x) * up, (odd ? v.z : s0) * up, hi.x, lo.x);
+          split_f16((odd ? s1 : v.y) * up, (odd ? v.w : s1) * up, hi.y, lo.y);
+          const int ch = 4 * ql;  // plane position of its 8 bytes
+          *reinterpret_cast<uint2*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(y, ch & 63)) = term ? lo : hi;
+          if (term) {
+            float q4[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) q4[g] = g < NG ? __shfl_sync(0xffffffffu, qs, (lane & ~(LPR - 1)) + 8 * (g % NG)) * up : 0.0f;
+            if (ql == 0) {
+              uint32_t h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};  // 7.5 x and 1 x the groups' sums
+#pragma unroll
+              for (int g = 0; g < NG; g += 2) {
+                split_f16(q4[g] * 7.5f, q4[g + 1] * 7.5f, h[g / 2], l[g / 2]);
+                split_f16(q4[g], q4[g + 1], h[NG / 2 + g / 2], l[NG / 2 + g / 2]);
+              }
+              *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(y, 0)) = make_uint4(h[0], h[1], h[2], h[3]);
+              *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(y, 1)) = make_uint4(l[0], l[1], l[2], l[3]);
+              rfac[y] = a.scale * 1.44269504088896341f * pow2i(-k);
+            }
           }
         }
-        const int k = max(min(7 - ceil_exp2(top), 100), -100);
-        const float up = live ? pow2i(k) : 0.0f;
-        rowf = a.scale * 1.44269504088896341f * pow2i(-k);
-#pragma unroll 2
-        for (int x = 0; x < HD / 8; ++x) {
-          const float4 u = *reinterpret_cast<const float4*>(q + 8 * x), v = *reinterpret_cast<const float4*>(q + 8 * x + 4);
-          uint4 hi, lo;
-          split_f16(u.x * up, v.x * up, hi.x, lo.x);
-          split_f16(u.y * up, v.y * up, hi.y, lo.y);
-          split_f16(u.z * up, v.z * up, hi.z, lo.z);
-          split_f16(u.w * up, v.w * up, hi.w, lo.w);
-          tmem_st4(t_row + kColQ + 4 * x, hi);
-          *reinterpret_cast<uint4*>(smem + SH::QL + (x >> 3) * (kPRows * 128) + sw128_offset(row, (x & 7) * 8)) = lo;
-        }
-        uint32_t h[4], l[4];  // 7.5 x and 1 x the groups' sums
+        if (term == 0) {
+          named_bar_sync(1, 256);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = l[i] = 0u;
+          for (int x = 0; x < HD / 64; ++x) {
+            const int ch = half * (HD / 2) + 32 * x;  // 32 channels: 16 columns
+            uint32_t h[16];
 #pragma unroll
-        for (int g = 0; g < NG; g += 2) {
-          split_f16(qs[g] * up * 7.5f, qs[g + 1] * up * 7.5f, h[g / 2], l[g / 2]);
-          split_f16(qs[g] * up, qs[g + 1] * up, h[NG / 2 + g / 2], l[NG / 2 + g / 2]);
+            for (int y = 0; y < 4; ++y) {
+              const uint4 v = *reinterpret_cast<const uint4*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(row, (ch & 63) + 8 * y));
+              h[4 * y] = v.x; h[4 * y + 1] = v.y; h[4 * y + 2] = v.z; h[4 * y + 3] = v.w;
+            }
+            tmem_st16(t_row + kColQ + ch / 2, h);
+          }
+          tmem_wait_st();
+          named_bar_sync(1, 256);
         }
-        *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(row, 0)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(row, 1)) = make_uint4(l[0], l[1], l[2], l[3]);
       }
-      tmem_wait_st();
       tc_fence_before();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar + B_QFULL);
+      named_bar_sync(1, 256);  // rfac
 
-      const uint64_t rowf2 = pair(rowf, rowf);
+      const int64_t r = r0 + row;
+      const bool live = r < rows;
+      const int p = a.pos0 + (live ? (int)(r / G) : a.M - 1);
+      const uint64_t rowf2 = pair(rfac[row], rfac[row]);
       float ref = kKv4Never;
       uint64_t l2 = pair(0.0f, 0.0f);
       bool summed = false;  // the second accumulator holds something
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
         const int b = it & 1;
-        if (!(ok = wait(B_SFULL + b, (it >> 1) & 1))) break;
+        ok = ok && wait(B_EFULL + (it & 3), (it >> 2) & 1) && wait(B_SFULL + b, (it >> 1) & 1);
         tc_fence_after();
-        const float* rp = reinterpret_cast<const float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF);
+        const float* rp = reinterpret_cast<const float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF) + 32 * half;
         const int* full = reinterpret_cast<const int*>(smem + SH::FULL) + (it & 3) * 2;
-        const bool masked = !(full[0] && full[1]);
-        const uint32_t t_s = t_row + kColS + b * kPKV;
-        // score + e in log2 units, back to the same columns, and the row's maximum
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int i = 0; i < kPKV; i += 16) {
-          uint32_t v[16];
-          tmem_ld16(t_s + i, v);
-          tmem_wait_ld();
-          tmem_loaded16(v);
-          float x[16];
+        const uint32_t t_s = t_row + kColS + b * kPKV + 32 * half;
+        // score + e in log2 units of this half's 32 rows, and the row's maximum
+        uint32_t v0[16], v1[16];
+        tmem_ld16(t_s, v0);
+        tmem_ld16(t_s + 16, v1);
+        tmem_wait_ld();
+        tmem_loaded16(v0);
+        tmem_loaded16(v1);
+        float x[32];
 #pragma unroll
-          for (int y = 0; y < 16; y += 4) {
-            const ulonglong2 kf = *reinterpret_cast<const ulonglong2*>(rp + i + y), ve = *reinterpret_cast<const ulonglong2*>(rp + 64 + i + y);
-            const float2 x0 = unpair(fma2(mul2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), rowf2), kf.x, ve.x));
-            const float2 x1 = unpair(fma2(mul2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), rowf2), kf.y, ve.y));
-            x[y] = x0.x; x[y + 1] = x0.y; x[y + 2] = x1.x; x[y + 3] = x1.y;
-          }
-          if (masked) {
-            const int* at = reinterpret_cast<const int*>(rp + 3 * kPKV) + i;
-#pragma unroll
-            for (int y = 0; y < 16; ++y)
-              if (!(at[y] <= p && p < at[kPKV + y])) x[y] = -INFINITY;
-          }
-#pragma unroll
-          for (int y = 0; y < 16; y += 2) top = fmaxf(top, fmaxf(x[y], x[y + 1]));
-#pragma unroll
-          for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(x[y]);
-          tmem_st16(t_s + i, v);
+        for (int y = 0; y < 32; y += 4) {
+          const ulonglong2 kf = *reinterpret_cast<const ulonglong2*>(rp + y), ve = *reinterpret_cast<const ulonglong2*>(rp + 64 + y);
+          const uint32_t* v = y < 16 ? v0 + y : v1 + (y - 16);
+          const float2 x0 = unpair(fma2(mul2(pair(__uint_as_float(v[0]), __uint_as_float(v[1])), rowf2), kf.x, ve.x));
+          const float2 x1 = unpair(fma2(mul2(pair(__uint_as_float(v[2]), __uint_as_float(v[3])), rowf2), kf.y, ve.y));
+          x[y] = x0.x; x[y + 1] = x0.y; x[y + 2] = x1.x; x[y + 3] = x1.y;
         }
+        if (!full[half]) {
+#pragma unroll
+          for (int y = 0; y < 32; y += 4) {
+            const int4 from = *reinterpret_cast<const int4*>(rp + 192 + y), until = *reinterpret_cast<const int4*>(rp + 256 + y);
+            if (!(from.x <= p && p < until.x)) x[y] = -INFINITY;
+            if (!(from.y <= p && p < until.y)) x[y + 1] = -INFINITY;
+            if (!(from.z <= p && p < until.z)) x[y + 2] = -INFINITY;
+            if (!(from.w <= p && p < until.w)) x[y + 3] = -INFINITY;
+          }
+        }
+        float top = fmaxf(x[0], x[1]);
+#pragma unroll
+        for (int y = 2; y < 32; y += 2) top = fmaxf(top, fmaxf(x[y], x[y + 1]));
+        red[(2 * b + half) * kPRows + row] = top;
+        named_bar_sync(4 + (warp & 3), 64);
+        top = fmaxf(top, red[(2 * b + (half ^ 1)) * kPRows + row]);
         float al = 1.0f;
-        const bool grow = __any_sync(0xffffffffu, top > ref + kRoom);
+        const bool grow = __any_sync(0xffffffffu, top > ref + kRoom);  // alike in both halves
         if (grow) {
           const float now = fmaxf(ref, top);
           al = exp2_fast(ref - now);
           ref = now;
           l2 = mul2(l2, pair(al, al));
         }
-        tmem_wait_st();
         // weights as two f16 terms, over the scores; their sum without the rows' powers of two
         const uint64_t shift = pair(kHead - ref, kHead - ref);
-#pragma unroll 1
-        for (int i = 0; i < kPKV; i += 16) {
-          uint32_t v[16], w[16];
-          tmem_ld16(t_s + i, v);
-          tmem_wait_ld();
-          tmem_loaded16(v);
 #pragma unroll
-          for (int y = 0; y < 16; y += 4) {
-            const ulonglong2 ie = *reinterpret_cast<const ulonglong2*>(rp + 128 + i + y);
-            const float2 x0 = unpair(add2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), shift));
-            const float2 x1 = unpair(add2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), shift));
-            const uint64_t w0 = pair(exp2_fast(x0.x), exp2_fast(x0.y)), w1 = pair(exp2_fast(x1.x), exp2_fast(x1.y));
-            l2 = fma2(w0, ie.x, l2);
-            l2 = fma2(w1, ie.y, l2);
-            split_pair(w0, w[y / 2], w[8 + y / 2]);
-            split_pair(w1, w[y / 2 + 1], w[8 + y / 2 + 1]);
-          }
-          tmem_st16(t_s + i, w);
+        for (int y = 0; y < 32; y += 4) {
+          const ulonglong2 ie = *reinterpret_cast<const ulonglong2*>(rp + 128 + y);
+          const float2 x0 = unpair(add2(pair(x[y], x[y + 1]), shift)), x1 = unpair(add2(pair(x[y + 2], x[y + 3]), shift));
+          const uint64_t w0 = pair(exp2_fast(x0.x), exp2_fast(x0.y)), w1 = pair(exp2_fast(x1.x), exp2_fast(x1.y));
+          l2 = fma2(w0, ie.x, l2);
+          l2 = fma2(w1, ie.y, l2);
+          uint32_t* w = y < 16 ? v0 : v1;
+          split_pair(w0, w[(y & 15) / 2], w[8 + (y & 15) / 2]);
+          split_pair(w1, w[(y & 15) / 2 + 1], w[8 + (y & 15) / 2 + 1]);
         }
+        tmem_st16(t_s, v0);
+        tmem_st16(t_s + 16, v1);
         // every kPDrain steps the sums so far go to the second accumulator; both follow the reference
         const int step = j - sg.begin;
         const bool drain = step > 0 && step % kPDrain == 0;
         if (step > 0 && (drain || grow)) {
-          if (!(ok = wait(B_PDONE + (b ^ 1), ((it - 1) >> 1) & 1))) break;
+          ok = ok && wait(B_PDONE + (b ^ 1), ((it - 1) >> 1) & 1);
           tc_fence_after();
           const uint64_t al2 = pair(al, al);
+          const int end = half ? SH::NV : HD / 2;
 #pragma unroll 1
-          for (int i = 0; i < SH::NV; i += 16) {
+          for (int i = half ? HD / 2 : 0; i < end; i += 16) {
             uint32_t o[16], s[16];
             tmem_ld16(t_row + kColO + i, o);
             if (summed) tmem_ld16(t_row + kColSum + i, s);
@@ -442,62 +491,91 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         __syncwarp();
         if (lane == 0) mbar_arrive(bar + B_PFULL + b);
       }
-      if (!ok) break;
 
-      // the row's result, or its part
-      if (!(ok = wait(B_PDONE + ((it - 1) & 1), ((it - 1) >> 1) & 1))) break;
+      // the rows' results, or their parts: 2 SC columns of a half's at a time through the queries' place
+      ok = ok && wait(B_PDONE + ((it - 1) & 1), ((it - 1) >> 1) & 1);
       tc_fence_after();
       const float2 lv = unpair(l2);
-      const float l = lv.x + lv.y, D = l == 0.0f ? 1.0f : l;
-      float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      red[(4 + half) * kPRows + row] = lv.x + lv.y;
+      named_bar_sync(1, 256);  // also: every warp is past its queries
+      const float l = __fadd_rn(red[4 * kPRows + row], red[5 * kPRows + row]);
       const bool whole = sg.begin == 0 && sg.end == sg.steps;
-      float* part = pa.parts + (((size_t)blockIdx.x * 2 + (t == t_begin ? 0 : 1)) * kPRows + row) * SH::PART;
-      const size_t out_at = (size_t)m * a.H * HD + (size_t)hq * HD;
-#pragma unroll 1
-      for (int x = SH::NV / 16 - 1; x >= 0; --x) {  // the minima's columns first
-        const int i = 16 * x;
+      const float inv = whole ? __frcp_rn(l == 0.0f ? 1.0f : l) : 1.0f;
+      float* parts = pa.parts + ((size_t)blockIdx.x * 2 + (t == t_begin ? 0 : 1)) * kPRows * SH::PART;
+      if (!whole && live && half == 0)
+        *reinterpret_cast<float2*>(parts + (size_t)row * SH::PART) = make_float2(ref == kKv4Never ? -INFINITY : ref, l);
+      // columns of O, both accumulators
+      auto load_o = [&](int i, float (&y)[16]) {
         uint32_t o[16], s[16];
         tmem_ld16(t_row + kColO + i, o);
         if (summed) tmem_ld16(t_row + kColSum + i, s);
         tmem_wait_ld();
         tmem_loaded16(o);
+        if (summed) tmem_loaded16(s);
+#pragma unroll
+        for (int n = 0; n < 16; ++n) y[n] = summed ? __uint_as_float(o[n]) + __uint_as_float(s[n]) : __uint_as_float(o[n]);
+      };
+      float z[4];
+      {
         float y[16];
+        load_o(HD, y);
 #pragma unroll
-        for (int n = 0; n < 16; ++n) y[n] = __uint_as_float(o[n]);
-        if (summed) {
-          tmem_loaded16(s);
+        for (int n = 0; n < 4; ++n) z[n] = y[n] + y[4 + n];
+      }
+      constexpr int SC = SH::SC, STRIDE = SC + 4;
+      float* stage = reinterpret_cast<float*>(smem + SH::QL) + warp * (32 * STRIDE);
+      // HD 128: a half is one block (groups 2 half, + 1), HD 64: half of the one block
+      const int g0 = HD == 128 ? 2 * half : 0;
+      const float za = (HD == 128 && half) ? z[2] : z[0], zb = (HD == 128 && half) ? z[3] : z[1];
+#pragma unroll 1
+      for (int q = 0; q < (HD / 2) / SC; ++q) {
+        const int col = half * (HD / 2) + q * SC;
 #pragma unroll
-          for (int n = 0; n < 16; ++n) y[n] += __uint_as_float(s[n]);
-        }
-        if (i == HD) {
+        for (int x = 0; x < SC / 16; ++x) {
+          float y[16];
+          load_o(col + 16 * x, y);
 #pragma unroll
-          for (int n = 0; n < 4; ++n) z[n] = y[n];
-          continue;
-        }
-        if (!live) continue;
-        const int g = i / 32;
-        const float zg = g == 0 ? z[0] : g == 1 ? z[1] : g == 2 ? z[2] : z[3];
-#pragma unroll
-        for (int n = 0; n < 16; n += 4) {
-          const float4 f = make_float4(y[n] + zg, y[n + 1] + zg, y[n + 2] + zg, y[n + 3] + zg);
-          if (whole) {
-            const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + out_at + i + n) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(a.out_c + out_at + i + n) =
-                make_float4(__fsub_rn(__fdiv_rn(f.x, D), mk.x), __fsub_rn(__fdiv_rn(f.y, D), mk.y),
-                            __fsub_rn(__fdiv_rn(f.z, D), mk.z), __fsub_rn(__fdiv_rn(f.w, D), mk.w));
-            *reinterpret_cast<float4*>(a.out_s + out_at + i + n) = mk;
-          } else {
-            *reinterpret_cast<float4*>(part + 4 + i + n) = f;
+          for (int u = 0; u < 2; ++u) {  // units of 4 channels of both groups
+            const float* f = y + 8 * u;
+            *reinterpret_cast<float4*>(stage + lane * STRIDE + 4 * (2 * x + u)) =
+                make_float4((f[0] + za) * inv, (f[2] + za) * inv, (f[4] + za) * inv, (f[6] + za) * inv);
+            *reinterpret_cast<float4*>(stage + lane * STRIDE + SC / 2 + 4 * (2 * x + u)) =
+                make_float4((f[1] + zb) * inv, (f[3] + zb) * inv, (f[5] + zb) * inv, (f[7] + zb) * inv);
           }
         }
+        __syncwarp();
+        // SC / 2 channels of each group from 4 * (first unit)
+        const int unit = (col & 63) / 8;
+        constexpr int LPR = SC / 4;
+#pragma unroll 1
+        for (int i = lane / LPR; i < 32; i += 32 / LPR) {
+          const int f = lane % LPR, g = g0 + f / (LPR / 2), ch = 32 * g + 4 * unit + 4 * (f % (LPR / 2));
+          const int y = (warp & 3) * 32 + i;
+          const int64_t rr = r0 + y;
+          if (rr >= rows) continue;
+          const float4 v = *reinterpret_cast<const float4*>(stage + i * STRIDE + 4 * f);
+          if (whole) {
+            const size_t to = (size_t)(rr / G) * a.H * HD + (size_t)(sg.head * G + (int)(rr % G)) * HD + ch;
+            const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + to) : make_float4(0.f, 0.f, 0.f, 0.f);
+            *reinterpret_cast<float4*>(a.out_c + to) =
+                make_float4(__fsub_rn(v.x, mk.x), __fsub_rn(v.y, mk.y), __fsub_rn(v.z, mk.z), __fsub_rn(v.w, mk.w));
+            *reinterpret_cast<float4*>(a.out_s + to) = mk;
+          } else {
+            *reinterpret_cast<float4*>(parts + (size_t)y * SH::PART + 4 + ch) = v;
+          }
+        }
+        __syncwarp();
       }
-      if (!whole && live) *reinterpret_cast<float2*>(part) = make_float2(ref == kKv4Never ? -INFINITY : ref, l);
       tc_fence_before();
-      t += sg.end - sg.begin;
+      named_bar_sync(1, 256);  // the queries' place is free again
     }
-  } else if (warp < 8) {
-    // ---- unpacking ----------------------------------------------------------------------------
-    const int th = tid - 128, w4 = warp - 4;
+  } else if (warp < 16) {
+    // ---- unpacking: keys (warps 8-11) or values (12-15), thread -> row th % 64, half th / 64 of its bytes --
+    const bool vals = warp >= 12;
+    const int th = tid & 127, w4 = warp & 3, r = th & 63, kh = th >> 6;
+    const uint8_t* codes = vals ? c.vc : c.kc;
+    const uint8_t* params = reinterpret_cast<const uint8_t*>(vals ? c.vp : c.kp);
+    uint8_t* raws = smem + SH::RAW + (vals ? 2 * SH::RAWBUF : 0);
     // a walk over the CTA's steps
     struct Walk {
       int64_t t;
@@ -505,105 +583,99 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       Kv4Spans sp;
       size_t base;
       int lo, hi, j;
+      bool live;
     };
     auto enter = [&](Walk& w) {
-      if (w.t >= t_end) return;
-      w.sg = find_segment(pre, pa.tiles, sum, c.heads, w.t, t_end);
+      w.live = next_segment(w.sg, pre, pa.tiles, sum, c.heads, w.t, t_end);
+      if (!w.live) return;
       tile_positions(a, w.sg.tile, G, w.lo, w.hi);
       w.sp = kv4_spans(c, w.lo, w.hi, a.window);
       w.base = kv4_base(c, a.slot0, w.sg.head);
       w.j = w.sg.begin;
     };
     auto advance = [&](Walk& w) {
-      ++w.t;
-      if (++w.j == w.sg.end) enter(w);
+      if (w.live && ++w.j == w.sg.end) {
+        w.t = w.sg.next;
+        enter(w);
+      }
     };
     // asynchronous copies of a step's rows as they are stored: warp w4 copies its w4-th chunk
     constexpr int CPR = HD / 32, NC = kKv4Chunk * CPR, NP = kKv4Chunk * 4 * NG / 16;
     auto fetch = [&](const Walk& w, int buf) {
       const int x = w.j * (kPKV / kKv4Chunk) + w4;
-      if (w.t < t_end && x < w.sp.total) {
+      if (w.live && x < w.sp.total) {
         const size_t row0 = w.base + (size_t)kv4_span_chunk(w.sp, x) * kKv4Chunk;
-        uint8_t* raw = smem + SH::RAW + buf * SH::RAWBUF;
+        uint8_t* raw = raws + buf * SH::RAWBUF;
 #pragma unroll
         for (int i = 0; i < NC / 32; ++i) {
-          const int y = lane + 32 * i, r = w4 * kKv4Chunk + y / CPR, q = y % CPR;
-          const uint32_t at = (uint32_t)(r * CPR + (HD == 128 ? q ^ ((r >> 1) & 3) : q)) * 16;
-          cp_async16(raw + at, c.kc + row0 * (HD / 2) + y * 16, 16);
-          cp_async16(raw + SH::RAWC + at, c.vc + row0 * (HD / 2) + y * 16, 16);
+          const int y = lane + 32 * i, rr = w4 * kKv4Chunk + y / CPR, q = y % CPR;
+          cp_async16(raw + (uint32_t)(rr * CPR + (HD == 128 ? q ^ ((rr >> 1) & 3) : q)) * 16, codes + row0 * (HD / 2) + y * 16, 16);
         }
-        if (lane < 2 * NP) {
-          const bool v = lane >= NP;
-          const int y = v ? lane - NP : lane;
-          cp_async16(raw + 2 * SH::RAWC + (v ? SH::RAWP : 0) + w4 * (kKv4Chunk * 4 * NG) + y * 16,
-                     reinterpret_cast<const uint8_t*>(v ? c.vp : c.kp) + row0 * (4 * NG) + y * 16, 16);
-        }
+        if (lane < NP) cp_async16(raw + SH::RAWC + w4 * (kKv4Chunk * 4 * NG) + lane * 16, params + row0 * (4 * NG) + lane * 16, 16);
       }
       cp_async_commit();
     };
+    // after a wait that ran out the walk goes on without waiting: the four warps meet at their barrier
     bool ok = true;
     Walk at{}, ahead{};
     at.t = ahead.t = t_begin;
     enter(at);
-    enter(ahead);
-    if (t_begin < t_end) {
-      fetch(ahead, 0);
-      advance(ahead);
-    }
-    for (int it = 0; at.t < t_end; ++it) {
+    ahead = at;
+    fetch(ahead, 0);
+    advance(ahead);
+    for (int it = 0; at.live; ++it) {
       const int b = it & 1;
-      const uint8_t* raw = smem + SH::RAW + b * SH::RAWBUF;
+      const uint8_t* raw = raws + b * SH::RAWBUF;
       cp_async_wait<0>();
-      named_bar_sync(1, 128);  // this step's rows have landed, and nobody reads the last step's
+      named_bar_sync(vals ? 3 : 2, 128);  // this step's rows have landed, and nobody reads the last step's
       fetch(ahead, b ^ 1);
       advance(ahead);
-      // after a wait that ran out the walk goes on without waiting: the four warps meet at their barriers
-      ok = ok && (it < 2 || wait(B_KFREE + b, ((it - 2) >> 1) & 1));
-      // one row a thread: keys 0-63, values 64-127
-      {
-        const int r = th & 63;
-        const bool vals = th >= 64;
-        // whether any query of the tile sees the row: at positions [from, until)
-        int from = 0x7fffffff, until = 0;
-        const int x = at.j * (kPKV / kKv4Chunk) + r / kKv4Chunk;
-        if (x < at.sp.total) {
-          const int row = kv4_span_chunk(at.sp, x) * kKv4Chunk + r % kKv4Chunk;
-          const int held = kv4_held(c, row, last);
-          const int64_t end = a.window > 0 && row >= c.sinks ? (int64_t)held + a.window : 0x7fffffff;
-          if ((row < c.sinks || held >= c.sinks) && held <= at.hi && end > at.lo) {
-            from = held;
-            until = (int)min(end, (int64_t)0x7fffffff);
-          }
+      // whether any query of the tile sees the row: at positions [from, until)
+      int from = 0x7fffffff, until = 0;
+      const int x = at.j * (kPKV / kKv4Chunk) + r / kKv4Chunk;
+      if (x < at.sp.total) {
+        const int row = kv4_span_chunk(at.sp, x) * kKv4Chunk + r % kKv4Chunk;
+        const int held = kv4_held(c, row, last);
+        const int64_t end = a.window > 0 && row >= c.sinks ? (int64_t)held + a.window : 0x7fffffff;
+        if ((row < c.sinks || held >= c.sinks) && held <= at.hi && end > at.lo) {
+          from = held;
+          until = (int)min(end, (int64_t)0x7fffffff);
         }
-        uint32_t w[NG];
-        const uint8_t* src = raw + 2 * SH::RAWC + (vals ? SH::RAWP : 0) + r * (4 * NG);
-        if constexpr (NG == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src);
-          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-        } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(src);
-          w[0] = v.x; w[1] = v.y;
-        }
-        if (until == 0) {
+      }
+      uint32_t w[NG];
+      if constexpr (NG == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(raw + SH::RAWC + r * 16);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(raw + SH::RAWC + r * 8);
+        w[0] = v.x; w[1] = v.y;
+      }
+      if (until == 0) {  // its parameters may be anything
 #pragma unroll
-          for (int g = 0; g < NG; ++g) w[g] = 0u;
+        for (int g = 0; g < NG; ++g) w[g] = 0u;
+      }
+      RowParams<NG> q;
+      q.set(w, vals);
+      const float down = pow2i(-q.e), up9 = down * 512.0f;
+      float* rp = reinterpret_cast<float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF);
+      const int free_bar = vals ? B_VFREE : B_KFREE;
+      if (vals) {
+        if (kh == 0) {
+          rp[64 + r] = (float)q.e;
+          rp[128 + r] = pow2i(-q.e);
         }
-        RowParams<NG> q;
-        q.set(w, vals);
-        const float down = pow2i(-q.e), up9 = down * 512.0f;
-        float* rp = reinterpret_cast<float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar + B_EFULL + (it & 3));
+      }
+      ok = ok && (it < 2 || wait(free_bar + b, ((it - 2) >> 1) & 1));
+      if (kh == 0) {
         if (!vals) {
-          uint32_t s[NG / 2], y[4] = {0u, 0u, 0u, 0u};
+          uint32_t y[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
           for (int g = 0; g < NG; g += 2) {
-            s[g / 2] = pack_f16(q.s[g] * up9, q.s[g + 1] * up9);
             y[g / 2] = pack_f16(q.s[g] * down, q.s[g + 1] * down);
             y[NG / 2 + g / 2] = pack_f16(q.z[g] * down, q.z[g + 1] * down);
           }
-          if constexpr (NG == 4)
-            *reinterpret_cast<uint2*>(smem + SH::KS + r * 8) = make_uint2(s[0], s[1]);
-          else
-            *reinterpret_cast<uint32_t*>(smem + SH::KS + r * 4) = s[0];
           uint8_t* kx = smem + SH::KX + b * SH::KXBUF;
           *reinterpret_cast<uint4*>(kx + plain16_offset(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
           *reinterpret_cast<uint4*>(kx + plain16_offset(r, 1)) = make_uint4(y[0], y[1], y[2], y[3]);
@@ -613,178 +685,141 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           const int full = __all_sync(0xffffffffu, from <= at.lo && at.hi < until);
           if (lane == 0) reinterpret_cast<int*>(smem + SH::FULL)[(it & 3) * 2 + w4] = full;
         } else {
-          rp[64 + r] = (float)q.e;
-          rp[128 + r] = pow2i(-q.e);
-          __half *vs = reinterpret_cast<__half*>(smem + SH::VS), *vm = reinterpret_cast<__half*>(smem + SH::VM);
+          // middles: column g the high term, 4 + g the low one
+          __half* vx = reinterpret_cast<__half*>(smem + SH::VX + b * SH::VXBUF + (r >> 3) * 256 + (r & 7) * 2);
 #pragma unroll
           for (int g = 0; g < NG; ++g) {
-            vs[g * kPKV + r] = __float2half_rn(q.s[g] * up9);
             const float y = q.z[g] * down;
             const __half h = __float2half_rn(y);
-            vm[g * kPKV + r] = h;
-            vm[(NG + g) * kPKV + r] = __float2half_rn(__fsub_rn(y, __half2float(h)));
+            vx[g * 8] = h;
+            vx[(4 + g) * 8] = __float2half_rn(__fsub_rn(y, __half2float(h)));
           }
         }
       }
-      named_bar_sync(1, 128);
-      // keys: thread -> row th % 64, words 2 (th / 64), + 1 of every group
-      {
-        const int r = th & 63, kh = th >> 6;
-        uint8_t* kb = smem + SH::K + b * SH::KBUF;
-        uint32_t s[NG / 2];
+      uint8_t* to = smem + (vals ? SH::V : SH::K) + b * SH::BUF + (r >> 3) * 1024 + (r & 7) * 128;
+      __half2 s2[NG / 2];
+#pragma unroll
+      for (int g = 0; g < NG; g += 2) s2[g / 2] = __floats2half2_rn(q.s[g] * up9, q.s[g + 1] * up9);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t cw[NG];
         if constexpr (NG == 4) {
-          const uint2 v = *reinterpret_cast<const uint2*>(smem + SH::KS + r * 8);
-          s[0] = v.x; s[1] = v.y;
+          const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 64 + (((2 * kh + x) ^ ((r >> 1) & 3)) << 4));
+          cw[0] = v.x; cw[1] = v.y; cw[2] = v.z; cw[3] = v.w;
         } else {
-          s[0] = *reinterpret_cast<const uint32_t*>(smem + SH::KS + r * 4);
+          const uint2 v = *reinterpret_cast<const uint2*>(raw + r * 32 + (2 * kh + x) * 8);
+          cw[0] = v.x; cw[1] = v.y;
         }
-#pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-          const int u = 2 * kh + x;
-          uint32_t kw[NG];
-          if constexpr (NG == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 64 + ((u ^ ((r >> 1) & 3)) << 4));
-            kw[0] = v.x; kw[1] = v.y; kw[2] = v.z; kw[3] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(raw + r * 32 + u * 8);
-            kw[0] = v.x; kw[1] = v.y;
-          }
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const __half2 sv = (g & 1) ? __high2half2(as_half2(s[g / 2])) : __low2half2(as_half2(s[g / 2]));
-            const uint32_t w = kw[g], w8 = w >> 8;
-            uint4 h, l;
-            scale_pair(centre_low(w), sv, h.x, l.x);
-            scale_pair(centre_high(w), sv, h.y, l.y);
-            scale_pair(centre_low(w8), sv, h.z, l.z);
-            scale_pair(centre_high(w8), sv, h.w, l.w);
-            uint8_t* to = kb + (g >> 1) * (kPKV * 128) + sw128_offset(r, (g & 1) * 32 + u * 8);
-            *reinterpret_cast<uint4*>(to) = h;
-            *reinterpret_cast<uint4*>(to + KB * kPKV * 128) = l;
-          }
+        for (int i = 0; i < NG; ++i) {
+          // keys: word 2 kh + x of group i; values: unit (2 kh + x) NG / 2 + i / (NG / 2) (HD 64: 2 (2 kh + x)
+          // + i) of groups 2 (i % (NG / 2)), + 1
+          const int ublk = i % (NG / 2), unit = (2 * kh + x) * 2 + i / (NG / 2);
+          const int blk = vals ? ublk : i >> 1, chunk = vals ? unit : (i & 1) * 4 + 2 * kh + x;
+          const __half2 sv = vals ? s2[ublk] : ((i & 1) ? __high2half2(s2[i / 2]) : __low2half2(s2[i / 2]));
+          const uint32_t cwi = cw[i], c8 = cwi >> 8;
+          uint4 h, l;
+          scale_pair(centre_low(cwi), sv, h.x, l.x);
+          scale_pair(centre_high(cwi), sv, h.y, l.y);
+          scale_pair(centre_low(c8), sv, h.z, l.z);
+          scale_pair(centre_high(c8), sv, h.w, l.w);
+          uint8_t* y = to + blk * (kPKV * 128) + ((chunk ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(y) = h;
+          *reinterpret_cast<uint4*>(y + KB * kPKV * 128) = l;
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar + B_KFULL + b);
-      ok = ok && (it < 2 || wait(B_VFREE + b, ((it - 2) >> 1) & 1));
-      // values, transposed: thread -> rows 2 lane, + 1, units 2 w4, + 1
-      {
-        uint8_t* vb = smem + SH::V + b * SH::VBUF;
-        const uint32_t col = (uint32_t)(lane >> 2), in = (uint32_t)(lane & 3) * 4;
-        const uint8_t* rv = raw + SH::RAWC;
-#pragma unroll 1
-        for (int x = 0; x < 2; ++x) {
-          const int u = 2 * w4 + x;
-          uint32_t va[NG / 2], vc[NG / 2];
-          if constexpr (NG == 4) {
-            const uint8_t* y = rv + lane * 128 + ((w4 ^ (lane & 3)) << 4) + x * 8;
-            const uint2 y0 = *reinterpret_cast<const uint2*>(y), y1 = *reinterpret_cast<const uint2*>(y + 64);
-            va[0] = y0.x; va[1] = y0.y; vc[0] = y1.x; vc[1] = y1.y;
-          } else {
-            va[0] = *reinterpret_cast<const uint32_t*>(rv + lane * 64 + u * 4);
-            vc[0] = *reinterpret_cast<const uint32_t*>(rv + lane * 64 + 32 + u * 4);
-          }
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const __half2 sv = *reinterpret_cast<const __half2*>(smem + SH::VS + g * (kPKV * 2) + lane * 4);
-            const uint32_t w = __byte_perm(va[g / 2], vc[g / 2], (g & 1) ? 0x7632 : 0x5410), w8 = w >> 8;
-            uint32_t h[4], l[4];
-            scale_pair(centre_low(w), sv, h[0], l[0]);
-            scale_pair(centre_high(w), sv, h[1], l[1]);
-            scale_pair(centre_low(w8), sv, h[2], l[2]);
-            scale_pair(centre_high(w8), sv, h[3], l[3]);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const int ch = 32 * g + 4 * u + n;  // its row in the swizzled tile; (ch & 7) = 4 x + n
-              uint8_t* to = vb + (uint32_t)(ch >> 3) * 1024u + (uint32_t)(4 * x + n) * 128u + ((col ^ (uint32_t)(4 * x + n)) << 4) + in;
-              *reinterpret_cast<uint32_t*>(to) = h[n];
-              *reinterpret_cast<uint32_t*>(to + SH::NV * 128) = l[n];
-            }
-          }
-        }
-        if (w4 < NG) {  // the middles of group w4
-          uint8_t* to = vb + (HD >> 3) * 1024 + w4 * 128 + ((col ^ (uint32_t)w4) << 4) + in;
-          *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(smem + SH::VM + w4 * (kPKV * 2) + lane * 4);
-          *reinterpret_cast<uint32_t*>(to + SH::NV * 128) = *reinterpret_cast<const uint32_t*>(smem + SH::VM + (NG + w4) * (kPKV * 2) + lane * 4);
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar + B_VFULL + b);
+      if (lane == 0) mbar_arrive(bar + (vals ? B_VFULL : B_KFULL) + b);
       advance(at);
     }
     cp_async_wait<0>();
-  } else if (lane == 0) {
-    // ---- MMAs -----------------------------------------------------------------------------------
-    constexpr uint32_t ids = idesc_f16_f32(kPRows, kPKV), idv = idesc_f16_f32(kPRows, SH::NV);
+  } else {
+    // ---- MMAs: the whole warp walks, one elected thread issues --------------------------------------
+    // Operands that the compiler knows to be the same in the warp (by way of the shuffles) keep an issue
+    // at 10 clocks; from a single thread's registers it takes 45, longer than most of these MMAs.
+    constexpr uint32_t ids = idesc_f16_f32(kPRows, kPKV), idv = idesc_f16_f32(kPRows, HD) | kBWide, idx = idesc_f16_f32(kPRows, 16);
+    const uint32_t tb = __shfl_sync(0xffffffffu, tbase, 0);
     int it = 0, seg = 0;
     bool ok = true;
     auto scores = [&](int i) -> bool {
-      const int b = i & 1;
-      if (!wait_one(B_KFULL + b, (i >> 1) & 1)) return false;
+      const int b = __shfl_sync(0xffffffffu, i & 1, 0);
+      if (!wait(B_KFULL + b, (i >> 1) & 1)) return false;
       tc_fence_after();
-      const uint32_t d = tbase + kColS + b * kPKV;
-      const uint8_t* kb = smem + SH::K + b * SH::KBUF;
-      // small terms first: low high, high low, then the parameters and high high
+      if (elect_one()) {
+        const uint32_t d = tb + kColS + b * kPKV;
+        const uint8_t* kb = smem + SH::K + b * SH::BUF;
+        // small terms first: low high, high low, then the parameters and high high
 #pragma unroll
-      for (int x = 0; x < KB; ++x) {
-        const uint64_t ad = smem_desc_sw128(smem + SH::QL + x * kPRows * 128), bd = smem_desc_sw128(kb + x * kPKV * 128);
+        for (int x = 0; x < KB; ++x) {
+          const uint64_t ad = smem_desc_sw128(smem + SH::QL + x * kPRows * 128), bd = smem_desc_sw128(kb + x * kPKV * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc_mma(d, ad + 2 * k, bd + 2 * k, ids, (x > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) tc_mma(d, ad + 2 * k, bd + 2 * k, ids, (x > 0 || k > 0) ? 1u : 0u);
+        }
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          const uint64_t bd = smem_desc_sw128(kb + (KB + x) * kPKV * 128);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_ts(d, tb + kColQ + 8 * (4 * x + k), bd + 2 * k, ids, 1u);
+        }
+        tc_mma(d, smem_desc_plain(smem + SH::QX, 128, 256), smem_desc_plain(smem + SH::KX + b * SH::KXBUF, 128, 256), ids, 1u);
+#pragma unroll
+        for (int x = 0; x < KB; ++x) {
+          const uint64_t bd = smem_desc_sw128(kb + x * kPKV * 128);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_ts(d, tb + kColQ + 8 * (4 * x + k), bd + 2 * k, ids, 1u);
+        }
+        tc_commit(bar + B_KFREE + b);
+        tc_commit(bar + B_SFULL + b);
       }
-#pragma unroll
-      for (int x = 0; x < KB; ++x) {
-        const uint64_t bd = smem_desc_sw128(kb + (KB + x) * kPKV * 128);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tc_mma_ts(d, tbase + kColQ + 8 * (4 * x + k), bd + 2 * k, ids, 1u);
-      }
-      tc_mma(d, smem_desc_plain16(smem + SH::QX), smem_desc_plain16(smem + SH::KX + b * SH::KXBUF), ids, 1u);
-#pragma unroll
-      for (int x = 0; x < KB; ++x) {
-        const uint64_t bd = smem_desc_sw128(kb + x * kPKV * 128);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) tc_mma_ts(d, tbase + kColQ + 8 * (4 * x + k), bd + 2 * k, ids, 1u);
-      }
-      tc_commit(bar + B_KFREE + b);
-      tc_commit(bar + B_SFULL + b);
+      __syncwarp();
       return true;
     };
-    for (int64_t t = t_begin; ok && t < t_end; ++seg) {
-      const Segment sg = find_segment(pre, pa.tiles, sum, c.heads, t, t_end);
+    Segment sg;
+    for (int64_t t = t_begin; ok && next_segment(sg, pre, pa.tiles, sum, c.heads, t, t_end); ++seg, t = sg.next) {
       const int n = sg.end - sg.begin;
-      if (!(ok = wait_one(B_QFULL, seg & 1))) break;
+      if (!(ok = wait(B_QFULL, seg & 1))) break;
       if (!(ok = scores(it))) break;
       for (int j = 0; j < n; ++j, ++it) {
-        const int b = it & 1;
+        const int b = __shfl_sync(0xffffffffu, it & 1, 0);
+        const uint32_t more = __shfl_sync(0xffffffffu, j % kPDrain > 0 ? 1u : 0u, 0);
         if (j + 1 < n && !(ok = scores(it + 1))) break;
-        if (!(ok = wait_one(B_VFULL + b, (it >> 1) & 1))) break;
-        if (!(ok = wait_one(B_PFULL + b, (it >> 1) & 1))) break;
+        if (!(ok = wait(B_VFULL + b, (it >> 1) & 1))) break;
+        if (!(ok = wait(B_PFULL + b, (it >> 1) & 1))) break;
         tc_fence_after();
-        const uint8_t* vb = smem + SH::V + b * SH::VBUF;
-        const uint32_t pcol = tbase + kColS + b * kPKV;
+        if (elect_one()) {
+          const uint8_t* vb = smem + SH::V + b * SH::BUF;
+          const uint32_t pcol = tb + kColS + b * kPKV, o = tb + kColO;
+          // low and high weights with both terms of the middles; low high, high low, high high
+          const uint64_t xd = smem_desc_plain(smem + SH::VX + b * SH::VXBUF, 256, 128);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {  // low high, high low, high high
-          const uint64_t bd = smem_desc_sw128(vb + (p == 1 ? SH::NV * 128 : 0));
+          for (int k = 0; k < 4; ++k) tc_mma_ts(o + HD, pcol + 8 + 16 * k, xd + 32 * k, idx, k > 0 ? 1u : more);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_ts(tbase + kColO, pcol + (p == 0 ? 8 : 0) + 16 * k, bd + 2 * k, idv, (j % kPDrain > 0 || p > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < 4; ++k) tc_mma_ts(o + HD, pcol + 16 * k, xd + 32 * k, idx, 1u);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            const uint64_t bd = smem_desc_wide128(vb + (p == 1 ? KB * kPKV * 128 : 0), kPKV * 128);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc_mma_ts(o, pcol + (p == 0 ? 8 : 0) + 16 * k, bd + 128 * k, idv, (p > 0 || k > 0) ? 1u : more);
+          }
+          tc_commit(bar + B_VFREE + b);
+          tc_commit(bar + B_PDONE + b);
         }
-        tc_commit(bar + B_VFREE + b);
-        tc_commit(bar + B_PDONE + b);
+        __syncwarp();
       }
-      if (!ok) break;
-      t += n;
     }
-    // every MMA issued has completed before tensor memory is released
-    tc_commit(bar + B_END);
-    if (!mbar_wait_bounded(bar + B_END, 0)) atomicOr(a.err, SHD_DEVERR_TIMEOUT_DRAIN);
+    // every MMA issued has completed before tensor memory is released (commits follow the thread that issued)
+    if (elect_one()) {
+      tc_commit(bar + B_END);
+      if (!mbar_wait_bounded(bar + B_END, 0)) atomicOr(a.err, SHD_DEVERR_TIMEOUT_DRAIN);
+    }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tbase, kCols);
+  if (warp == 16) tmem_dealloc(tbase, kCols);
 }
 
 // Items that a share boundary cuts, joined in CTA order: block (b, y) takes rows 8 y .. + 7 of the item
@@ -794,7 +829,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ P
   using SH = PromptShape<HD>;
   const Kv4AttnArgs& a = pa.a;
   __shared__ int pre[kPTiles];
-  __shared__ int scratch[16];
+  __shared__ int scratch[32];
   pdl_trigger();
   pdl_wait();
   const int G = a.H / a.c.heads;
@@ -802,9 +837,10 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ P
   const int64_t T = (int64_t)sum * a.c.heads, per = (T + ctas - 1) / ctas, t = (blockIdx.x + 1) * per;
   if (t >= T) return;
   const Segment sg = find_segment(pre, pa.tiles, sum, a.c.heads, t, T);
-  const int64_t item = t - sg.begin;
-  if (sg.begin == 0 || item / per != (int64_t)blockIdx.x) return;  // not cut here, or not for the first time
-  const int w0 = (int)(item / per), parts = (int)((item + sg.steps - 1) / per) - w0 + 1;
+  // not cut here, or not for the first time
+  if (sg.begin == 0 || (sg.item + kPItem) / per != (int64_t)blockIdx.x) return;
+  const int64_t item = sg.item;
+  const int w0 = (int)blockIdx.x, parts = (int)((item + kPItem + sg.steps - 1) / per) - w0 + 1;
   const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
   const int64_t r = (int64_t)sg.tile * kPRows + row;
   if (r >= (int64_t)a.M * G) return;
