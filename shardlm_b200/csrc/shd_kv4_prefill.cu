@@ -16,7 +16,8 @@
 //
 // Warps: 0-7 softmax (two threads share a row, half of its 64 scores each: scores come from tensor
 // memory, weights go back to the same columns as the second product's A operand), 8-11 unpack keys and
-// 12-15 values into shared memory, 16 issues the MMAs. Scores, keys and values are double-buffered, so
+// 12-15 values into shared memory, 16 issues the MMAs, 17 walks ahead, fetching rows as they are stored
+// and noting which queries see them. Scores, keys and values are double-buffered, so
 // that S of the next 64 rows and O of the last run while the softmax works; the queries' high terms are
 // an A operand in tensor memory too, which spares shared memory most of the first product's reads. A
 // value row is unpacked as it lies (the second product's B operand is the wide dimension's major). O
@@ -39,7 +40,7 @@ namespace {
 
 constexpr int kPRows = 128;    // (position, head) pairs of a tile
 constexpr int kPKV = 64;       // cache rows of a step
-constexpr int kPThreads = 544;
+constexpr int kPThreads = 576;
 constexpr int kPTiles = 2048;  // tiles a launch (their step counts are in shared memory)
 constexpr int kPItem = 3;      // cost of an item's queries and results, in steps
 constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
@@ -59,12 +60,12 @@ struct PromptShape {
   static constexpr uint32_t KXBUF = kPKV * 32;
   static constexpr uint32_t VX = KX + 2 * KXBUF;               // [2 buffers][64 rows / 8][16 columns][16 B]: value middles
   static constexpr uint32_t VXBUF = kPKV * 32;
-  static constexpr uint32_t RAW = VX + 2 * VXBUF;              // [2 kinds][2 buffers] codes and parameters as stored
-  static constexpr uint32_t RAWC = kPKV * HD / 2, RAWBUF = RAWC + kPKV * 4 * NG;
-  static constexpr uint32_t ROW = RAW + 4 * RAWBUF;            // [4][5][64]: key scale, e, 2^-e, position, out of sight from
+  static constexpr uint32_t RAW = VX + 2 * VXBUF;              // [2 buffers][keys, values] codes, then parameters, as stored
+  static constexpr uint32_t RAWC = kPKV * HD / 2, RAWP = kPKV * 4 * NG, RAWBUF = 2 * (RAWC + RAWP);
+  static constexpr uint32_t ROW = RAW + 2 * RAWBUF;            // [8][5][64]: key scale, e, 2^-e, position, out of sight from
   static constexpr uint32_t ROWBUF = 5 * kPKV * 4;
-  static constexpr uint32_t FULL = ROW + 4 * ROWBUF;           // [4][2]: every query sees all of 32 rows
-  static constexpr uint32_t RED = FULL + 32;                   // [3][2 halves][128]: maxima of even and odd steps, sums
+  static constexpr uint32_t FULL = ROW + 8 * ROWBUF;           // [8][2]: every query sees all of 32 rows
+  static constexpr uint32_t RED = FULL + 64;                   // [3][2 halves][128]: maxima of even and odd steps, sums
   static constexpr uint32_t RFAC = RED + 6 * kPRows * 4;       // [128] queries' scale
   static constexpr uint32_t BAR = RFAC + kPRows * 4;
   static constexpr uint32_t PRE = BAR + 256;                   // [kPTiles] cost of the tiles before
@@ -76,7 +77,7 @@ struct PromptShape {
 // Tensor memory columns. Of each 16 columns of scores, 8 take the weights' high terms and 8 the low ones.
 constexpr uint32_t kColS = 0, kColO = 128, kColSum = 272, kColQ = 416, kCols = 512;
 
-enum Bar { B_QFULL = 0, B_KFULL = 1, B_KFREE = 3, B_VFULL = 5, B_VFREE = 7, B_SFULL = 9, B_PFULL = 11, B_PDONE = 13, B_EFULL = 15, B_END = 19 };
+enum Bar { B_QFULL = 0, B_KFULL = 1, B_KFREE = 3, B_VFULL = 5, B_VFREE = 7, B_SFULL = 9, B_PFULL = 11, B_PDONE = 13, B_EFULL = 15, B_RFULL = 19, B_RFREE = 21, B_END = 23 };
 
 // D f32, A and B f16, both K-major
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int m, int n) {
@@ -96,6 +97,23 @@ __device__ __forceinline__ uint64_t smem_desc_wide128(const void* p, uint32_t n)
   return ((uint64_t)(smem_u32(p) & 0x3FFFFu) >> 4) | ((uint64_t)(n >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// Sleeps on the barrier for up to 0.1 ms: many warps wait here, and a poll takes issue slots from the others.
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 // One thread of a converged warp, the same one each time.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -260,7 +278,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
   if (tid == 0) {
     abort_word = 0;
     for (int i = 0; i <= B_END; ++i) {
-      const bool eight = i == B_QFULL || i == B_PFULL || i == B_PFULL + 1;
+      const bool eight = i == B_QFULL || i == B_PFULL || i == B_PFULL + 1 || i == B_RFREE || i == B_RFREE + 1;
       const bool four = i == B_KFULL || i == B_KFULL + 1 || i == B_VFULL || i == B_VFULL + 1 || (i >= B_EFULL && i < B_EFULL + 4);
       mbar_init(bar + i, eight ? 8 : four ? 4 : 1);
     }
@@ -288,8 +306,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     bool ok = false;
     const uint64_t t0 = globaltimer_ns();
     while (true) {
-#pragma unroll 1
-      for (int i = 0; i < 64 && !ok; ++i) ok = mbar_try_wait(bar + b, parity);
+      ok = mbar_try_wait_long(bar + b, parity);
       if (ok || *abort_flag) break;
       if (globaltimer_ns() - t0 > SHD_WAIT_LIMIT_NS) {
         *abort_flag = 1;
@@ -313,20 +330,20 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     bool ok = true;
     Segment sg;
     for (int64_t t = t_begin; next_segment(sg, pre, pa.tiles, sum, c.heads, t, t_end); t = sg.next) {
-      const int64_t r0 = (int64_t)sg.tile * kPRows, rows = (int64_t)a.M * G;
+      const int r0 = sg.tile * kPRows, rows = a.M * G;  // at most kPTiles * kPRows
       // queries as two terms of q * 2^k, |q| 2^k < 2^7, channels in the order of the key words: a warp
       // takes 16 rows, HD / 4 lanes a row; the high terms go to tensor memory by way of the low terms' place
 #pragma unroll 1
       for (int term = 0; term < 2; ++term) {
         constexpr int LPR = HD / 4, RPW = 32 / LPR;
         const int ql = lane % LPR;
-#pragma unroll 4
+#pragma unroll 1
         for (int i = 0; i < 16; i += RPW) {
           const int y = warp * 16 + i + lane / LPR;
-          const int64_t r = r0 + y;
+          const int r = r0 + y;
           float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
           if (r < rows)
-            v = *reinterpret_cast<const float4*>(a.q + (size_t)(r / G) * a.ldq + (size_t)(sg.head * G + (int)(r % G)) * HD + 4 * ql);
+            v = *reinterpret_cast<const float4*>(a.q + (size_t)(r / G) * a.ldq + (size_t)(sg.head * G + r % G) * HD + 4 * ql);
           float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
           float qs = __fadd_rn(__fadd_rn(v.x, v.y), __fadd_rn(v.z, v.w));
 #pragma unroll
@@ -383,9 +400,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       if (lane == 0) mbar_arrive(bar + B_QFULL);
       named_bar_sync(1, 256);  // rfac
 
-      const int64_t r = r0 + row;
-      const bool live = r < rows;
-      const int p = a.pos0 + (live ? (int)(r / G) : a.M - 1);
+      const bool live = r0 + row < rows;
+      const int p = a.pos0 + (live ? (r0 + row) / G : a.M - 1);
       const uint64_t rowf2 = pair(rfac[row], rfac[row]);
       float ref = kKv4Never;
       uint64_t l2 = pair(0.0f, 0.0f);
@@ -394,38 +410,42 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         const int b = it & 1;
         ok = ok && wait(B_EFULL + (it & 3), (it >> 2) & 1) && wait(B_SFULL + b, (it >> 1) & 1);
         tc_fence_after();
-        const float* rp = reinterpret_cast<const float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF) + 32 * half;
-        const int* full = reinterpret_cast<const int*>(smem + SH::FULL) + (it & 3) * 2;
+        const float* rp = reinterpret_cast<const float*>(smem + SH::ROW + (it & 7) * SH::ROWBUF) + 32 * half;
+        const int* full = reinterpret_cast<const int*>(smem + SH::FULL) + (it & 7) * 2;
         const uint32_t t_s = t_row + kColS + b * kPKV + 32 * half;
-        // score + e in log2 units of this half's 32 rows, and the row's maximum
-        uint32_t v0[16], v1[16];
-        tmem_ld16(t_s, v0);
-        tmem_ld16(t_s + 16, v1);
-        tmem_wait_ld();
-        tmem_loaded16(v0);
-        tmem_loaded16(v1);
-        float x[32];
+        // score + e in log2 units of this half's 32 rows, back to the same columns, and the row's maximum
+        float top = -INFINITY;
+        const bool masked = !full[half];
+#pragma unroll 1
+        for (int i = 0; i < 32; i += 16) {
+          uint32_t v[16];
+          tmem_ld16(t_s + i, v);
+          tmem_wait_ld();
+          tmem_loaded16(v);
+          float x[16];
 #pragma unroll
-        for (int y = 0; y < 32; y += 4) {
-          const ulonglong2 kf = *reinterpret_cast<const ulonglong2*>(rp + y), ve = *reinterpret_cast<const ulonglong2*>(rp + 64 + y);
-          const uint32_t* v = y < 16 ? v0 + y : v1 + (y - 16);
-          const float2 x0 = unpair(fma2(mul2(pair(__uint_as_float(v[0]), __uint_as_float(v[1])), rowf2), kf.x, ve.x));
-          const float2 x1 = unpair(fma2(mul2(pair(__uint_as_float(v[2]), __uint_as_float(v[3])), rowf2), kf.y, ve.y));
-          x[y] = x0.x; x[y + 1] = x0.y; x[y + 2] = x1.x; x[y + 3] = x1.y;
-        }
-        if (!full[half]) {
-#pragma unroll
-          for (int y = 0; y < 32; y += 4) {
-            const int4 from = *reinterpret_cast<const int4*>(rp + 192 + y), until = *reinterpret_cast<const int4*>(rp + 256 + y);
-            if (!(from.x <= p && p < until.x)) x[y] = -INFINITY;
-            if (!(from.y <= p && p < until.y)) x[y + 1] = -INFINITY;
-            if (!(from.z <= p && p < until.z)) x[y + 2] = -INFINITY;
-            if (!(from.w <= p && p < until.w)) x[y + 3] = -INFINITY;
+          for (int y = 0; y < 16; y += 4) {
+            const ulonglong2 kf = *reinterpret_cast<const ulonglong2*>(rp + i + y), ve = *reinterpret_cast<const ulonglong2*>(rp + 64 + i + y);
+            const float2 x0 = unpair(fma2(mul2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), rowf2), kf.x, ve.x));
+            const float2 x1 = unpair(fma2(mul2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), rowf2), kf.y, ve.y));
+            x[y] = x0.x; x[y + 1] = x0.y; x[y + 2] = x1.x; x[y + 3] = x1.y;
           }
-        }
-        float top = fmaxf(x[0], x[1]);
+          if (masked) {
 #pragma unroll
-        for (int y = 2; y < 32; y += 2) top = fmaxf(top, fmaxf(x[y], x[y + 1]));
+            for (int y = 0; y < 16; y += 4) {
+              const int4 from = *reinterpret_cast<const int4*>(rp + 192 + i + y), until = *reinterpret_cast<const int4*>(rp + 256 + i + y);
+              if (!(from.x <= p && p < until.x)) x[y] = -INFINITY;
+              if (!(from.y <= p && p < until.y)) x[y + 1] = -INFINITY;
+              if (!(from.z <= p && p < until.z)) x[y + 2] = -INFINITY;
+              if (!(from.w <= p && p < until.w)) x[y + 3] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < 16; y += 2) top = fmaxf(top, fmaxf(x[y], x[y + 1]));
+#pragma unroll
+          for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(x[y]);
+          tmem_st16(t_s + i, v);
+        }
         red[(2 * b + half) * kPRows + row] = top;
         named_bar_sync(4 + (warp & 3), 64);
         top = fmaxf(top, red[(2 * b + (half ^ 1)) * kPRows + row]);
@@ -437,21 +457,28 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           ref = now;
           l2 = mul2(l2, pair(al, al));
         }
+        tmem_wait_st();
         // weights as two f16 terms, over the scores; their sum without the rows' powers of two
         const uint64_t shift = pair(kHead - ref, kHead - ref);
+#pragma unroll 1
+        for (int i = 0; i < 32; i += 16) {
+          uint32_t v[16], w[16];
+          tmem_ld16(t_s + i, v);
+          tmem_wait_ld();
+          tmem_loaded16(v);
 #pragma unroll
-        for (int y = 0; y < 32; y += 4) {
-          const ulonglong2 ie = *reinterpret_cast<const ulonglong2*>(rp + 128 + y);
-          const float2 x0 = unpair(add2(pair(x[y], x[y + 1]), shift)), x1 = unpair(add2(pair(x[y + 2], x[y + 3]), shift));
-          const uint64_t w0 = pair(exp2_fast(x0.x), exp2_fast(x0.y)), w1 = pair(exp2_fast(x1.x), exp2_fast(x1.y));
-          l2 = fma2(w0, ie.x, l2);
-          l2 = fma2(w1, ie.y, l2);
-          uint32_t* w = y < 16 ? v0 : v1;
-          split_pair(w0, w[(y & 15) / 2], w[8 + (y & 15) / 2]);
-          split_pair(w1, w[(y & 15) / 2 + 1], w[8 + (y & 15) / 2 + 1]);
+          for (int y = 0; y < 16; y += 4) {
+            const ulonglong2 ie = *reinterpret_cast<const ulonglong2*>(rp + 128 + i + y);
+            const float2 x0 = unpair(add2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), shift));
+            const float2 x1 = unpair(add2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), shift));
+            const uint64_t w0 = pair(exp2_fast(x0.x), exp2_fast(x0.y)), w1 = pair(exp2_fast(x1.x), exp2_fast(x1.y));
+            l2 = fma2(w0, ie.x, l2);
+            l2 = fma2(w1, ie.y, l2);
+            split_pair(w0, w[y / 2], w[8 + y / 2]);
+            split_pair(w1, w[y / 2 + 1], w[8 + y / 2 + 1]);
+          }
+          tmem_st16(t_s + i, w);
         }
-        tmem_st16(t_s, v0);
-        tmem_st16(t_s + 16, v1);
         // every kPDrain steps the sums so far go to the second accumulator; both follow the reference
         const int step = j - sg.begin;
         const bool drain = step > 0 && step % kPDrain == 0;
@@ -551,11 +578,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         for (int i = lane / LPR; i < 32; i += 32 / LPR) {
           const int f = lane % LPR, g = g0 + f / (LPR / 2), ch = 32 * g + 4 * unit + 4 * (f % (LPR / 2));
           const int y = (warp & 3) * 32 + i;
-          const int64_t rr = r0 + y;
+          const int rr = r0 + y;
           if (rr >= rows) continue;
           const float4 v = *reinterpret_cast<const float4*>(stage + i * STRIDE + 4 * f);
           if (whole) {
-            const size_t to = (size_t)(rr / G) * a.H * HD + (size_t)(sg.head * G + (int)(rr % G)) * HD + ch;
+            const size_t to = (size_t)(rr / G) * a.H * HD + (size_t)(sg.head * G + rr % G) * HD + ch;
             const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + to) : make_float4(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<float4*>(a.out_c + to) =
                 make_float4(__fsub_rn(v.x, mk.x), __fsub_rn(v.y, mk.y), __fsub_rn(v.z, mk.z), __fsub_rn(v.w, mk.w));
@@ -572,168 +599,159 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
   } else if (warp < 16) {
     // ---- unpacking: keys (warps 8-11) or values (12-15), thread -> row th % 64, half th / 64 of its bytes --
     const bool vals = warp >= 12;
-    const int th = tid & 127, w4 = warp & 3, r = th & 63, kh = th >> 6;
-    const uint8_t* codes = vals ? c.vc : c.kc;
-    const uint8_t* params = reinterpret_cast<const uint8_t*>(vals ? c.vp : c.kp);
-    uint8_t* raws = smem + SH::RAW + (vals ? 2 * SH::RAWBUF : 0);
-    // a walk over the CTA's steps
-    struct Walk {
-      int64_t t;
-      Segment sg;
-      Kv4Spans sp;
-      size_t base;
-      int lo, hi, j;
-      bool live;
-    };
-    auto enter = [&](Walk& w) {
-      w.live = next_segment(w.sg, pre, pa.tiles, sum, c.heads, w.t, t_end);
-      if (!w.live) return;
-      tile_positions(a, w.sg.tile, G, w.lo, w.hi);
-      w.sp = kv4_spans(c, w.lo, w.hi, a.window);
-      w.base = kv4_base(c, a.slot0, w.sg.head);
-      w.j = w.sg.begin;
-    };
-    auto advance = [&](Walk& w) {
-      if (w.live && ++w.j == w.sg.end) {
-        w.t = w.sg.next;
-        enter(w);
-      }
-    };
-    // asynchronous copies of a step's rows as they are stored: warp w4 copies its w4-th chunk
-    constexpr int CPR = HD / 32, NC = kKv4Chunk * CPR, NP = kKv4Chunk * 4 * NG / 16;
-    auto fetch = [&](const Walk& w, int buf) {
-      const int x = w.j * (kPKV / kKv4Chunk) + w4;
-      if (w.live && x < w.sp.total) {
-        const size_t row0 = w.base + (size_t)kv4_span_chunk(w.sp, x) * kKv4Chunk;
-        uint8_t* raw = raws + buf * SH::RAWBUF;
-#pragma unroll
-        for (int i = 0; i < NC / 32; ++i) {
-          const int y = lane + 32 * i, rr = w4 * kKv4Chunk + y / CPR, q = y % CPR;
-          cp_async16(raw + (uint32_t)(rr * CPR + (HD == 128 ? q ^ ((rr >> 1) & 3) : q)) * 16, codes + row0 * (HD / 2) + y * 16, 16);
-        }
-        if (lane < NP) cp_async16(raw + SH::RAWC + w4 * (kKv4Chunk * 4 * NG) + lane * 16, params + row0 * (4 * NG) + lane * 16, 16);
-      }
-      cp_async_commit();
-    };
-    // after a wait that ran out the walk goes on without waiting: the four warps meet at their barrier
+    const int th = tid & 127, r = th & 63, kh = th >> 6;
+    int it = 0;
     bool ok = true;
-    Walk at{}, ahead{};
-    at.t = ahead.t = t_begin;
-    enter(at);
-    ahead = at;
-    fetch(ahead, 0);
-    advance(ahead);
-    for (int it = 0; at.live; ++it) {
-      const int b = it & 1;
-      const uint8_t* raw = raws + b * SH::RAWBUF;
-      cp_async_wait<0>();
-      named_bar_sync(vals ? 3 : 2, 128);  // this step's rows have landed, and nobody reads the last step's
-      fetch(ahead, b ^ 1);
-      advance(ahead);
-      // whether any query of the tile sees the row: at positions [from, until)
-      int from = 0x7fffffff, until = 0;
-      const int x = at.j * (kPKV / kKv4Chunk) + r / kKv4Chunk;
-      if (x < at.sp.total) {
-        const int row = kv4_span_chunk(at.sp, x) * kKv4Chunk + r % kKv4Chunk;
-        const int held = kv4_held(c, row, last);
-        const int64_t end = a.window > 0 && row >= c.sinks ? (int64_t)held + a.window : 0x7fffffff;
-        if ((row < c.sinks || held >= c.sinks) && held <= at.hi && end > at.lo) {
-          from = held;
-          until = (int)min(end, (int64_t)0x7fffffff);
-        }
-      }
-      uint32_t w[NG];
-      if constexpr (NG == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(raw + SH::RAWC + r * 16);
-        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(raw + SH::RAWC + r * 8);
-        w[0] = v.x; w[1] = v.y;
-      }
-      if (until == 0) {  // its parameters may be anything
-#pragma unroll
-        for (int g = 0; g < NG; ++g) w[g] = 0u;
-      }
-      RowParams<NG> q;
-      q.set(w, vals);
-      const float down = pow2i(-q.e), up9 = down * 512.0f;
-      float* rp = reinterpret_cast<float*>(smem + SH::ROW + (it & 3) * SH::ROWBUF);
-      const int free_bar = vals ? B_VFREE : B_KFREE;
-      if (vals) {
-        if (kh == 0) {
-          rp[64 + r] = (float)q.e;
-          rp[128 + r] = pow2i(-q.e);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar + B_EFULL + (it & 3));
-      }
-      ok = ok && (it < 2 || wait(free_bar + b, ((it - 2) >> 1) & 1));
-      if (kh == 0) {
-        if (!vals) {
-          uint32_t y[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-          for (int g = 0; g < NG; g += 2) {
-            y[g / 2] = pack_f16(q.s[g] * down, q.s[g + 1] * down);
-            y[NG / 2 + g / 2] = pack_f16(q.z[g] * down, q.z[g + 1] * down);
-          }
-          uint8_t* kx = smem + SH::KX + b * SH::KXBUF;
-          *reinterpret_cast<uint4*>(kx + plain16_offset(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
-          *reinterpret_cast<uint4*>(kx + plain16_offset(r, 1)) = make_uint4(y[0], y[1], y[2], y[3]);
-          rp[r] = pow2i(q.e);
-          reinterpret_cast<int*>(rp)[192 + r] = from;
-          reinterpret_cast<int*>(rp)[256 + r] = until;
-          const int full = __all_sync(0xffffffffu, from <= at.lo && at.hi < until);
-          if (lane == 0) reinterpret_cast<int*>(smem + SH::FULL)[(it & 3) * 2 + w4] = full;
-        } else {
-          // middles: column g the high term, 4 + g the low one
-          __half* vx = reinterpret_cast<__half*>(smem + SH::VX + b * SH::VXBUF + (r >> 3) * 256 + (r & 7) * 2);
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const float y = q.z[g] * down;
-            const __half h = __float2half_rn(y);
-            vx[g * 8] = h;
-            vx[(4 + g) * 8] = __float2half_rn(__fsub_rn(y, __half2float(h)));
-          }
-        }
-      }
-      uint8_t* to = smem + (vals ? SH::V : SH::K) + b * SH::BUF + (r >> 3) * 1024 + (r & 7) * 128;
-      __half2 s2[NG / 2];
-#pragma unroll
-      for (int g = 0; g < NG; g += 2) s2[g / 2] = __floats2half2_rn(q.s[g] * up9, q.s[g + 1] * up9);
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        uint32_t cw[NG];
+    Segment sg;
+    for (int64_t t = t_begin; ok && next_segment(sg, pre, pa.tiles, sum, c.heads, t, t_end); t = sg.next) {
+      for (int j = sg.begin; j < sg.end; ++j, ++it) {
+        const int b = it & 1;
+        const uint8_t* raw = smem + SH::RAW + b * SH::RAWBUF + (vals ? SH::RAWC : 0);
+        const uint8_t* rawp = smem + SH::RAW + b * SH::RAWBUF + 2 * SH::RAWC + (vals ? SH::RAWP : 0);
+        float* rp = reinterpret_cast<float*>(smem + SH::ROW + (it & 7) * SH::ROWBUF);
+        if (!(ok = wait(B_RFULL + b, (it >> 1) & 1))) break;
+        uint32_t w[NG];
         if constexpr (NG == 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 64 + (((2 * kh + x) ^ ((r >> 1) & 3)) << 4));
-          cw[0] = v.x; cw[1] = v.y; cw[2] = v.z; cw[3] = v.w;
+          const uint4 v = *reinterpret_cast<const uint4*>(rawp + r * 16);
+          w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
         } else {
-          const uint2 v = *reinterpret_cast<const uint2*>(raw + r * 32 + (2 * kh + x) * 8);
-          cw[0] = v.x; cw[1] = v.y;
+          const uint2 v = *reinterpret_cast<const uint2*>(rawp + r * 8);
+          w[0] = v.x; w[1] = v.y;
         }
+        if (reinterpret_cast<const int*>(rp)[256 + r] == 0) {  // no query sees it: its parameters may be anything
 #pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          // keys: word 2 kh + x of group i; values: unit (2 kh + x) NG / 2 + i / (NG / 2) (HD 64: 2 (2 kh + x)
-          // + i) of groups 2 (i % (NG / 2)), + 1
-          const int ublk = i % (NG / 2), unit = (2 * kh + x) * 2 + i / (NG / 2);
-          const int blk = vals ? ublk : i >> 1, chunk = vals ? unit : (i & 1) * 4 + 2 * kh + x;
-          const __half2 sv = vals ? s2[ublk] : ((i & 1) ? __high2half2(s2[i / 2]) : __low2half2(s2[i / 2]));
-          const uint32_t cwi = cw[i], c8 = cwi >> 8;
-          uint4 h, l;
-          scale_pair(centre_low(cwi), sv, h.x, l.x);
-          scale_pair(centre_high(cwi), sv, h.y, l.y);
-          scale_pair(centre_low(c8), sv, h.z, l.z);
-          scale_pair(centre_high(c8), sv, h.w, l.w);
-          uint8_t* y = to + blk * (kPKV * 128) + ((chunk ^ (r & 7)) << 4);
-          *reinterpret_cast<uint4*>(y) = h;
-          *reinterpret_cast<uint4*>(y + KB * kPKV * 128) = l;
+          for (int g = 0; g < NG; ++g) w[g] = 0u;
+        }
+        RowParams<NG> q;
+        q.set(w, vals);
+        const float down = pow2i(-q.e), up9 = down * 512.0f;
+        if (vals) {
+          if (kh == 0) {
+            rp[64 + r] = (float)q.e;
+            rp[128 + r] = pow2i(-q.e);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar + B_EFULL + (it & 3));
+        }
+        if (it >= 2 && !(ok = wait((vals ? B_VFREE : B_KFREE) + b, ((it - 2) >> 1) & 1))) break;
+        if (kh == 0) {
+          if (!vals) {
+            uint32_t y[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int g = 0; g < NG; g += 2) {
+              y[g / 2] = pack_f16(q.s[g] * down, q.s[g + 1] * down);
+              y[NG / 2 + g / 2] = pack_f16(q.z[g] * down, q.z[g + 1] * down);
+            }
+            uint8_t* kx = smem + SH::KX + b * SH::KXBUF;
+            *reinterpret_cast<uint4*>(kx + plain16_offset(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(kx + plain16_offset(r, 1)) = make_uint4(y[0], y[1], y[2], y[3]);
+            rp[r] = pow2i(q.e);
+          } else {
+            // middles: column g the high term, 4 + g the low one
+            __half* vx = reinterpret_cast<__half*>(smem + SH::VX + b * SH::VXBUF + (r >> 3) * 256 + (r & 7) * 2);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              const float y = q.z[g] * down;
+              const __half h = __float2half_rn(y);
+              vx[g * 8] = h;
+              vx[(4 + g) * 8] = __float2half_rn(__fsub_rn(y, __half2float(h)));
+            }
+          }
+        }
+        uint8_t* to = smem + (vals ? SH::V : SH::K) + b * SH::BUF + (r >> 3) * 1024 + (r & 7) * 128;
+        __half2 s2[NG / 2];
+#pragma unroll
+        for (int g = 0; g < NG; g += 2) s2[g / 2] = __floats2half2_rn(q.s[g] * up9, q.s[g + 1] * up9);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          // sixteenth (HD 64: eighth) part of the row's bytes; neighbouring rows take theirs in another
+          // order, so that the reads of 8 lanes fall into different banks
+          const int part = HD == 128 ? (2 * kh + x) ^ ((r >> 1) & 3) : 2 * kh + x;
+          uint32_t cw[NG];
+          if constexpr (NG == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 64 + part * 16);
+            cw[0] = v.x; cw[1] = v.y; cw[2] = v.z; cw[3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(raw + r * 32 + part * 8);
+            cw[0] = v.x; cw[1] = v.y;
+          }
+#pragma unroll
+          for (int i = 0; i < NG; ++i) {
+            // keys: word `part` of group i; values: unit 2 part + i / (NG / 2) of groups 2 (i % (NG / 2)), + 1
+            const int ublk = i % (NG / 2), unit = 2 * part + i / (NG / 2);
+            const int blk = vals ? ublk : i >> 1, chunk = vals ? unit : (i & 1) * 4 + part;
+            const __half2 sv = vals ? s2[ublk] : ((i & 1) ? __high2half2(s2[i / 2]) : __low2half2(s2[i / 2]));
+            const uint32_t cwi = cw[i], c8 = cwi >> 8;
+            uint4 h, l;
+            scale_pair(centre_low(cwi), sv, h.x, l.x);
+            scale_pair(centre_high(cwi), sv, h.y, l.y);
+            scale_pair(centre_low(c8), sv, h.z, l.z);
+            scale_pair(centre_high(c8), sv, h.w, l.w);
+            uint8_t* y = to + blk * (kPKV * 128) + ((chunk ^ (r & 7)) << 4);
+            *reinterpret_cast<uint4*>(y) = h;
+            *reinterpret_cast<uint4*>(y + KB * kPKV * 128) = l;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar + (vals ? B_VFULL : B_KFULL) + b);
+          mbar_arrive(bar + B_RFREE + b);
         }
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar + (vals ? B_VFULL : B_KFULL) + b);
-      advance(at);
     }
-    cp_async_wait<0>();
+  } else if (warp == 17) {
+    // ---- fetching: a step's chunks as they are stored, and from and until which position its rows are seen --
+    int it = 0;
+    bool ok = true;
+    Segment sg;
+    for (int64_t t = t_begin; ok && next_segment(sg, pre, pa.tiles, sum, c.heads, t, t_end); t = sg.next) {
+      int lo, hi;
+      tile_positions(a, sg.tile, G, lo, hi);
+      const Kv4Spans sp = kv4_spans(c, lo, hi, a.window);
+      const size_t base = kv4_base(c, a.slot0, sg.head);
+      for (int j = sg.begin; j < sg.end; ++j, ++it) {
+        const int b = it & 1;
+        if (it >= 2 && !(ok = wait(B_RFREE + b, ((it - 2) >> 1) & 1))) break;
+        const int x0 = j * (kPKV / kKv4Chunk), chunks = min(kPKV / kKv4Chunk, sp.total - x0);
+        int* rp = reinterpret_cast<int*>(smem + SH::ROW + (it & 7) * SH::ROWBUF);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = 32 * h + lane;
+          int from = 0x7fffffff, until = 0;
+          if (r / kKv4Chunk < chunks) {
+            const int row = kv4_span_chunk(sp, x0 + r / kKv4Chunk) * kKv4Chunk + r % kKv4Chunk;
+            const int held = kv4_held(c, row, last);
+            const int64_t end = a.window > 0 && row >= c.sinks ? (int64_t)held + a.window : 0x7fffffff;
+            if ((row < c.sinks || held >= c.sinks) && held <= hi && end > lo) {
+              from = held;
+              until = (int)min(end, (int64_t)0x7fffffff);
+            }
+          }
+          rp[192 + r] = from;
+          rp[256 + r] = until;
+          const int full = __all_sync(0xffffffffu, from <= lo && hi < until);
+          if (lane == 0) reinterpret_cast<int*>(smem + SH::FULL)[(it & 7) * 2 + h] = full;
+        }
+        constexpr uint32_t CODE = kKv4Chunk * HD / 2, PAR = kKv4Chunk * 4 * NG;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(bar + B_RFULL + b, chunks * 2 * (CODE + PAR));
+        __syncwarp();
+        if (lane < 16 && (lane & 3) < chunks) {
+          const size_t row0 = base + (size_t)kv4_span_chunk(sp, x0 + (lane & 3)) * kKv4Chunk;
+          const int kind = lane >> 2;  // key codes, value codes, key and value parameters
+          uint8_t* raw = smem + SH::RAW + b * SH::RAWBUF;
+          if (kind < 2)
+            bulk_copy(raw + kind * SH::RAWC + (lane & 3) * CODE, (kind ? c.vc : c.kc) + row0 * (HD / 2), CODE, bar + B_RFULL + b);
+          else
+            bulk_copy(raw + 2 * SH::RAWC + (kind - 2) * SH::RAWP + (lane & 3) * PAR,
+                      reinterpret_cast<const uint8_t*>(kind == 3 ? c.vp : c.kp) + row0 * (4 * NG), PAR, bar + B_RFULL + b);
+        }
+      }
+    }
+    // no copy is in flight when the block ends
+    for (int i = max(it - 2, 0); i < it; ++i)
+      if (lane == 0 && !mbar_wait_bounded(bar + B_RFULL + (i & 1), (i >> 1) & 1)) atomicOr(a.err, SHD_DEVERR_TIMEOUT_DRAIN);
   } else {
     // ---- MMAs: the whole warp walks, one elected thread issues --------------------------------------
     // Operands that the compiler knows to be the same in the warp (by way of the shuffles) keep an issue
