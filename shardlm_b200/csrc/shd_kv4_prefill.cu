@@ -4,14 +4,15 @@
 // A tile is 128 (position, head) pairs of one kv head, heads fastest, so that the heads of a group
 // share every unpacked row. It walks the rows that any of its positions sees, 64 at a time:
 //   S [128 x 64]       = Q [128 x HD] K^T      O [128 x HD] += P [128 x 64] V
-// Operands are f16 in two terms. A key row is divided by a power of two of its own and s (c - 7.5) is
-// then exactly two terms (11 + 5 bits); queries, weights and minima keep 22 bits of theirs. Three of the
+// Operands are f16 in two terms. The keys of 32 rows are divided by a power of two of theirs and
+// s (c - 7.5) is then exactly two terms (11 + 5 bits; of a row 2^19 smaller than the largest of the 32
+// the error is 2^-34 of the largest); queries, weights and minima keep 22 bits of theirs. Three of the
 // four term products are formed (the fourth is below 2^-22 of the sum), accumulated in f32 in
 // tensor memory. What the minima add,
 //   sum_g (z_tg + 7.5 s_tg) (sum_(i in g) q_i)    and    sum_t p_t (z_tg + 7.5 s_tg),
 // is one more step of 16 along the first product's depth (a row's parameters against the groups' query
-// sums) and 16 more columns of the second's width. A value row is divided by a power of two 2^e of
-// its own too, and its weight is 2^(score + e - ref): the running reference follows score + e, so no
+// sums) and 16 more columns of the second's width. 32 value rows are divided by a power of two 2^e of
+// theirs too, and their weights are 2^(score + e - ref): the running reference follows score + e, so no
 // product overflows f16 whatever the scales of the rows, and the softmax's sum takes 2^-e back out.
 //
 // Warps: 0-7 softmax (two threads share a row, half of its 64 scores each: scores come from tensor
@@ -62,10 +63,10 @@ struct PromptShape {
   static constexpr uint32_t VXBUF = kPKV * 32;
   static constexpr uint32_t RAW = VX + 2 * VXBUF;              // [2 buffers][keys, values] codes, then parameters, as stored
   static constexpr uint32_t RAWC = kPKV * HD / 2, RAWP = kPKV * 4 * NG, RAWBUF = 2 * (RAWC + RAWP);
-  static constexpr uint32_t ROW = RAW + 2 * RAWBUF;            // [8][5][64]: key scale, e, 2^-e, position, out of sight from
-  static constexpr uint32_t ROWBUF = 5 * kPKV * 4;
-  static constexpr uint32_t FULL = ROW + 8 * ROWBUF;           // [8][2]: every query sees all of 32 rows
-  static constexpr uint32_t RED = FULL + 64;                   // [3][2 halves][128]: maxima of even and odd steps, sums
+  static constexpr uint32_t ROW = RAW + 2 * RAWBUF;            // [8][2][64]: a row's position, out of sight from
+  static constexpr uint32_t ROWBUF = 2 * kPKV * 4;
+  static constexpr uint32_t OF32 = ROW + 8 * ROWBUF;           // [8][2][4], of 32 rows: 2^(key e), e, 2^-e, seen by every query
+  static constexpr uint32_t RED = OF32 + 8 * 2 * 16;                   // [3][2 halves][128]: maxima of even and odd steps, sums
   static constexpr uint32_t RFAC = RED + 6 * kPRows * 4;       // [128] queries' scale
   static constexpr uint32_t BAR = RFAC + kPRows * 4;
   static constexpr uint32_t PRE = BAR + 256;                   // [kPTiles] cost of the tiles before
@@ -159,8 +160,8 @@ __device__ __forceinline__ void scale_pair(__half2 c, __half2 s, uint32_t& hi, u
   lo = as_u32(__hfma2(s, c, __hneg2(h)));
 }
 
-// A row's parameters and the power of two that it is divided by: 8 s and |z| (values: |z + 7.5 s|) come
-// to at most 2^9.
+// A row's parameters and the power of two that it is divided by, which is that of its warp's 32 rows:
+// 8 s and |z| (values: |z + 7.5 s|) come to at most 2^9.
 template <int NG>
 struct RowParams {
   float s[NG], z[NG];
@@ -176,7 +177,7 @@ struct RowParams {
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) top = fmaxf(top, fmaxf(8.0f * s[g], fabsf(z[g])));
-    e = max(ceil_exp2(top), -40) - 9;
+    e = max(__reduce_max_sync(0xffffffffu, ceil_exp2(top)), -40) - 9;
   }
 };
 
@@ -333,37 +334,41 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       const int r0 = sg.tile * kPRows, rows = a.M * G;  // at most kPTiles * kPRows
       // queries as two terms of q * 2^k, |q| 2^k < 2^7, channels in the order of the key words: a warp
       // takes 16 rows, HD / 4 lanes a row; the high terms go to tensor memory by way of the low terms' place
-#pragma unroll 1
-      for (int term = 0; term < 2; ++term) {
-        constexpr int LPR = HD / 4, RPW = 32 / LPR;
-        const int ql = lane % LPR;
-#pragma unroll 1
-        for (int i = 0; i < 16; i += RPW) {
-          const int y = warp * 16 + i + lane / LPR;
-          const int r = r0 + y;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (r < rows)
-            v = *reinterpret_cast<const float4*>(a.q + (size_t)(r / G) * a.ldq + (size_t)(sg.head * G + r % G) * HD + 4 * ql);
-          float top = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
-          float qs = __fadd_rn(__fadd_rn(v.x, v.y), __fadd_rn(v.z, v.w));
+      {
+        constexpr int LPR = HD / 4, RPW = 32 / LPR, N = 16 / RPW;
+        const int ql = lane % LPR, y0 = warp * 16 + lane / LPR;
+        uint2 low[N];
 #pragma unroll
-          for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int i0 = 0; i0 < N; i0 += 4) {
+          float4 v[4];
 #pragma unroll
-          for (int o = 1; o < 8; o <<= 1) qs = __fadd_rn(qs, __shfl_xor_sync(0xffffffffu, qs, o));
-          const int k = max(min(7 - ceil_exp2(top), 100), -100);
-          const float up = pow2i(k);
-          // of 8 channels the even lane makes pairs (0, 4), (1, 5), the odd one (2, 6), (3, 7)
-          const bool odd = lane & 1;
-          const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.z, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v.y : v.w, 1);
-          uint2 hi, lo;
-          split_f16((odd ? s0 : v.x) * up, (odd ? v.z : s0) * up, hi.x, lo.x);
-          split_f16((odd ? s1 : v.y) * up, (odd ? v.w : s1) * up, hi.y, lo.y);
-          const int ch = 4 * ql;  // plane position of its 8 bytes
-          *reinterpret_cast<uint2*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(y, ch & 63)) = term ? lo : hi;
-          if (term) {
-            float q4[4];
+          for (int i = 0; i < 4; ++i) {
+            const int r = r0 + y0 + (i0 + i) * RPW;
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows)
+              v[i] = *reinterpret_cast<const float4*>(a.q + (size_t)(r / G) * a.ldq + (size_t)(sg.head * G + r % G) * HD + 4 * ql);
+          }
 #pragma unroll
-            for (int g = 0; g < 4; ++g) q4[g] = g < NG ? __shfl_sync(0xffffffffu, qs, (lane & ~(LPR - 1)) + 8 * (g % NG)) * up : 0.0f;
+          for (int i = 0; i < 4; ++i) {
+            const int y = y0 + (i0 + i) * RPW;
+            float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+            float qs = __fadd_rn(__fadd_rn(v[i].x, v[i].y), __fadd_rn(v[i].z, v[i].w));
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) qs = __fadd_rn(qs, __shfl_xor_sync(0xffffffffu, qs, o));
+            const int k = max(min(7 - ceil_exp2(top), 60), -60);  // 2^-k times a power of two of the keys stays normal
+            const float up = pow2i(k);
+            // of 8 channels the even lane makes pairs (0, 4), (1, 5), the odd one (2, 6), (3, 7)
+            const bool odd = lane & 1;
+            const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[i].x : v[i].z, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v[i].y : v[i].w, 1);
+            uint2 hi;
+            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, low[i0 + i].x);
+            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, low[i0 + i].y);
+            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = hi;
+            float q4[NG];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) q4[g] = __shfl_sync(0xffffffffu, qs, (lane & ~(LPR - 1)) + 8 * g) * up;
             if (ql == 0) {
               uint32_t h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};  // 7.5 x and 1 x the groups' sums
 #pragma unroll
@@ -377,22 +382,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             }
           }
         }
-        if (term == 0) {
-          named_bar_sync(1, 256);
+        named_bar_sync(1, 256);
 #pragma unroll
-          for (int x = 0; x < HD / 64; ++x) {
-            const int ch = half * (HD / 2) + 32 * x;  // 32 channels: 16 columns
-            uint32_t h[16];
+        for (int x = 0; x < HD / 64; ++x) {
+          const int ch = half * (HD / 2) + 32 * x;  // 32 channels: 16 columns
+          uint32_t h[16];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint4 v = *reinterpret_cast<const uint4*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(row, (ch & 63) + 8 * y));
-              h[4 * y] = v.x; h[4 * y + 1] = v.y; h[4 * y + 2] = v.z; h[4 * y + 3] = v.w;
-            }
-            tmem_st16(t_row + kColQ + ch / 2, h);
+          for (int y = 0; y < 4; ++y) {
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(row, (ch & 63) + 8 * y));
+            h[4 * y] = v.x; h[4 * y + 1] = v.y; h[4 * y + 2] = v.z; h[4 * y + 3] = v.w;
           }
-          tmem_wait_st();
-          named_bar_sync(1, 256);
+          tmem_st16(t_row + kColQ + ch / 2, h);
         }
+        tmem_wait_st();
+        named_bar_sync(1, 256);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y0 + i * RPW, (4 * ql) & 63)) = low[i];
       }
       tc_fence_before();
       fence_proxy_async_smem();
@@ -402,50 +408,41 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
 
       const bool live = r0 + row < rows;
       const int p = a.pos0 + (live ? (r0 + row) / G : a.M - 1);
-      const uint64_t rowf2 = pair(rfac[row], rfac[row]);
-      float ref = kKv4Never;
-      uint64_t l2 = pair(0.0f, 0.0f);
+      const float rowf = rfac[row];
+      float ref = kKv4Never, l = 0.0f;
       bool summed = false;  // the second accumulator holds something
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
         const int b = it & 1;
         ok = ok && wait(B_EFULL + (it & 3), (it >> 2) & 1) && wait(B_SFULL + b, (it >> 1) & 1);
         tc_fence_after();
-        const float* rp = reinterpret_cast<const float*>(smem + SH::ROW + (it & 7) * SH::ROWBUF) + 32 * half;
-        const int* full = reinterpret_cast<const int*>(smem + SH::FULL) + (it & 7) * 2;
+        const int* rp = reinterpret_cast<const int*>(smem + SH::ROW + (it & 7) * SH::ROWBUF) + 32 * half;
+        const float4 of32 = *reinterpret_cast<const float4*>(smem + SH::OF32 + ((it & 7) * 2 + half) * 16);
+        const bool masked = of32.w == 0.0f;
         const uint32_t t_s = t_row + kColS + b * kPKV + 32 * half;
-        // score + e in log2 units of this half's 32 rows, back to the same columns, and the row's maximum
-        float top = -INFINITY;
-        const bool masked = !full[half];
-#pragma unroll 1
-        for (int i = 0; i < 32; i += 16) {
-          uint32_t v[16];
-          tmem_ld16(t_s + i, v);
-          tmem_wait_ld();
-          tmem_loaded16(v);
-          float x[16];
+        // this half's 32 scores: score + e in log2 units is fac * v + of32.y
+        const float fac = rowf * of32.x;
+        uint32_t v[2][16];
+        tmem_ld16(t_s, v[0]);
+        tmem_ld16(t_s + 16, v[1]);
+        tmem_wait_ld();
+        tmem_loaded16(v[0]);
+        tmem_loaded16(v[1]);
+        if (masked) {  // fac > 0: a value of -inf weighs 0
 #pragma unroll
-          for (int y = 0; y < 16; y += 4) {
-            const ulonglong2 kf = *reinterpret_cast<const ulonglong2*>(rp + i + y), ve = *reinterpret_cast<const ulonglong2*>(rp + 64 + i + y);
-            const float2 x0 = unpair(fma2(mul2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), rowf2), kf.x, ve.x));
-            const float2 x1 = unpair(fma2(mul2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), rowf2), kf.y, ve.y));
-            x[y] = x0.x; x[y + 1] = x0.y; x[y + 2] = x1.x; x[y + 3] = x1.y;
+          for (int y = 0; y < 32; y += 4) {
+            const int4 from = *reinterpret_cast<const int4*>(rp + y), until = *reinterpret_cast<const int4*>(rp + 64 + y);
+            uint32_t* w = &v[y / 16][y % 16];
+            if (!(from.x <= p && p < until.x)) w[0] = 0xff800000u;
+            if (!(from.y <= p && p < until.y)) w[1] = 0xff800000u;
+            if (!(from.z <= p && p < until.z)) w[2] = 0xff800000u;
+            if (!(from.w <= p && p < until.w)) w[3] = 0xff800000u;
           }
-          if (masked) {
-#pragma unroll
-            for (int y = 0; y < 16; y += 4) {
-              const int4 from = *reinterpret_cast<const int4*>(rp + 192 + i + y), until = *reinterpret_cast<const int4*>(rp + 256 + i + y);
-              if (!(from.x <= p && p < until.x)) x[y] = -INFINITY;
-              if (!(from.y <= p && p < until.y)) x[y + 1] = -INFINITY;
-              if (!(from.z <= p && p < until.z)) x[y + 2] = -INFINITY;
-              if (!(from.w <= p && p < until.w)) x[y + 3] = -INFINITY;
-            }
-          }
-#pragma unroll
-          for (int y = 0; y < 16; y += 2) top = fmaxf(top, fmaxf(x[y], x[y + 1]));
-#pragma unroll
-          for (int y = 0; y < 16; ++y) v[y] = __float_as_uint(x[y]);
-          tmem_st16(t_s + i, v);
         }
+        float top = __uint_as_float(v[0][0]);
+#pragma unroll
+        for (int y = 1; y < 31; y += 2)
+          top = fmaxf(top, fmaxf(__uint_as_float(v[y / 16][y % 16]), __uint_as_float(v[(y + 1) / 16][(y + 1) % 16])));
+        top = fmaf(fmaxf(top, __uint_as_float(v[1][15])), fac, of32.y);
         red[(2 * b + half) * kPRows + row] = top;
         named_bar_sync(4 + (warp & 3), 64);
         top = fmaxf(top, red[(2 * b + (half ^ 1)) * kPRows + row]);
@@ -455,30 +452,26 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           const float now = fmaxf(ref, top);
           al = exp2_fast(ref - now);
           ref = now;
-          l2 = mul2(l2, pair(al, al));
+          l *= al;
         }
-        tmem_wait_st();
-        // weights as two f16 terms, over the scores; their sum without the rows' powers of two
-        const uint64_t shift = pair(kHead - ref, kHead - ref);
-#pragma unroll 1
-        for (int i = 0; i < 32; i += 16) {
-          uint32_t v[16], w[16];
-          tmem_ld16(t_s + i, v);
-          tmem_wait_ld();
-          tmem_loaded16(v);
+        // weights as two f16 terms, over the scores; their sum without 2^e
+        const float sh = of32.y + (kHead - ref);
+        const uint64_t shift = pair(sh, sh), fac2 = pair(fac, fac);
+        uint64_t sum = pair(0.0f, 0.0f);
 #pragma unroll
-          for (int y = 0; y < 16; y += 4) {
-            const ulonglong2 ie = *reinterpret_cast<const ulonglong2*>(rp + 128 + i + y);
-            const float2 x0 = unpair(add2(pair(__uint_as_float(v[y]), __uint_as_float(v[y + 1])), shift));
-            const float2 x1 = unpair(add2(pair(__uint_as_float(v[y + 2]), __uint_as_float(v[y + 3])), shift));
-            const uint64_t w0 = pair(exp2_fast(x0.x), exp2_fast(x0.y)), w1 = pair(exp2_fast(x1.x), exp2_fast(x1.y));
-            l2 = fma2(w0, ie.x, l2);
-            l2 = fma2(w1, ie.y, l2);
-            split_pair(w0, w[y / 2], w[8 + y / 2]);
-            split_pair(w1, w[y / 2 + 1], w[8 + y / 2 + 1]);
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[16];
+#pragma unroll
+          for (int y = 0; y < 16; y += 2) {
+            const float2 x = unpair(fma2(pair(__uint_as_float(v[i][y]), __uint_as_float(v[i][y + 1])), fac2, shift));
+            const uint64_t w2 = pair(exp2_fast(x.x), exp2_fast(x.y));
+            sum = add2(sum, w2);
+            split_pair(w2, w[y / 2], w[8 + y / 2]);
           }
-          tmem_st16(t_s + i, w);
+          tmem_st16(t_s + 16 * i, w);
         }
+        const float2 sum2 = unpair(sum);
+        l = fmaf(sum2.x + sum2.y, of32.z, l);
         // every kPDrain steps the sums so far go to the second accumulator; both follow the reference
         const int step = j - sg.begin;
         const bool drain = step > 0 && step % kPDrain == 0;
@@ -500,13 +493,21 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
 #pragma unroll
               for (int y = 0; y < 16; ++y) s[y] = 0u;
             }
+            if (drain) {
 #pragma unroll
-            for (int y = 0; y < 16; y += 2) {
-              uint64_t ov = pair(__uint_as_float(o[y]), __uint_as_float(o[y + 1])), sv = pair(__uint_as_float(s[y]), __uint_as_float(s[y + 1]));
-              if (drain) sv = add2(sv, ov);
-              const float2 so = unpair(mul2(sv, al2)), oo = unpair(mul2(ov, al2));
-              s[y] = __float_as_uint(so.x); s[y + 1] = __float_as_uint(so.y);
-              o[y] = __float_as_uint(oo.x); o[y + 1] = __float_as_uint(oo.y);
+              for (int y = 0; y < 16; y += 2) {
+                const float2 f = unpair(add2(pair(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), pair(__uint_as_float(o[y]), __uint_as_float(o[y + 1]))));
+                s[y] = __float_as_uint(f.x); s[y + 1] = __float_as_uint(f.y);
+              }
+            }
+            if (grow) {
+#pragma unroll
+              for (int y = 0; y < 16; y += 2) {
+                const float2 f = unpair(mul2(pair(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), al2));
+                const float2 h = unpair(mul2(pair(__uint_as_float(o[y]), __uint_as_float(o[y + 1])), al2));
+                s[y] = __float_as_uint(f.x); s[y + 1] = __float_as_uint(f.y);
+                o[y] = __float_as_uint(h.x); o[y + 1] = __float_as_uint(h.y);
+              }
             }
             if (summed || drain) tmem_st16(t_row + kColSum + i, s);
             if (!drain) tmem_st16(t_row + kColO + i, o);
@@ -522,10 +523,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       // the rows' results, or their parts: 2 SC columns of a half's at a time through the queries' place
       ok = ok && wait(B_PDONE + ((it - 1) & 1), ((it - 1) >> 1) & 1);
       tc_fence_after();
-      const float2 lv = unpair(l2);
-      red[(4 + half) * kPRows + row] = lv.x + lv.y;
+      red[(4 + half) * kPRows + row] = l;
       named_bar_sync(1, 256);  // also: every warp is past its queries
-      const float l = __fadd_rn(red[4 * kPRows + row], red[5 * kPRows + row]);
+      l = __fadd_rn(red[4 * kPRows + row], red[5 * kPRows + row]);
       const bool whole = sg.begin == 0 && sg.end == sg.steps;
       const float inv = whole ? __frcp_rn(l == 0.0f ? 1.0f : l) : 1.0f;
       float* parts = pa.parts + ((size_t)blockIdx.x * 2 + (t == t_begin ? 0 : 1)) * kPRows * SH::PART;
@@ -608,7 +608,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         const int b = it & 1;
         const uint8_t* raw = smem + SH::RAW + b * SH::RAWBUF + (vals ? SH::RAWC : 0);
         const uint8_t* rawp = smem + SH::RAW + b * SH::RAWBUF + 2 * SH::RAWC + (vals ? SH::RAWP : 0);
-        float* rp = reinterpret_cast<float*>(smem + SH::ROW + (it & 7) * SH::ROWBUF);
+        const int* rp = reinterpret_cast<const int*>(smem + SH::ROW + (it & 7) * SH::ROWBUF);
+        float* of32 = reinterpret_cast<float*>(smem + SH::OF32 + ((it & 7) * 2 + (warp & 1)) * 16);
         if (!(ok = wait(B_RFULL + b, (it >> 1) & 1))) break;
         uint32_t w[NG];
         if constexpr (NG == 4) {
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           const uint2 v = *reinterpret_cast<const uint2*>(rawp + r * 8);
           w[0] = v.x; w[1] = v.y;
         }
-        if (reinterpret_cast<const int*>(rp)[256 + r] == 0) {  // no query sees it: its parameters may be anything
+        if (rp[64 + r] == 0) {  // no query sees it: its parameters may be anything
 #pragma unroll
           for (int g = 0; g < NG; ++g) w[g] = 0u;
         }
@@ -626,12 +627,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         q.set(w, vals);
         const float down = pow2i(-q.e), up9 = down * 512.0f;
         if (vals) {
-          if (kh == 0) {
-            rp[64 + r] = (float)q.e;
-            rp[128 + r] = pow2i(-q.e);
+          if (lane == 0) {
+            if (kh == 0) {
+              of32[1] = (float)q.e;
+              of32[2] = pow2i(-q.e);
+            }
+            mbar_arrive(bar + B_EFULL + (it & 3));
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar + B_EFULL + (it & 3));
         }
         if (it >= 2 && !(ok = wait((vals ? B_VFREE : B_KFREE) + b, ((it - 2) >> 1) & 1))) break;
         if (kh == 0) {
@@ -645,7 +647,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             uint8_t* kx = smem + SH::KX + b * SH::KXBUF;
             *reinterpret_cast<uint4*>(kx + plain16_offset(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
             *reinterpret_cast<uint4*>(kx + plain16_offset(r, 1)) = make_uint4(y[0], y[1], y[2], y[3]);
-            rp[r] = pow2i(q.e);
+            if (lane == 0) of32[0] = pow2i(q.e);
           } else {
             // middles: column g the high term, 4 + g the low one
             __half* vx = reinterpret_cast<__half*>(smem + SH::VX + b * SH::VXBUF + (r >> 3) * 256 + (r & 7) * 2);
@@ -664,9 +666,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         for (int g = 0; g < NG; g += 2) s2[g / 2] = __floats2half2_rn(q.s[g] * up9, q.s[g + 1] * up9);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          // sixteenth (HD 64: eighth) part of the row's bytes; neighbouring rows take theirs in another
-          // order, so that the reads of 8 lanes fall into different banks
-          const int part = HD == 128 ? (2 * kh + x) ^ ((r >> 1) & 3) : 2 * kh + x;
+          // a quarter of the row's bytes; of keys neighbouring rows take theirs in another order, so that
+          // the reads of 8 lanes fall into different banks (values would then collide where they go)
+          const int part = HD == 128 && !vals ? (2 * kh + x) ^ ((r >> 1) & 3) : 2 * kh + x;
           uint32_t cw[NG];
           if constexpr (NG == 4) {
             const uint4 v = *reinterpret_cast<const uint4*>(raw + r * 64 + part * 16);
@@ -728,10 +730,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
               until = (int)min(end, (int64_t)0x7fffffff);
             }
           }
-          rp[192 + r] = from;
-          rp[256 + r] = until;
+          rp[r] = from;
+          rp[64 + r] = until;
           const int full = __all_sync(0xffffffffu, from <= lo && hi < until);
-          if (lane == 0) reinterpret_cast<int*>(smem + SH::FULL)[(it & 7) * 2 + h] = full;
+          if (lane == 0) reinterpret_cast<float*>(smem + SH::OF32)[((it & 7) * 2 + h) * 4 + 3] = full ? 1.0f : 0.0f;
         }
         constexpr uint32_t CODE = kKv4Chunk * HD / 2, PAR = kKv4Chunk * 4 * NG;
         __syncwarp();
