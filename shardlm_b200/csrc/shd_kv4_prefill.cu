@@ -51,7 +51,6 @@ template <int HD>
 struct PromptShape {
   static constexpr int NG = HD / kKv4Group;
   static constexpr int KB = HD / 64;            // 64-channel blocks
-  static constexpr int NV = HD + 16;            // columns of O: channels (see o_channel) and minima
   static constexpr uint32_t QL = 0;             // [KB][128 rows][128 B]: low terms of the queries
   static constexpr uint32_t QX = QL + KB * kPRows * 128;       // [128 rows][32 B]: query sums
   static constexpr uint32_t K = QX + kPRows * 32;              // [2 buffers][2 terms][KB][64 rows][128 B]
@@ -186,6 +185,7 @@ struct PromptArgs {
   float* parts;    // [CTA][2][128][PART]
   int tiles;       // of a kv head
   int last;        // newest position written
+  uint32_t per_group;  // 2^32 / G, rounded up (0 for G = 1): r / G = high word of the product for r < 2^18
 };
 
 // Positions of a tile's first and last row.
@@ -304,8 +304,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
 
   // Bounded wait of one thread; false: it ran out here or elsewhere, and the CTA gives up.
   auto wait_one = [&](int b, uint32_t parity) -> bool {
-    bool ok = false;
-    const uint64_t t0 = globaltimer_ns();
+    bool ok = mbar_try_wait(bar + b, parity);
+    if (ok) return true;
+    const uint64_t t0 = globaltimer_ns();  // some 200 clocks: not read for a phase that is complete
     while (true) {
       ok = mbar_try_wait_long(bar + b, parity);
       if (ok || *abort_flag) break;
@@ -317,11 +318,14 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     }
     return ok;
   };
+  auto group_of = [&](int r) -> int { return pa.per_group ? (int)__umulhi((uint32_t)r, pa.per_group) : r; };
   // The same for a whole warp.
   auto wait = [&](int b, uint32_t parity) -> bool { return __all_sync(0xffffffffu, wait_one(b, parity)); };
 
   if (warp < 8) {
     // ---- softmax ------------------------------------------------------------------------------
+    // registers of the block: 256 x 120 + 256 x 72 + 64 x 96 = 576 x 96, as launched
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
     // After a wait that ran out the walk goes on without waiting: the warps meet at their barriers.
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_row = tbase + ((uint32_t)((warp & 3) * 32) << 16);
@@ -337,16 +341,34 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       {
         constexpr int LPR = HD / 4, RPW = 32 / LPR, N = 16 / RPW;
         const int ql = lane % LPR, y0 = warp * 16 + lane / LPR;
-        uint2 low[N];
+        auto high_terms = [&]() {
+          named_bar_sync(1, 256);
 #pragma unroll
-        for (int i0 = 0; i0 < N; i0 += 4) {
+          for (int x = 0; x < HD / 64; ++x) {
+            const int ch = half * (HD / 2) + 32 * x;  // 32 channels: 16 columns
+            uint32_t h[16];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const uint4 v = *reinterpret_cast<const uint4*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(row, (ch & 63) + 8 * y));
+              h[4 * y] = v.x; h[4 * y + 1] = v.y; h[4 * y + 2] = v.z; h[4 * y + 3] = v.w;
+            }
+            tmem_st16(t_row + kColQ + ch / 2, h);
+          }
+          tmem_wait_st();
+          named_bar_sync(1, 256);
+        };
+#pragma unroll 1
+        for (int x = 0; x < 2 * N; x += 4) {  // high terms, then (the rows again) low ones
+          const int i0 = x % N;
+          const bool low = x >= N;
+          if (x == N) high_terms();
           float4 v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = r0 + y0 + (i0 + i) * RPW;
             v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < rows)
-              v[i] = *reinterpret_cast<const float4*>(a.q + (size_t)(r / G) * a.ldq + (size_t)(sg.head * G + r % G) * HD + 4 * ql);
+              v[i] = *reinterpret_cast<const float4*>(a.q + (size_t)group_of(r) * a.ldq + (size_t)(sg.head * G + r - group_of(r) * G) * HD + 4 * ql);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -362,10 +384,11 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             // of 8 channels the even lane makes pairs (0, 4), (1, 5), the odd one (2, 6), (3, 7)
             const bool odd = lane & 1;
             const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[i].x : v[i].z, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v[i].y : v[i].w, 1);
-            uint2 hi;
-            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, low[i0 + i].x);
-            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, low[i0 + i].y);
-            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = hi;
+            uint2 hi, lo;
+            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, lo.x);
+            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, lo.y);
+            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = low ? lo : hi;
+            if (!low) continue;
             float q4[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) q4[g] = __shfl_sync(0xffffffffu, qs, (lane & ~(LPR - 1)) + 8 * g) * up;
@@ -382,23 +405,6 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             }
           }
         }
-        named_bar_sync(1, 256);
-#pragma unroll
-        for (int x = 0; x < HD / 64; ++x) {
-          const int ch = half * (HD / 2) + 32 * x;  // 32 channels: 16 columns
-          uint32_t h[16];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const uint4 v = *reinterpret_cast<const uint4*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(row, (ch & 63) + 8 * y));
-            h[4 * y] = v.x; h[4 * y + 1] = v.y; h[4 * y + 2] = v.z; h[4 * y + 3] = v.w;
-          }
-          tmem_st16(t_row + kColQ + ch / 2, h);
-        }
-        tmem_wait_st();
-        named_bar_sync(1, 256);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y0 + i * RPW, (4 * ql) & 63)) = low[i];
       }
       tc_fence_before();
       fence_proxy_async_smem();
@@ -407,7 +413,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       named_bar_sync(1, 256);  // rfac
 
       const bool live = r0 + row < rows;
-      const int p = a.pos0 + (live ? (r0 + row) / G : a.M - 1);
+      const int p = a.pos0 + (live ? group_of(r0 + row) : a.M - 1);
       const float rowf = rfac[row];
       float ref = kKv4Never, l = 0.0f;
       bool summed = false;  // the second accumulator holds something
@@ -427,7 +433,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         tmem_wait_ld();
         tmem_loaded16(v[0]);
         tmem_loaded16(v[1]);
-        if (masked) {  // fac > 0: a value of -inf weighs 0
+        auto mask_scores = [&]() {  // fac > 0: a value of -inf weighs 0
 #pragma unroll
           for (int y = 0; y < 32; y += 4) {
             const int4 from = *reinterpret_cast<const int4*>(rp + y), until = *reinterpret_cast<const int4*>(rp + 64 + y);
@@ -437,13 +443,48 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             if (!(from.z <= p && p < until.z)) w[2] = 0xff800000u;
             if (!(from.w <= p && p < until.w)) w[3] = 0xff800000u;
           }
-        }
-        float top = __uint_as_float(v[0][0]);
+        };
+        if (masked) mask_scores();
+        float t4[4];  // short chains: a dependent instruction takes 8 clocks here
 #pragma unroll
-        for (int y = 1; y < 31; y += 2)
-          top = fmaxf(top, fmaxf(__uint_as_float(v[y / 16][y % 16]), __uint_as_float(v[(y + 1) / 16][(y + 1) % 16])));
-        top = fmaf(fmaxf(top, __uint_as_float(v[1][15])), fac, of32.y);
+        for (int y = 0; y < 4; ++y) t4[y] = __uint_as_float(v[0][y]);
+#pragma unroll
+        for (int y = 4; y < 32; y += 8)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float e = y + 4 + x < 32 ? __uint_as_float(v[((y + 4 + x) % 32) / 16][(y + 4 + x) % 16]) : -INFINITY;
+            t4[x] = fmaxf(t4[x], fmaxf(__uint_as_float(v[(y + x) / 16][(y + x) % 16]), e));
+          }
+        float top = fmaf(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), fac, of32.y);
         red[(2 * b + half) * kPRows + row] = top;
+        // weights as two f16 terms (in the scores' places: high terms of 16 first), and their sum without 2^e
+        float part = 0.0f;
+        auto weigh = [&]() {
+          const float sh = of32.y + (kHead - ref);
+          const uint64_t shift = pair(sh, sh), fac2 = pair(fac, fac);
+          uint64_t s0 = pair(0.0f, 0.0f), s1 = s0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t w[16];
+#pragma unroll
+            for (int y = 0; y < 16; y += 4) {
+              const float2 x0 = unpair(fma2(pair(__uint_as_float(v[i][y]), __uint_as_float(v[i][y + 1])), fac2, shift));
+              const float2 x1 = unpair(fma2(pair(__uint_as_float(v[i][y + 2]), __uint_as_float(v[i][y + 3])), fac2, shift));
+              const uint64_t w0 = pair(exp2_fast(x0.x), exp2_fast(x0.y)), w1 = pair(exp2_fast(x1.x), exp2_fast(x1.y));
+              s0 = add2(s0, w0);
+              s1 = add2(s1, w1);
+              split_pair(w0, w[y / 2], w[8 + y / 2]);
+              split_pair(w1, w[y / 2 + 1], w[8 + y / 2 + 1]);
+            }
+#pragma unroll
+            for (int y = 0; y < 16; ++y) v[i][y] = w[y];
+          }
+          const float2 f = unpair(add2(s0, s1));
+          part = f.x + f.y;
+        };
+        // under the reference as it is, while the other half's maximum is on its way; again, rarely, when
+        // the reference has to grow
+        if (j > sg.begin) weigh();
         named_bar_sync(4 + (warp & 3), 64);
         top = fmaxf(top, red[(2 * b + (half ^ 1)) * kPRows + row]);
         float al = 1.0f;
@@ -454,24 +495,20 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           ref = now;
           l *= al;
         }
-        // weights as two f16 terms, over the scores; their sum without 2^e
-        const float sh = of32.y + (kHead - ref);
-        const uint64_t shift = pair(sh, sh), fac2 = pair(fac, fac);
-        uint64_t sum = pair(0.0f, 0.0f);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t w[16];
-#pragma unroll
-          for (int y = 0; y < 16; y += 2) {
-            const float2 x = unpair(fma2(pair(__uint_as_float(v[i][y]), __uint_as_float(v[i][y + 1])), fac2, shift));
-            const uint64_t w2 = pair(exp2_fast(x.x), exp2_fast(x.y));
-            sum = add2(sum, w2);
-            split_pair(w2, w[y / 2], w[8 + y / 2]);
+        if (grow || j == sg.begin) {
+          if (j > sg.begin) {
+            tmem_ld16(t_s, v[0]);
+            tmem_ld16(t_s + 16, v[1]);
+            tmem_wait_ld();
+            tmem_loaded16(v[0]);
+            tmem_loaded16(v[1]);
+            if (masked) mask_scores();
           }
-          tmem_st16(t_s + 16 * i, w);
+          weigh();
         }
-        const float2 sum2 = unpair(sum);
-        l = fmaf(sum2.x + sum2.y, of32.z, l);
+        l = fmaf(part, of32.z, l);
+        tmem_st16(t_s, v[0]);
+        tmem_st16(t_s + 16, v[1]);
         // every kPDrain steps the sums so far go to the second accumulator; both follow the reference
         const int step = j - sg.begin;
         const bool drain = step > 0 && step % kPDrain == 0;
@@ -479,9 +516,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           ok = ok && wait(B_PDONE + (b ^ 1), ((it - 1) >> 1) & 1);
           tc_fence_after();
           const uint64_t al2 = pair(al, al);
-          const int end = half ? SH::NV : HD / 2;
+          const int end = half ? HD + 16 : HD / 2;
 #pragma unroll 1
-          for (int i = half ? HD / 2 : 0; i < end; i += 16) {
+          for (int i = half * (HD / 2); i < end; i += 16) {
             uint32_t o[16], s[16];
             tmem_ld16(t_row + kColO + i, o);
             if (summed) tmem_ld16(t_row + kColSum + i, s);
@@ -493,21 +530,13 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
 #pragma unroll
               for (int y = 0; y < 16; ++y) s[y] = 0u;
             }
-            if (drain) {
 #pragma unroll
-              for (int y = 0; y < 16; y += 2) {
-                const float2 f = unpair(add2(pair(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), pair(__uint_as_float(o[y]), __uint_as_float(o[y + 1]))));
-                s[y] = __float_as_uint(f.x); s[y + 1] = __float_as_uint(f.y);
-              }
-            }
-            if (grow) {
-#pragma unroll
-              for (int y = 0; y < 16; y += 2) {
-                const float2 f = unpair(mul2(pair(__uint_as_float(s[y]), __uint_as_float(s[y + 1])), al2));
-                const float2 h = unpair(mul2(pair(__uint_as_float(o[y]), __uint_as_float(o[y + 1])), al2));
-                s[y] = __float_as_uint(f.x); s[y + 1] = __float_as_uint(f.y);
-                o[y] = __float_as_uint(h.x); o[y + 1] = __float_as_uint(h.y);
-              }
+            for (int y = 0; y < 16; y += 2) {
+              uint64_t ov = pair(__uint_as_float(o[y]), __uint_as_float(o[y + 1])), sv = pair(__uint_as_float(s[y]), __uint_as_float(s[y + 1]));
+              if (drain) sv = add2(sv, ov);
+              const float2 f = unpair(mul2(sv, al2)), h = unpair(mul2(ov, al2));
+              s[y] = __float_as_uint(f.x); s[y + 1] = __float_as_uint(f.y);
+              o[y] = __float_as_uint(h.x); o[y + 1] = __float_as_uint(h.y);
             }
             if (summed || drain) tmem_st16(t_row + kColSum + i, s);
             if (!drain) tmem_st16(t_row + kColO + i, o);
@@ -582,7 +611,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           if (rr >= rows) continue;
           const float4 v = *reinterpret_cast<const float4*>(stage + i * STRIDE + 4 * f);
           if (whole) {
-            const size_t to = (size_t)(rr / G) * a.H * HD + (size_t)(sg.head * G + rr % G) * HD + ch;
+            const int mm = group_of(rr);
+            const size_t to = (size_t)mm * a.H * HD + (size_t)(sg.head * G + rr - mm * G) * HD + ch;
             const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + to) : make_float4(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<float4*>(a.out_c + to) =
                 make_float4(__fsub_rn(v.x, mk.x), __fsub_rn(v.y, mk.y), __fsub_rn(v.z, mk.z), __fsub_rn(v.w, mk.w));
@@ -598,6 +628,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     }
   } else if (warp < 16) {
     // ---- unpacking: keys (warps 8-11) or values (12-15), thread -> row th % 64, half th / 64 of its bytes --
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const bool vals = warp >= 12;
     const int th = tid & 127, r = th & 63, kh = th >> 6;
     int it = 0;
@@ -929,6 +960,7 @@ int launch_prefill_t(shd_ctx* ctx, const Kv4AttnArgs& a0) {
     pa.a.out_c += m * width;
     pa.a.out_s += m * width;
     pa.last = a0.pos0 + a0.M - 1;
+    pa.per_group = G == 1 ? 0u : (uint32_t)(((1ull << 32) + G - 1) / G);
     pa.parts = ctx->d_kv4_parts;
     pa.tiles = (int)(((int64_t)pa.a.M * G + kPRows - 1) / kPRows);
     SHD_CHECK_CUDA(ctx, launch_pdl(kv4_prefill_kernel<HD>, dim3(ctas), dim3(kPThreads), SH::SMEM, ctx->stream, pa));
