@@ -43,7 +43,7 @@ constexpr int kPRows = 128;    // (position, head) pairs of a tile
 constexpr int kPKV = 64;       // cache rows of a step
 constexpr int kPThreads = 576;
 constexpr int kPTiles = 2048;  // tiles a launch (their step counts are in shared memory)
-constexpr int kPItem = 3;      // cost of an item's queries and results, in steps
+constexpr int kPItem = 8;      // cost of an item's queries and results, in steps
 constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
 constexpr float kRoom = 8.0f, kHead = 6.0f;  // weights are 2^(score' - ref + 6), score' - ref <= 8
 
@@ -357,21 +357,19 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           tmem_wait_st();
           named_bar_sync(1, 256);
         };
-#pragma unroll 1
-        for (int x = 0; x < 2 * N; x += 4) {  // high terms, then (the rows again) low ones
-          const int i0 = x % N;
-          const bool low = x >= N;
-          if (x == N) high_terms();
-          float4 v[4];
+        uint2 low[N];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+        for (int i0 = 0; i0 < N; i0 += 8) {
+          float4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
             const int r = r0 + y0 + (i0 + i) * RPW;
             v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < rows)
               v[i] = *reinterpret_cast<const float4*>(a.q + (size_t)group_of(r) * a.ldq + (size_t)(sg.head * G + r - group_of(r) * G) * HD + 4 * ql);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const int y = y0 + (i0 + i) * RPW;
             float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
             float qs = __fadd_rn(__fadd_rn(v[i].x, v[i].y), __fadd_rn(v[i].z, v[i].w));
@@ -384,11 +382,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             // of 8 channels the even lane makes pairs (0, 4), (1, 5), the odd one (2, 6), (3, 7)
             const bool odd = lane & 1;
             const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[i].x : v[i].z, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v[i].y : v[i].w, 1);
-            uint2 hi, lo;
-            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, lo.x);
-            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, lo.y);
-            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = low ? lo : hi;
-            if (!low) continue;
+            uint2 hi;
+            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, low[i0 + i].x);
+            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, low[i0 + i].y);
+            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = hi;
             float q4[NG];
 #pragma unroll
             for (int g = 0; g < NG; ++g) q4[g] = __shfl_sync(0xffffffffu, qs, (lane & ~(LPR - 1)) + 8 * g) * up;
@@ -405,6 +402,10 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             }
           }
         }
+        high_terms();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y0 + i * RPW, (4 * ql) & 63)) = low[i];
       }
       tc_fence_before();
       fence_proxy_async_smem();
@@ -743,6 +744,19 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       tile_positions(a, sg.tile, G, lo, hi);
       const Kv4Spans sp = kv4_spans(c, lo, hi, a.window);
       const size_t base = kv4_base(c, a.slot0, sg.head);
+      // the next item's queries into L2: the softmax warps take them with nothing else to do meanwhile
+      Segment then;
+      int64_t t2 = sg.next;
+      if (next_segment(then, pre, pa.tiles, sum, c.heads, t2, t_end)) {
+        for (int i = lane; i < kPRows; i += 32) {
+          const int r = then.tile * kPRows + i, m = group_of(r);
+          const float* q = a.q + (size_t)m * a.ldq + (size_t)(then.head * G + r - m * G) * HD;
+          if (m < a.M) {
+#pragma unroll
+            for (int x = 0; x < HD; x += 32) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + x));
+          }
+        }
+      }
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
         const int b = it & 1;
         if (it >= 2 && !(ok = wait(B_RFREE + b, ((it - 2) >> 1) & 1))) break;

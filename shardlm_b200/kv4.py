@@ -21,6 +21,7 @@ from .sharing import SharingError
 
 GROUP = 32
 CHUNK = 16
+_F32, _I32 = torch.float32, torch.int32
 
 
 class Kv4Cache:
@@ -68,18 +69,19 @@ class Kv4Cache:
         self._c = Kv4CacheC(k_codes.data_ptr(), k_params.data_ptr(), v_codes.data_ptr(), v_params.data_ptr(), slots,
                             heads, cap, 2 * half, sinks)
         self._ref = C.byref(self._c)
+        self._f32 = k_params.new_empty(0, dtype=_F32)  # new_empty of a tensor is the cheapest allocation
 
     @property
     def device_bytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_params, self.v_codes, self.v_params))
 
-    # -- argument checks -----------------------------------------------------------------------
+    # -- argument checks (a few microseconds a call: the smallest calls take not much longer) ----------
     def _rows(self, t: torch.Tensor, width: int, name: str) -> torch.Tensor:
         """f32 [rows, width] on the cache's device whose rows the kernels can read: unit column stride,
         16-byte aligned rows (anything else is copied)."""
-        if t.dtype is not torch.float32 or t.device != self._device:
-            raise SharingError(f"{name}: expected a float32 tensor on {self._device}")
         shape = t.shape
+        if t.dtype is not _F32 or t.device != self._device:
+            raise SharingError(f"{name}: expected a float32 tensor on {self._device}")
         if len(shape) != 2 or shape[1] != width or shape[0] == 0:
             raise SharingError(f"ShapeMismatch: {name}: expected [rows, {width}], got {list(shape)}")
         ld, step = t.stride()
@@ -89,51 +91,46 @@ class Kv4Cache:
 
     def _index(self, t: torch.Tensor, rows: int, name: str) -> int:
         """Address of `rows` device int32."""
-        if t.dtype is not torch.int32 or t.device != self._device or not t.is_contiguous():
+        if t.dtype is not _I32 or t.device != self._device or not t.is_contiguous():
             raise SharingError(f"{name}: expected a contiguous int32 tensor on {self._device}")
         if t.numel() != rows:
             raise SharingError(f"ShapeMismatch: {name}: expected [{rows}], got {list(t.shape)}")
         return t.data_ptr()
 
-    def _call(self, name: str, *args) -> None:
+    def _call(self, fn, *args) -> None:
         ctx = self.ctx
         ctx.bind_stream()
-        rc = getattr(lib(), name)(ctx.ptr, self._ref, *args)
+        rc = fn(ctx.ptr, self._ref, *args)
         if rc:
             check(rc, ctx.ptr)
-
-    def _pair(self, rows: int, width: int):
-        """Two f32 [rows, width] outputs and their addresses."""
-        out = torch.empty((2, rows, width), dtype=torch.float32, device=self._device)
-        at = out.data_ptr()
-        return out.unbind(0), at, at + 4 * rows * width
 
     # -- writing and reading -------------------------------------------------------------------
     def _write(self, k_client, k_server, v_client, v_server, slot, pos, slot0, pos0, values):
         width = self.kv_dim
         kc, vc = self._rows(k_client, width, "k_client"), self._rows(v_client, width, "v_client")
-        if (k_server is None) != (v_server is None):
-            raise SharingError("server shares are given for K and V or for neither")
+        rows, ld = kc.shape[0], kc.stride(0)
+        same = vc.shape[0] == rows and vc.stride(0) == ld
         ks = vs = None
-        if k_server is not None:
+        if k_server is not None and v_server is not None:
             ks, vs = self._rows(k_server, width, "k_server"), self._rows(v_server, width, "v_server")
-        t = (kc, vc) if ks is None else (kc, vc, ks, vs)
-        rows = kc.shape[0]
-        for x in t:
-            if x.shape[0] != rows:
-                raise SharingError("ShapeMismatch: K and V shares differ in rows")
-        ld = kc.stride(0) if rows > 1 else width
-        for x in t:
-            if rows > 1 and x.stride(0) != ld:
-                kc, vc, ks, vs = (None if y is None else y.contiguous() for y in (kc, vc, ks, vs))
-                ld = width
-                break
+            same = same and ks.shape[0] == rows == vs.shape[0] and ks.stride(0) == ld == vs.stride(0)
+        elif k_server is not None or v_server is not None:
+            raise SharingError("server shares are given for K and V or for neither")
+        if not same:
+            for x in (kc, vc, ks, vs):
+                if x is not None and x.shape[0] != rows:
+                    raise SharingError("ShapeMismatch: K and V shares differ in rows")
+            kc, vc, ks, vs = (None if x is None else x.contiguous() for x in (kc, vc, ks, vs))
+            ld = width
         if pos is not None:
             slot, pos = self._index(slot, rows, "slot"), self._index(pos, rows, "pos")
-        out, k_at, v_at = self._pair(rows, width) if values else (None, None, None)
-        self._call("shd_kv4_write", kc.data_ptr(), None if ks is None else ks.data_ptr(), vc.data_ptr(),
-                   None if vs is None else vs.data_ptr(), ld, slot, pos, slot0, pos0, rows, k_at, v_at)
-        return out
+        k = v = None
+        if values:
+            k, v = self._f32.new_empty(rows, width), self._f32.new_empty(rows, width)
+        self._call(lib().shd_kv4_write, kc.data_ptr(), None if ks is None else ks.data_ptr(), vc.data_ptr(),
+                   None if vs is None else vs.data_ptr(), width if rows == 1 else ld, slot, pos, slot0, pos0, rows,
+                   k.data_ptr() if values else None, v.data_ptr() if values else None)
+        return (k, v) if values else None
 
     def write(self, k_client, k_server, v_client, v_server, *, slot: torch.Tensor, pos: torch.Tensor, values: bool = False):
         """Quantise one row for each sequence: row m goes to position pos[m] of slot[m] (device int32;
@@ -149,9 +146,9 @@ class Kv4Cache:
         """Positions [pos0, pos0 + n) of a slot as (K, V), f32 [n, kv_dim]."""
         if n <= 0:
             raise SharingError("read: n must be positive")
-        out, k_at, v_at = self._pair(n, self.kv_dim)
-        self._call("shd_kv4_read", slot, pos0, n, k_at, v_at)
-        return out
+        k, v = self._f32.new_empty(n, self.kv_dim), self._f32.new_empty(n, self.kv_dim)
+        self._call(lib().shd_kv4_read, slot, pos0, n, k.data_ptr(), v.data_ptr())
+        return k, v
 
     # -- attention -----------------------------------------------------------------------------
     def _queries(self, q, mask):
@@ -160,26 +157,28 @@ class Kv4Cache:
                                f"{self.n_kv_heads}, got {list(q.shape)}")
         rows, width = q.shape
         q = self._rows(q, width, "q")
+        at = None
         if mask is not None:
             mask = self._rows(mask, width, "mask").contiguous()
             if mask.shape[0] != rows:
                 raise SharingError("ShapeMismatch: mask and q differ in rows")
-        return q, (q.stride(0) if rows > 1 else width), rows, width, mask
+            at = mask.data_ptr()
+        # the mask is returned too: it has to live until the call
+        return q, (q.stride(0) if rows > 1 else width), rows, width, at, mask
 
     def attend(self, q: torch.Tensor, *, slot: torch.Tensor, pos: torch.Tensor, window: int = 0, mask: torch.Tensor | None = None):
         """One token for each sequence: q [M, heads * head_dim] reconstructed, row m at position pos[m] of
         slot[m] (device int32), whose K/V row is written. Output shares (attn - mask, mask), or (attn, 0)."""
-        q, ldq, rows, width, mask = self._queries(q, mask)
-        slot_at, pos_at = self._index(slot, rows, "slot"), self._index(pos, rows, "pos")
-        out, c_at, s_at = self._pair(rows, width)
-        self._call("shd_kv4_attn_decode", q.data_ptr(), ldq, width // self.head_dim, slot_at, pos_at, rows, window,
-                   None if mask is None else mask.data_ptr(), c_at, s_at)
-        return out
+        q, ldq, rows, width, mask_at, mask = self._queries(q, mask)
+        c, s = self._f32.new_empty(rows, width), self._f32.new_empty(rows, width)
+        self._call(lib().shd_kv4_attn_decode, q.data_ptr(), ldq, width // self.head_dim, self._index(slot, rows, "slot"),
+                   self._index(pos, rows, "pos"), rows, window, mask_at, c.data_ptr(), s.data_ptr())
+        return c, s
 
     def attend_prompt(self, q: torch.Tensor, *, slot: int, pos0: int, window: int = 0, mask: torch.Tensor | None = None):
         """Consecutive positions pos0, pos0 + 1, .. of one slot, all of whose K/V rows are written."""
-        q, ldq, rows, width, mask = self._queries(q, mask)
-        out, c_at, s_at = self._pair(rows, width)
-        self._call("shd_kv4_attn_prefill", q.data_ptr(), ldq, width // self.head_dim, slot, pos0, rows, window,
-                   None if mask is None else mask.data_ptr(), c_at, s_at)
-        return out
+        q, ldq, rows, width, mask_at, mask = self._queries(q, mask)
+        c, s = self._f32.new_empty(rows, width), self._f32.new_empty(rows, width)
+        self._call(lib().shd_kv4_attn_prefill, q.data_ptr(), ldq, width // self.head_dim, slot, pos0, rows, window, mask_at,
+                   c.data_ptr(), s.data_ptr())
+        return c, s

@@ -42,8 +42,8 @@ class Context:
 
     # -- plumbing ------------------------------------------------------------------------------
     def bind_stream(self, stream: torch.cuda.Stream | None = None) -> None:
-        s = stream if stream is not None else torch.cuda.current_stream(self.torch_device)
-        raw = s.cuda_stream
+        # the raw handle: a Stream object would cost 2 us a call
+        raw = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device)
         if raw != self._bound_stream:
             check(lib().shd_set_stream(self.ptr, raw), self.ptr)
             self._bound_stream = raw
