@@ -34,10 +34,11 @@ __global__ void __launch_bounds__(kWriteThreads) kv4_write_kernel(const WriteArg
   pdl_trigger();
   pdl_wait();
   const int hd = a.c.head_dim, lanes = hd / 4, ng = hd / kKv4Group;
-  const int64_t unit = ((int64_t)blockIdx.x * kWriteThreads + threadIdx.x) / lanes;  // (row, head)
+  // (row, head) of this thread; below 2^31 by the launch's limit
+  const uint32_t unit = blockIdx.x * (kWriteThreads / lanes) + threadIdx.x / lanes;
   const int l = threadIdx.x % lanes;
-  const bool live = unit < (int64_t)a.M * a.c.heads;
-  const int m = live ? (int)(unit / a.c.heads) : 0, h = live ? (int)(unit % a.c.heads) : 0;
+  const bool live = unit < (uint32_t)a.M * (uint32_t)a.c.heads;
+  const int m = live ? (int)(unit / (uint32_t)a.c.heads) : 0, h = live ? (int)(unit - (uint32_t)m * a.c.heads) : 0;
   int slot = a.slot0, pos = a.pos0 + m;
   if (a.pos) {
     slot = live ? a.slot[m] : 0;
@@ -50,19 +51,21 @@ __global__ void __launch_bounds__(kWriteThreads) kv4_write_kernel(const WriteArg
   const size_t dst = ((size_t)m * a.c.heads + h) * hd + 4 * l;
   const size_t row = store ? kv4_base(a.c, slot, h) + kv4_row(a.c, pos) : 0;
   bool odd = false;
+  float4 in[2][2];  // [K, V][client, server], all requested before any is used
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
     const float* pc = kv ? a.vc : a.kc;
     const float* ps = kv ? a.vs : a.ks;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (store) {
-      const float4 c4 = *reinterpret_cast<const float4*>(pc + src);
-      x[0] = c4.x; x[1] = c4.y; x[2] = c4.z; x[3] = c4.w;
-      if (ps) {
-        const float4 s4 = *reinterpret_cast<const float4*>(ps + src);
-        x[0] = __fadd_rn(x[0], s4.x); x[1] = __fadd_rn(x[1], s4.y);
-        x[2] = __fadd_rn(x[2], s4.z); x[3] = __fadd_rn(x[3], s4.w);
-      }
+    in[kv][0] = store ? __ldcs(reinterpret_cast<const float4*>(pc + src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    in[kv][1] = store && ps ? __ldcs(reinterpret_cast<const float4*>(ps + src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const bool shared = a.ks != nullptr;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    float x[4] = {in[kv][0].x, in[kv][0].y, in[kv][0].z, in[kv][0].w};
+    if (shared) {
+      x[0] = __fadd_rn(x[0], in[kv][1].x); x[1] = __fadd_rn(x[1], in[kv][1].y);
+      x[2] = __fadd_rn(x[2], in[kv][1].z); x[3] = __fadd_rn(x[3], in[kv][1].w);
     }
     // values that f16 parameters cannot hold: clamped, NaN as 0, and reported
 #pragma unroll
@@ -99,99 +102,83 @@ __global__ void __launch_bounds__(kWriteThreads) kv4_write_kernel(const WriteArg
       }
     }
     float* out = kv ? a.v_val : a.k_val;
-    if (live && out) *reinterpret_cast<float4*>(out + dst) = store ? make_float4(val[0], val[1], val[2], val[3])
-                                                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live && out)
+      __stcs(reinterpret_cast<float4*>(out + dst), store ? make_float4(val[0], val[1], val[2], val[3]) : make_float4(0.f, 0.f, 0.f, 0.f));
   }
   if (odd) atomicOr(a.err, SHD_DEVERR_NONFINITE);
 }
 
-// Four channels a thread (one half word), [n][heads * head_dim] f32 out.
-__global__ void __launch_bounds__(kWriteThreads) kv4_read_kernel(const Kv4View c, int slot, int pos0, int n,
+// 8 threads a row (slot, head): thread u reads 2 NG bytes of the keys' codes (words of NG / 2 groups) and
+// unit u of the values, and writes both. A value unit's NG pieces of 4 channels go out 128 bytes at a time;
+// of the keys neighbouring threads exchange halves, so that theirs do too.
+template <int NG>
+__global__ void __launch_bounds__(kWriteThreads) kv4_read_kernel(const Kv4View c, int slot, int pos0, uint32_t units,
                                                                  float* k_out, float* v_out) {
+  constexpr int HD = NG * kKv4Group;
   pdl_trigger();
   pdl_wait();
-  const int hd = c.head_dim, lanes = hd / 4, ng = hd / kKv4Group;
-  const int64_t unit = ((int64_t)blockIdx.x * kWriteThreads + threadIdx.x) / lanes;
-  if (unit >= (int64_t)n * c.heads) return;
-  const int l = threadIdx.x % lanes, g = l / 8, u = l % 8;
-  const int m = (int)(unit / c.heads), h = (int)(unit % c.heads);
-  const size_t row = kv4_base(c, slot, h) + kv4_row(c, pos0 + m);
-  const size_t dst = ((size_t)m * c.heads + h) * hd + 4 * l;
-#pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    float* out = kv ? v_out : k_out;
-    if (!out) continue;
-    const uint16_t* codes = reinterpret_cast<const uint16_t*>((kv ? c.vc : c.kc) + row * (hd / 2));
-    const __half* p = (kv ? c.vp : c.kp) + row * (2 * ng);
-    const uint32_t w = codes[kv ? u * ng + g : 2 * ((u >> 1) * ng + g) + (u & 1)];
-    const float s = __half2float(p[g]), z = __half2float(p[ng + g]);
-    float4 y;
-    y.x = __fmaf_rn(s, (float)(w & 15u), z);
-    y.y = __fmaf_rn(s, (float)((w >> 4) & 15u), z);
-    y.z = __fmaf_rn(s, (float)((w >> 8) & 15u), z);
-    y.w = __fmaf_rn(s, (float)((w >> 12) & 15u), z);
-    *reinterpret_cast<float4*>(out + dst) = y;
+  const uint32_t unit = blockIdx.x * (kWriteThreads / 8) + threadIdx.x / 8;  // (row, head)
+  const int u = threadIdx.x % 8;
+  const bool live = unit < units;
+  const uint32_t m = live ? unit / (uint32_t)c.heads : 0, h = live ? unit - m * c.heads : 0;
+  const size_t row = kv4_base(c, slot, (int)h) + kv4_row(c, pos0 + (int)m);
+  const size_t dst = ((size_t)m * c.heads + h) * HD;
+  uint32_t kw[NG / 2], vw[NG / 2];
+  uint32_t kp[NG], vp[NG];  // NG scales, NG minima, two a word
+  if constexpr (NG == 4) {
+    const uint2 x = __ldcs(reinterpret_cast<const uint2*>(c.kc + row * 64) + u), y = __ldcs(reinterpret_cast<const uint2*>(c.vc + row * 64) + u);
+    const uint4 p = __ldg(reinterpret_cast<const uint4*>(c.kp + row * 8)), q = __ldg(reinterpret_cast<const uint4*>(c.vp + row * 8));
+    kw[0] = x.x; kw[1] = x.y; vw[0] = y.x; vw[1] = y.y;
+    kp[0] = p.x; kp[1] = p.y; kp[2] = p.z; kp[3] = p.w;
+    vp[0] = q.x; vp[1] = q.y; vp[2] = q.z; vp[3] = q.w;
+  } else {
+    kw[0] = __ldcs(reinterpret_cast<const uint32_t*>(c.kc + row * 32) + u);
+    vw[0] = __ldcs(reinterpret_cast<const uint32_t*>(c.vc + row * 32) + u);
+    const uint2 p = __ldg(reinterpret_cast<const uint2*>(c.kp + row * 4)), q = __ldg(reinterpret_cast<const uint2*>(c.vp + row * 4));
+    kp[0] = p.x; kp[1] = p.y; vp[0] = q.x; vp[1] = q.y;
   }
-}
-
-// Attention of one (query row, head) a warp, one position at a time: lane l holds head_dim / 32
-// channels, scores are summed over the warp, the softmax is online.
-__global__ void __launch_bounds__(256) kv4_attn_kernel(const Kv4AttnArgs a) {
-  const Kv4View& c = a.c;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (item >= (int64_t)a.M * a.H) return;
-  const int lane = threadIdx.x & 31, hd = c.head_dim, ng = hd / kKv4Group;
-  const int m = (int)(item / a.H), hq = (int)(item % a.H), h = hq / (a.H / c.heads);
-  int slot = a.slot0, pos = a.pos0 + m, last = a.pos0 + a.M - 1;
-  if (a.pos) {
-    slot = a.slot[m];
-    pos = last = a.pos[m];
-    if (pos >= 0 && (slot < 0 || slot >= c.slots || !kv4_in_reach(c, pos, a.window, 0))) {
-      if (lane == 0) atomicOr(a.err, SHD_DEVERR_ARG);
-      pos = -1;
-    }
-  }
-  const size_t base = pos >= 0 ? kv4_base(c, slot, h) : 0;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY, sum = 0.0f;
+  if (k_out) {
+    // word t of group g is number t NG + g: this thread's are 2 u, 2 u + 1 (HD 64: u)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = lane + 32 * i < hd ? a.q[(size_t)m * a.ldq + (size_t)hq * hd + lane + 32 * i] : 0.0f;
-  const Kv4Spans sp = kv4_spans(c, pos, last, a.window);
-  for (int i = 0; pos >= 0 && i < sp.total; ++i) {
-    const int r0 = kv4_span_chunk(sp, i) * kKv4Chunk;
-    for (int r = r0; r < r0 + kKv4Chunk; ++r) {
-      const int t = kv4_held(c, r, last);
-      if (!kv4_sees(c, pos, r, t, a.window)) continue;
-      const uint16_t* kc = reinterpret_cast<const uint16_t*>(c.kc + (base + r) * (hd / 2));
-      const uint16_t* vc = reinterpret_cast<const uint16_t*>(c.vc + (base + r) * (hd / 2));
-      const __half *kp = c.kp + (base + r) * (2 * ng), *vp = c.vp + (base + r) * (2 * ng);
-      float dot = 0.0f, v[4];
+    for (int i = 0; i < NG / 2; ++i) {
+      const int w = u * (NG / 2) + i, t = w / NG, g = w % NG;
+      const float2 s2 = unpack_f16(NG == 4 && g >= 2 ? kp[1] : kp[0]), z2 = unpack_f16(NG == 4 ? (g >= 2 ? kp[3] : kp[2]) : kp[1]);
+      const float s = (g & 1) ? s2.y : s2.x, z = (g & 1) ? z2.y : z2.x;
+      float y[8];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        v[g] = 0.0f;
-        if (g >= ng) continue;
-        const int u = lane / 4, n = lane % 4;  // channel 32 g + lane
-        const uint32_t kw = kc[2 * ((u >> 1) * ng + g) + (u & 1)], vw = vc[u * ng + g];
-        dot = fmaf(q[g], fmaf(__half2float(kp[g]), (float)((kw >> (4 * n)) & 15u), __half2float(kp[ng + g])), dot);
-        v[g] = fmaf(__half2float(vp[g]), (float)((vw >> (4 * n)) & 15u), __half2float(vp[ng + g]));
+      for (int n = 0; n < 8; ++n) y[n] = __fmaf_rn(s, (float)((kw[i] >> (4 * n)) & 15u), z);
+      // words t, t + 1 (t even) of the group are NG / 2 threads apart (HD 64: 2): the first keeps the low
+      // halves of both, and with them 16 neighbouring bytes of each
+      constexpr int FAR = 2;  // NG == 4: u + 2 holds t + 1 of the same groups; NG == 2: u + 2 as well
+      const bool odd = t & 1;
+      float4 mine, other;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const float send = odd ? y[n] : y[4 + n];
+        const float got = __shfl_xor_sync(0xffffffffu, send, FAR);
+        (&mine.x)[n] = odd ? got : y[n];       // of word t (even)
+        (&other.x)[n] = odd ? y[4 + n] : got;  // of word t + 1
       }
-#pragma unroll
-      for (int s = 16; s >= 1; s >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, s);
-      dot *= a.scale;
-      const float mn = fmaxf(mx, dot), al = mx == -INFINITY ? 0.0f : expf(mx - mn), w = expf(dot - mn);
-      mx = mn;
-      sum = fmaf(sum, al, w);
-#pragma unroll
-      for (int g = 0; g < 4; ++g) o[g] = fmaf(w, v[g], o[g] * al);
+      if (live) {
+        float* to = k_out + dst + 32 * g + 8 * (t & ~1) + (odd ? 4 : 0);
+        __stcs(reinterpret_cast<float4*>(to), mine);
+        __stcs(reinterpret_cast<float4*>(to + 8), other);
+      }
     }
   }
-  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+  if (v_out && live) {
 #pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    if (g >= ng) continue;
-    const size_t at = (size_t)m * a.H * hd + (size_t)hq * hd + 32 * g + lane;
-    const float mk = a.mask ? a.mask[at] : 0.0f;
-    a.out_c[at] = __fsub_rn(o[g] * inv, mk);
-    a.out_s[at] = mk;
+    for (int g = 0; g < NG; ++g) {
+      const uint32_t w = (vw[g / 2] >> (16 * (g & 1))) & 0xffffu;
+      const float2 s2 = unpack_f16(vp[g / 2]), z2 = unpack_f16(vp[NG / 2 + g / 2]);
+      const float s = (g & 1) ? s2.y : s2.x, z = (g & 1) ? z2.y : z2.x;
+      float4 y;
+      y.x = __fmaf_rn(s, (float)(w & 15u), z);
+      y.y = __fmaf_rn(s, (float)((w >> 4) & 15u), z);
+      y.z = __fmaf_rn(s, (float)((w >> 8) & 15u), z);
+      y.w = __fmaf_rn(s, (float)(w >> 12), z);
+      __stcs(reinterpret_cast<float4*>(v_out + dst + 32 * g + 4 * u), y);
+    }
   }
 }
 
@@ -240,14 +227,6 @@ int check_attn(shd_ctx* ctx, const char* fn, const shd_kv4_cache* cache, const f
   return SHD_OK;
 }
 
-int launch_attn(shd_ctx* ctx, const Kv4AttnArgs& a) {
-  const int64_t blocks = ((int64_t)a.M * a.H + 7) / 8;
-  SHD_REQUIRE(ctx, blocks <= 0x7fffffff, "kv4 attention: too many rows");
-  kv4_attn_kernel<<<(unsigned)blocks, 256, 0, ctx->stream>>>(a);
-  SHD_CHECK_LAUNCH(ctx, "kv4_attn_kernel");
-  return SHD_OK;
-}
-
 }  // namespace
 }  // namespace shd
 
@@ -277,9 +256,9 @@ extern "C" int shd_kv4_write(shd_ctx* ctx, const shd_kv4_cache* cache, const flo
   a.slot = slot; a.pos = pos; a.slot0 = slot0; a.pos0 = pos0; a.M = M;
   a.k_val = k_val; a.v_val = v_val;
   a.err = ctx->d_err;
-  const int64_t threads = (int64_t)M * a.c.heads * (a.c.head_dim / 4);
-  const int64_t blocks = (threads + kWriteThreads - 1) / kWriteThreads;
-  SHD_REQUIRE(ctx, blocks <= 0x7fffffff, "shd_kv4_write: too many rows");
+  SHD_REQUIRE(ctx, (int64_t)M * a.c.heads <= 0x7fffffff, "shd_kv4_write: too many rows");
+  const int per_block = kWriteThreads / (a.c.head_dim / 4);
+  const int64_t blocks = ((int64_t)M * a.c.heads + per_block - 1) / per_block;
   SHD_CHECK_CUDA(ctx, launch_pdl(kv4_write_kernel, dim3((unsigned)blocks), dim3(kWriteThreads), 0, ctx->stream, a));
   ctx->launches++;
   return SHD_OK;
@@ -297,10 +276,10 @@ extern "C" int shd_kv4_read(shd_ctx* ctx, const shd_kv4_cache* cache, int slot, 
   SHD_REQUIRE(ctx, (int64_t)pos0 + n <= c.capacity || n <= c.capacity - c.sinks, "shd_kv4_read: more rows than the ring holds");
   SHD_REQUIRE(ctx, shd_aligned16(k_out) && shd_aligned16(v_out), "shd_kv4_read: tensors must be 16-byte aligned");
   SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
-  const int64_t blocks = ((int64_t)n * c.heads * (c.head_dim / 4) + kWriteThreads - 1) / kWriteThreads;
-  SHD_REQUIRE(ctx, blocks <= 0x7fffffff, "shd_kv4_read: too many rows");
-  SHD_CHECK_CUDA(ctx, launch_pdl(kv4_read_kernel, dim3((unsigned)blocks), dim3(kWriteThreads), 0, ctx->stream, c, slot,
-                                 pos0, n, k_out, v_out));
+  SHD_REQUIRE(ctx, (int64_t)n * c.heads <= 0x7fffffff, "shd_kv4_read: too many rows");
+  const uint32_t units = (uint32_t)n * (uint32_t)c.heads, blocks = units / (kWriteThreads / 8) + (units % (kWriteThreads / 8) ? 1 : 0);
+  SHD_CHECK_CUDA(ctx, launch_pdl(c.head_dim == 128 ? kv4_read_kernel<4> : kv4_read_kernel<2>, dim3(blocks),
+                                 dim3(kWriteThreads), 0, ctx->stream, c, slot, pos0, units, k_out, v_out));
   ctx->launches++;
   return SHD_OK;
 }

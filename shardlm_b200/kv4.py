@@ -76,6 +76,10 @@ class Kv4Cache:
         return sum(t.numel() * t.element_size() for t in (self.k_codes, self.k_params, self.v_codes, self.v_params))
 
     # -- argument checks (a few microseconds a call: the smallest calls take not much longer) ----------
+    def _plain(self, t: torch.Tensor, shape) -> bool:
+        return (t.shape == shape and t.dtype is _F32 and t.device == self._device and t.is_contiguous()
+                and not t.data_ptr() & 15)
+
     def _rows(self, t: torch.Tensor, width: int, name: str) -> torch.Tensor:
         """f32 [rows, width] on the cache's device whose rows the kernels can read: unit column stride,
         16-byte aligned rows (anything else is copied)."""
@@ -106,29 +110,34 @@ class Kv4Cache:
 
     # -- writing and reading -------------------------------------------------------------------
     def _write(self, k_client, k_server, v_client, v_server, slot, pos, slot0, pos0, values):
-        width = self.kv_dim
-        kc, vc = self._rows(k_client, width, "k_client"), self._rows(v_client, width, "v_client")
-        rows, ld = kc.shape[0], kc.stride(0)
-        same = vc.shape[0] == rows and vc.stride(0) == ld
-        ks = vs = None
-        if k_server is not None and v_server is not None:
-            ks, vs = self._rows(k_server, width, "k_server"), self._rows(v_server, width, "v_server")
-            same = same and ks.shape[0] == rows == vs.shape[0] and ks.stride(0) == ld == vs.stride(0)
-        elif k_server is not None or v_server is not None:
-            raise SharingError("server shares are given for K and V or for neither")
-        if not same:
-            for x in (kc, vc, ks, vs):
-                if x is not None and x.shape[0] != rows:
-                    raise SharingError("ShapeMismatch: K and V shares differ in rows")
-            kc, vc, ks, vs = (None if x is None else x.contiguous() for x in (kc, vc, ks, vs))
-            ld = width
+        width, plain = self.kv_dim, self._plain
+        kc, ks, vc, vs = k_client, k_server, v_client, v_server
+        shape = kc.shape
+        if len(shape) == 2 and shape[1] == width and shape[0] and plain(kc, shape) and plain(vc, shape) and (
+                plain(ks, shape) and plain(vs, shape) if ks is not None and vs is not None else ks is vs):
+            rows, ld = shape[0], width
+        else:
+            kc, vc = self._rows(kc, width, "k_client"), self._rows(vc, width, "v_client")
+            if (ks is None) != (vs is None):
+                raise SharingError("server shares are given for K and V or for neither")
+            if ks is not None:
+                ks, vs = self._rows(ks, width, "k_server"), self._rows(vs, width, "v_server")
+            rows, ld = kc.shape[0], kc.stride(0)
+            all_ = [x for x in (kc, vc, ks, vs) if x is not None]
+            if any(x.shape[0] != rows for x in all_):
+                raise SharingError("ShapeMismatch: K and V shares differ in rows")
+            if rows == 1:
+                ld = width
+            elif any(x.stride(0) != ld for x in all_):
+                kc, vc, ks, vs = (None if x is None else x.contiguous() for x in (kc, vc, ks, vs))
+                ld = width
         if pos is not None:
             slot, pos = self._index(slot, rows, "slot"), self._index(pos, rows, "pos")
         k = v = None
         if values:
             k, v = self._f32.new_empty(rows, width), self._f32.new_empty(rows, width)
         self._call(lib().shd_kv4_write, kc.data_ptr(), None if ks is None else ks.data_ptr(), vc.data_ptr(),
-                   None if vs is None else vs.data_ptr(), width if rows == 1 else ld, slot, pos, slot0, pos0, rows,
+                   None if vs is None else vs.data_ptr(), ld, slot, pos, slot0, pos0, rows,
                    k.data_ptr() if values else None, v.data_ptr() if values else None)
         return (k, v) if values else None
 
@@ -152,19 +161,24 @@ class Kv4Cache:
 
     # -- attention -----------------------------------------------------------------------------
     def _queries(self, q, mask):
-        if q.dim() != 2 or q.shape[1] % self.kv_dim:
+        shape = q.shape
+        if len(shape) != 2 or shape[1] % self.kv_dim:
             raise SharingError(f"ShapeMismatch: q: expected [rows, heads * {self.head_dim}] with heads a multiple of "
-                               f"{self.n_kv_heads}, got {list(q.shape)}")
-        rows, width = q.shape
-        q = self._rows(q, width, "q")
+                               f"{self.n_kv_heads}, got {list(shape)}")
+        rows, width = shape
+        ldq = width
+        if not (rows and self._plain(q, shape)):
+            q = self._rows(q, width, "q")
+            ldq = q.stride(0) if rows > 1 else width
         at = None
         if mask is not None:
-            mask = self._rows(mask, width, "mask").contiguous()
-            if mask.shape[0] != rows:
-                raise SharingError("ShapeMismatch: mask and q differ in rows")
+            if not self._plain(mask, shape):
+                mask = self._rows(mask, width, "mask").contiguous()
+                if mask.shape[0] != rows:
+                    raise SharingError("ShapeMismatch: mask and q differ in rows")
             at = mask.data_ptr()
         # the mask is returned too: it has to live until the call
-        return q, (q.stride(0) if rows > 1 else width), rows, width, at, mask
+        return q, ldq, rows, width, at, mask
 
     def attend(self, q: torch.Tensor, *, slot: torch.Tensor, pos: torch.Tensor, window: int = 0, mask: torch.Tensor | None = None):
         """One token for each sequence: q [M, heads * head_dim] reconstructed, row m at position pos[m] of
