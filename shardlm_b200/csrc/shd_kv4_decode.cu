@@ -17,11 +17,13 @@
 // leave their thread. A lane's row order within 8 rows (sigma) is t, t + 4: with it every shared-memory
 // read below is free of bank conflicts.
 //
-// Work: an item is (query row, kv head, up to 8 query heads); its visible 16-row chunks (kv4_spans)
-// are laid end to end with those of every other item and cut into equal shares, one a CTA, whatever
-// the lengths. In a CTA the 8 warps take chunks in turn, each with its own ring of asynchronous copies
-// and its own online softmax, and are combined in warp order. An item that is cut leaves partial
-// results; the CTA that arrives last joins them in CTA order, so results do not depend on timing.
+// Work: an item is (query row, kv head, up to 8 query heads) with its visible 16-row chunks (kv4_spans).
+// When the items are few, each is cut evenly into as many parts as give every CTA at most one; else the
+// chunks of all items, with kDItem for an item's start and end, are laid end to end and cut into equal
+// shares, whatever the lengths. In a CTA the 8 warps take pairs of chunks in turn, each with its own ring
+// of asynchronous copies and its own online softmax, and are combined in warp order. An item that is cut
+// leaves partial results; the CTA that arrives last joins them in CTA order, so results do not depend on
+// timing.
 #include <cmath>
 
 #include "shd_kv4.cuh"
@@ -32,9 +34,9 @@ namespace {
 constexpr int kDWarps = 8;
 constexpr int kDThreads = 32 * kDWarps;
 constexpr int kDStages = 2;       // of a warp's ring, two chunks each
-constexpr int kDRows = 1024;      // query rows of one launch (their chunk counts are in shared memory)
-constexpr int kDItem = 8;         // what an item costs a CTA besides its chunks, in chunks
-constexpr int kDMinShare = 16 + kDItem;  // least cost worth a CTA
+constexpr int kDRows = 512;       // query rows of one launch (their chunk counts are in shared memory)
+constexpr int kDItem = 18;        // what an item costs a CTA besides its chunks, in chunks
+constexpr int kDSizes = 8;        // sizes of a part that are tried, 16 chunks apart
 
 template <int HD>
 struct DecodeShape {
@@ -48,7 +50,7 @@ struct DecodeShape {
   static constexpr int ROWS = 3 * 32 * NG * 4;         // f32 parameters of a stage's 32 rows, see Rows
   static constexpr int RING = kDWarps * (kDStages * STAGE + ROWS);
   static constexpr int JOIN = kDWarps * 8 * PART * 4;  // per warp and head, over the rings
-  static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + kDRows * 8 + 8 * 8 * 4 * 2 + 256;
+  static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + kDRows * 16 + 64 * 4 + 16 * 4 + 256;
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -180,10 +182,12 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   constexpr int NG = SH::NG, PART = SH::PART;
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr size_t kBody = SH::RING > SH::JOIN ? SH::RING : SH::JOIN;
-  int64_t* pre = reinterpret_cast<int64_t*>(smem + kBody);              // chunks of the rows before
-  float* wgt = reinterpret_cast<float*>(smem + kBody + kDRows * 8);     // [warp][head] combine weights
+  int64_t* pre = reinterpret_cast<int64_t*>(smem + kBody);              // costs (or parts) of the rows before
+  int2* rows = reinterpret_cast<int2*>(smem + kBody + kDRows * 8);      // (position or -1, slot)
+  float* wgt = reinterpret_cast<float*>(smem + kBody + kDRows * 16);    // [warp][head] combine weights
   float* total = wgt + 64;                                              // [head] max, [head] sum
   int* flag = reinterpret_cast<int*>(total + 16);
+  uint32_t* fits = reinterpret_cast<uint32_t*>(flag + 2);               // [kDSizes] parts of all rows
   int64_t* scan = reinterpret_cast<int64_t*>(total + 32);               // [8] warp sums
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   const Kv4View& c = a.c;
@@ -192,40 +196,76 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   pdl_trigger();
   pdl_wait();
 
-  // costs of the rows in chunks, summed up to each (a row that sees nothing counts one, for its output)
+  // chunk counts of the rows (a row that sees nothing counts one, for its output)
   const int G = a.H / c.heads, nsub = (G + 7) / 8, HS = c.heads * nsub;
-  int64_t sum = 0;
-  for (int m0 = 0; m0 < a.M; m0 += kDThreads) {
-    const int m = m0 + tid;
-    int64_t n = 0;
+  int counts[kDRows / kDThreads];
+#pragma unroll
+  for (int i = 0; i < kDRows / kDThreads; ++i) {
+    const int m = i * kDThreads + tid;
+    counts[i] = 0;
     if (m < a.M) {
-      const int p = a.pos[m], sl = a.slot[m];
+      int p = a.pos[m];
+      const int sl = a.slot[m];
       const bool ok = p >= 0 && sl >= 0 && sl < c.slots && kv4_in_reach(c, p, a.window, 0);
       if (p >= 0 && !ok && blockIdx.x == 0) atomicOr(a.err, SHD_DEVERR_ARG);
-      n = (ok ? max(kv4_spans(c, p, p, a.window).total, 1) : 1) + kDItem;
+      if (!ok) p = -1;
+      rows[m] = make_int2(p, sl);
+      counts[i] = max(kv4_spans(c, p, p, a.window).total, 1);
     }
-    int64_t x = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) scan[warp] = x;
-    __syncthreads();
-    int64_t base = sum;
-    for (int w = 0; w < kDWarps; ++w) {
-      if (w < warp) base += scan[w];
-      sum += scan[w];
-    }
-    if (m < a.M) pre[m] = base + x - n;
-    __syncthreads();
   }
+  if (tid < kDSizes) fits[tid] = 0u;
+  // sums over the rows before each, of f(count), into pre; returns the sum over all
+  auto prefix = [&](auto f) -> int64_t {
+    int64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < kDRows / kDThreads; ++i) {
+      if (i * kDThreads >= a.M) break;
+      const int m = i * kDThreads + tid;
+      const int64_t n = m < a.M ? f(counts[i]) : 0;
+      int64_t x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) scan[warp] = x;
+      __syncthreads();
+      int64_t base = sum;
+#pragma unroll
+      for (int w = 0; w < kDWarps; ++w) {
+        if (w < warp) base += scan[w];
+        sum += scan[w];
+      }
+      if (m < a.M) pre[m] = base + x - n;
+    }
+    return sum;
+  };
+  int64_t sum = prefix([](int n) { return (int64_t)n + kDItem; });
+  const int64_t share = ((sum - (int64_t)a.M * kDItem) * HS + gridDim.x - 1) / gridDim.x;  // chunks a CTA
+  int size = 0;  // of a part; 0: equal shares
+  if ((int64_t)a.M * HS <= gridDim.x) {
+    const uint32_t first = (uint32_t)((share + 15) / 16) * 16;
+#pragma unroll
+    for (int y = 0; y < kDSizes; ++y) {
+      uint32_t n = 0;
+#pragma unroll
+      for (int i = 0; i < kDRows / kDThreads; ++i) n += ((uint32_t)counts[i] + first + 16 * y - 1) / (first + 16 * y);
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0 && n) atomicAdd(fits + y, n);
+    }
+    __syncthreads();
+    for (int y = kDSizes - 1; y >= 0; --y)
+      if ((uint64_t)fits[y] * HS <= gridDim.x) size = (int)first + 16 * y;
+    if (size) sum = prefix([size](int n) { return (int64_t)((n + size - 1) / size); });
+  }
+  __syncthreads();
   const int64_t T = sum * HS;
-  const int64_t per = max((T + gridDim.x - 1) / gridDim.x, (int64_t)kDMinShare);
+  const int64_t per = size ? 1 : (T + gridDim.x - 1) / gridDim.x;
   const int64_t t_begin = blockIdx.x * per, t_end = min(T, t_begin + per);
 
   for (int64_t t = t_begin; t < t_end;) {
-    // the item that t falls into: kDItem for its start and end, then its chunks
+    // the item that t falls into: its parts, or kDItem for its start and end, then its chunks
     int lo = 0, hi = a.M - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
@@ -233,19 +273,33 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     }
     const int m = lo;
     const int64_t row_t = pre[m] * HS;
-    const int cost = (int)((m + 1 < a.M ? pre[m + 1] : sum) - pre[m]), n = cost - kDItem;
-    const int hs = (int)((t - row_t) / cost);
+    const int cost = (int)((m + 1 < a.M ? pre[m + 1] : sum) - pre[m]);
+    const uint64_t in_row = (uint64_t)(t - row_t);
+    const int hs = in_row >> 32 ? (int)(in_row / (uint64_t)cost) : (int)((uint32_t)in_row / (uint32_t)cost);
     const int64_t item_t = row_t + (int64_t)hs * cost;
     const int64_t done = min(t_end, item_t + cost);
-    const int c0 = max((int)(t - item_t) - kDItem, 0), c1 = (int)(done - item_t) - kDItem;
-    if (c1 <= c0) {  // none of its chunks
-      t = done;
-      continue;
+    const int p = rows[m].x, sl = rows[m].y;
+    const Kv4Spans sp = kv4_spans(c, p, p, a.window);
+    int n, c0, c1, w0, parts;  // chunks, this CTA's of them, first CTA of the item and how many
+    if (size) {
+      const int part = (int)(t - item_t);
+      n = max(sp.total, 1);
+      c0 = (int)((int64_t)n * part / cost);
+      c1 = (int)((int64_t)n * (part + 1) / cost);
+      w0 = (int)item_t;
+      parts = cost;
+    } else {
+      n = cost - kDItem;
+      c0 = max((int)(t - item_t) - kDItem, 0);
+      c1 = (int)(done - item_t) - kDItem;
+      if (c1 <= c0) {  // none of its chunks
+        t = done;
+        continue;
+      }
+      w0 = (int)((item_t + kDItem) / per);
+      parts = (int)((item_t + cost - 1) / per) - w0 + 1;
     }
     const int kvh = hs / nsub, h0 = kvh * G + (hs % nsub) * 8, nh = min(8, kvh * G + G - h0);
-    int p = a.pos[m], sl = a.slot[m];
-    if (!(p >= 0 && sl >= 0 && sl < c.slots && kv4_in_reach(c, p, a.window, 0))) p = -1;
-    const Kv4Spans sp = kv4_spans(c, p, p, a.window);
     const Seen seen = make_seen(c, p, a.window);
     const size_t base = p >= 0 ? kv4_base(c, sl, kvh) : 0;
 
@@ -563,7 +617,6 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     }
     if (!whole) {
       // the last CTA of the item joins the parts in CTA order
-      const int w0 = (int)((item_t + kDItem) / per), parts = (int)((item_t + cost - 1) / per) - w0 + 1;
       __threadfence();
       __syncthreads();
       if (tid == 0) {
