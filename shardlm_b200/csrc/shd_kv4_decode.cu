@@ -20,7 +20,7 @@
 // Work: an item is (query row, kv head, up to 8 query heads) with its visible 16-row chunks (kv4_spans).
 // When the items are few, each is cut evenly into as many parts as give every CTA at most one; else the
 // chunks of all items, with kDItem for an item's start and end, are laid end to end and cut into equal
-// shares, whatever the lengths. In a CTA the 8 warps take pairs of chunks in turn, each with its own ring
+// shares, whatever the lengths. In a CTA the 8 warps take chunks in turn, each with its own ring
 // of asynchronous copies and its own online softmax, and are combined in warp order. An item that is cut
 // leaves partial results; the CTA that arrives last joins them in CTA order, so results do not depend on
 // timing.
@@ -33,21 +33,22 @@ namespace {
 
 constexpr int kDWarps = 8;
 constexpr int kDThreads = 32 * kDWarps;
-constexpr int kDStages = 2;       // of a warp's ring, two chunks each
+constexpr int kDStages = 4;       // chunks of a warp's ring
 constexpr int kDRows = 512;       // query rows of one launch (their chunk counts are in shared memory)
 constexpr int kDItem = 18;        // what an item costs a CTA besides its chunks, in chunks
-constexpr int kDSizes = 8;        // sizes of a part that are tried, 16 chunks apart
+constexpr int kDSizes = 8;        // sizes of a part that are tried, kDWarps chunks apart
 
 template <int HD>
 struct DecodeShape {
   static constexpr int NG = HD / kKv4Group;
   static constexpr int CODE = kKv4Chunk * HD / 2;      // bytes of a chunk's codes (K or V)
   static constexpr int PAR = kKv4Chunk * 4 * NG;       // bytes of a chunk's parameters
-  static constexpr int CHUNK = 2 * (CODE + PAR);
-  static constexpr int STAGE = 2 * CHUNK;
+  static constexpr int STAGE = 2 * (CODE + PAR);
   static constexpr int PART = HD + 4;                  // of one head: running max, sum, 2 unused, weighted V
   static constexpr int LEFT = 8 * HD + 16;             // of a cut item: weighted V of 8 heads, maxima, sums
-  static constexpr int ROWS = 3 * 32 * NG * 4;         // f32 parameters of a stage's 32 rows, see Rows
+  // a chunk's parameters in f32: [keys, values][scale, middle][half of the chunk][tig][group][row sigma(2 tig),
+  // sigma(2 tig + 1)]
+  static constexpr int ROWS = 4 * kKv4Chunk * NG * 4;
   static constexpr int RING = kDWarps * (kDStages * STAGE + ROWS);
   static constexpr int JOIN = kDWarps * 8 * PART * 4;  // per warp and head, over the rings
   static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + kDRows * 16 + 64 * 4 + 16 * 4 + 256;
@@ -245,18 +246,18 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   const int64_t share = ((sum - (int64_t)a.M * kDItem) * HS + gridDim.x - 1) / gridDim.x;  // chunks a CTA
   int size = 0;  // of a part; 0: equal shares
   if ((int64_t)a.M * HS <= gridDim.x) {
-    const uint32_t first = (uint32_t)((share + 15) / 16) * 16;
+    const uint32_t first = (uint32_t)((share + kDWarps - 1) / kDWarps) * kDWarps;
 #pragma unroll
     for (int y = 0; y < kDSizes; ++y) {
       uint32_t n = 0;
 #pragma unroll
-      for (int i = 0; i < kDRows / kDThreads; ++i) n += ((uint32_t)counts[i] + first + 16 * y - 1) / (first + 16 * y);
+      for (int i = 0; i < kDRows / kDThreads; ++i) n += ((uint32_t)counts[i] + first + kDWarps * y - 1) / (first + kDWarps * y);
       n = __reduce_add_sync(0xffffffffu, n);
       if (lane == 0 && n) atomicAdd(fits + y, n);
     }
     __syncthreads();
     for (int y = kDSizes - 1; y >= 0; --y)
-      if ((uint64_t)fits[y] * HS <= gridDim.x) size = (int)first + 16 * y;
+      if ((uint64_t)fits[y] * HS <= gridDim.x) size = (int)first + kDWarps * y;
     if (size) sum = prefix([size](int n) { return (int64_t)((n + size - 1) / size); });
   }
   __syncthreads();
@@ -303,30 +304,18 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     const Seen seen = make_seen(c, p, a.window);
     const size_t base = p >= 0 ? kv4_base(c, sl, kvh) : 0;
 
-    // this warp's chunk pairs: c0 + 2 warp, + 16, ..
-    const int first = c0 + 2 * warp, stop = p >= 0 ? min(c1, sp.total) : 0;
-    const int mine = first < stop ? (stop - first + 2 * kDWarps - 1) / (2 * kDWarps) : 0;
+    // this warp's chunks: c0 + warp, + 8, ..
+    const int first = c0 + warp, stop = p >= 0 ? min(c1, sp.total) : 0;
+    const int mine = first < stop ? (stop - first + kDWarps - 1) / kDWarps : 0;
     uint8_t* ring = smem + warp * (kDStages * SH::STAGE + SH::ROWS);
     const uint32_t ring_at = smem_u32(ring);
-    feed.source(c, base, lane);
     float* rows_f32 = reinterpret_cast<float*>(ring + kDStages * SH::STAGE);
-    int row0 = 0, row1 = 0, next0 = 0, next1 = 0;  // first rows of the chunks at work, and of those on their way
-    auto issue = [&](int i) {
-      const int x = first + i * 2 * kDWarps;
-      const uint32_t st = ring_at + (i % kDStages) * SH::STAGE;
-      const int a0 = kv4_span_chunk(sp, x);
-      feed.chunk(a0, st, lane);
-      next0 = a0 * kKv4Chunk;
-      if (x + 1 < stop) {
-        const int a1 = kv4_span_chunk(sp, x + 1);
-        feed.chunk(a1, st + SH::CHUNK, lane);
-        next1 = a1 * kKv4Chunk;
-      }
-    };
-    if (mine > 0) issue(0);
-    cp_async_commit();
-    row0 = next0;
-    row1 = next1;
+    feed.source(c, base, lane);
+#pragma unroll
+    for (int i = 0; i < kDStages - 1; ++i) {
+      if (i < mine) feed.chunk(kv4_span_chunk(sp, first + i * kDWarps), ring_at + i * SH::STAGE, lane);
+      cp_async_commit();
+    }
 
     // queries of head gid: two f16 terms of q * 2^k, in the order of the masked code words
     uint32_t qh[NG][4], ql[NG][4], zh, zl;
@@ -388,99 +377,93 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     uint32_t vbound = 0u;
     int ev = 0;
 
+#pragma unroll 1
     for (int i = 0; i < mine; ++i) {
-      cp_async_wait<0>();
+      cp_async_wait<kDStages - 2>();
       __syncwarp();
-      const uint8_t* st = ring + (i % kDStages) * SH::STAGE;
-      // row `lane` of the 32: whether it is seen, and its parameters in f32 for the 8 heads' lanes; a
+      const int at = i % kDStages;
+      {
+        const int nx = i + kDStages - 1;
+        if (nx < mine) feed.chunk(kv4_span_chunk(sp, first + nx * kDWarps), ring_at + (nx % kDStages) * SH::STAGE, lane);
+        cp_async_commit();
+      }
+      const uint8_t* st = ring + at * SH::STAGE;
+      // lanes 0-15: the rows' key parameters, 16-31: their value parameters, in f32 for the 8 heads' lanes; a
       // row out of sight has them 0, whatever its memory holds
       uint32_t sight, vtop;
       {
-        const int u = lane >> 4, r = lane & 15;
-        const bool ok = (u == 0 || first + i * 2 * kDWarps + 1 < stop) && seen.row((u ? row1 : row0) + r);
+        const int r = lane & 15, kind = lane >> 4;
+        const bool ok = seen.row(kv4_span_chunk(sp, first + i * kDWarps) * kKv4Chunk + r);
         sight = __ballot_sync(0xffffffffu, ok);
-        uint8_t* kp = ring + (i % kDStages) * SH::STAGE + u * SH::CHUNK + 2 * SH::CODE + r * (4 * NG);
-        const uint8_t* vp = kp + SH::PAR;
-        uint32_t ks[NG / 2], vs[NG / 2], vz[NG / 2];
+        uint8_t* from = ring + at * SH::STAGE + 2 * SH::CODE + kind * SH::PAR + r * (4 * NG);
+        uint32_t w[NG];
         if constexpr (NG == 4) {
-          const uint2 x = *reinterpret_cast<const uint2*>(kp);
-          const uint4 y = *reinterpret_cast<const uint4*>(vp);
-          ks[0] = x.x; ks[1] = x.y; vs[0] = y.x; vs[1] = y.y; vz[0] = y.z; vz[1] = y.w;
+          const uint4 x = *reinterpret_cast<const uint4*>(from);
+          w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
         } else {
-          const uint2 y = *reinterpret_cast<const uint2*>(vp);
-          ks[0] = *reinterpret_cast<const uint32_t*>(kp);
-          vs[0] = y.x; vz[0] = y.y;
+          const uint2 x = *reinterpret_cast<const uint2*>(from);
+          w[0] = x.x; w[1] = x.y;
         }
         if (!ok) {
 #pragma unroll
-          for (int g = 0; g < NG / 2; ++g) {
-            ks[g] = vs[g] = vz[g] = 0u;
-            *reinterpret_cast<uint2*>(kp + 8 * g) = make_uint2(0u, 0u);
+          for (int g = 0; g < NG; ++g) {
+            w[g] = 0u;
+            *reinterpret_cast<uint32_t*>(from + 4 * g) = 0u;
           }
         }
-        // [chunk][half of the chunk][tig][group][row sigma(2 tig), sigma(2 tig + 1)]
-        float* out = rows_f32 + (((lane >> 3) * 4 + (lane & 3)) * NG) * 2 + ((lane >> 2) & 1);
-        vtop = 0u;
+        float* out = rows_f32 + kind * (2 * kKv4Chunk * NG) + (((r >> 3) * 4 + (r & 3)) * NG) * 2 + ((r >> 2) & 1);
+        uint32_t top = 0u;
 #pragma unroll
         for (int g = 0; g < NG / 2; ++g) {
-          const float2 k = unpack_f16(ks[g]), v = unpack_f16(vs[g]), z = unpack_f16(vz[g]);
-          out[4 * g] = k.x;
-          out[4 * g + 2] = k.y;
-          out[32 * NG + 4 * g] = v.x;
-          out[32 * NG + 4 * g + 2] = v.y;
-          out[64 * NG + 4 * g] = fmaf(7.5f, v.x, z.x);
-          out[64 * NG + 4 * g + 2] = fmaf(7.5f, v.y, z.y);
-          vtop = max(vtop, max(vs[g] & 0xffffu, vs[g] >> 16));  // positive f16 order as integers
+          const float2 v = unpack_f16(w[g]), z = unpack_f16(w[NG / 2 + g]);
+          out[4 * g] = v.x;
+          out[4 * g + 2] = v.y;
+          out[kKv4Chunk * NG + 4 * g] = fmaf(7.5f, v.x, z.x);
+          out[kKv4Chunk * NG + 4 * g + 2] = fmaf(7.5f, v.y, z.y);
+          top = max(top, max(w[g] & 0xffffu, w[g] >> 16));  // positive f16 order as integers
         }
-        vtop = __reduce_max_sync(0xffffffffu, vtop);
+        vtop = __reduce_max_sync(0xffffffffu, kind ? top : 0u);
       }
       __syncwarp();
-      if (i + 1 < mine) issue(i + 1);
-      cp_async_commit();
 
-      // scores (log2 units) of head gid with row 8 j + tig (and + 4) of chunk u: s[4 u + 2 j (+ 1)]
-      float s[8];
+      // scores (log2 units) of head gid with row 8 j + tig (and + 4): s[2 j (+ 1)]
+      float s[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint8_t* kc = st + u * SH::CHUNK;
-          const uint8_t* kp = kc + 2 * SH::CODE;
-          uint32_t kw[NG];
-          if constexpr (NG == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(kc + (8 * j + gid) * (HD / 2) + 16 * tig);
-            kw[0] = v.x; kw[1] = v.y; kw[2] = v.z; kw[3] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(kc + (8 * j + gid) * (HD / 2) + 8 * tig);
-            kw[0] = v.x; kw[1] = v.y;
-          }
-          uint64_t sc[NG];
-          load_pairs<NG>(rows_f32 + ((2 * u + j) * 4 + tig) * NG * 2, sc);
-          // the minima's part: all parameters of row sigma(gid) times (7.5 and 1) x the groups' query sums
-          float z[4];
-          const int zr = 8 * j + (gid >> 1) + 4 * (gid & 1);
-          mma_f16_k8_new(z, zh, zl, *reinterpret_cast<const uint32_t*>(kp + zr * (4 * NG) + 4 * (NG == 4 ? tig : (tig & 1))));
-          uint64_t d = pair(0.0f, 0.0f);
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            float acc[4];
-            const uint32_t w = kw[g], w8 = w >> 8;
-            mma_f16_new(acc, qh[g][0], ql[g][0], qh[g][1], ql[g][1], as_u32(centre_low(w)), as_u32(centre_high(w)));
-            mma_f16(acc, qh[g][2], ql[g][2], qh[g][3], ql[g][3], as_u32(centre_low(w8)), as_u32(centre_high(w8)));
-            d = fma2(sc[g], add2(pair(acc[0], acc[1]), pair(acc[2], acc[3])), d);
-          }
-          const float2 y = unpair(fma2(d, pair(factor, factor), mul2(add2(pair(z[0], z[1]), pair(z[2], z[3])), pair(zfactor, zfactor))));
-          s[4 * u + 2 * j] = y.x;
-          s[4 * u + 2 * j + 1] = y.y;
+      for (int j = 0; j < 2; ++j) {
+        const uint8_t* kp = st + 2 * SH::CODE;
+        uint32_t kw[NG];
+        if constexpr (NG == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(st + (8 * j + gid) * (HD / 2) + 16 * tig);
+          kw[0] = v.x; kw[1] = v.y; kw[2] = v.z; kw[3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(st + (8 * j + gid) * (HD / 2) + 8 * tig);
+          kw[0] = v.x; kw[1] = v.y;
         }
-      }
-      if (sight != 0xffffffffu) {
-        const uint32_t at = sight >> tig;
+        uint64_t sc[NG];
+        load_pairs<NG>(rows_f32 + (j * 4 + tig) * NG * 2, sc);
+        // the minima's part: all parameters of row sigma(gid) times (7.5 and 1) x the groups' query sums
+        float z[4];
+        const int zr = 8 * j + (gid >> 1) + 4 * (gid & 1);
+        mma_f16_k8_new(z, zh, zl, *reinterpret_cast<const uint32_t*>(kp + zr * (4 * NG) + 4 * (NG == 4 ? tig : (tig & 1))));
+        uint64_t d = pair(0.0f, 0.0f);
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          if (!(at >> (4 * x) & 1u)) s[x] = -INFINITY;
+        for (int g = 0; g < NG; ++g) {
+          float acc[4];
+          const uint32_t w = kw[g], w8 = w >> 8;
+          mma_f16_new(acc, qh[g][0], ql[g][0], qh[g][1], ql[g][1], as_u32(centre_low(w)), as_u32(centre_high(w)));
+          mma_f16(acc, qh[g][2], ql[g][2], qh[g][3], ql[g][3], as_u32(centre_low(w8)), as_u32(centre_high(w8)));
+          d = fma2(sc[g], add2(pair(acc[0], acc[1]), pair(acc[2], acc[3])), d);
+        }
+        const float2 y = unpair(fma2(d, pair(factor, factor), mul2(add2(pair(z[0], z[1]), pair(z[2], z[3])), pair(zfactor, zfactor))));
+        s[2 * j] = y.x;
+        s[2 * j + 1] = y.y;
       }
-      float tm = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      if ((sight & 0xffffu) != 0xffffu) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (!(sight >> (4 * x + tig) & 1u)) s[x] = -INFINITY;
+      }
+      float tm = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
 
@@ -504,57 +487,53 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
         }
       }
 
+      // weights: plain for the sum and the minima, times scale and as two f16 terms for the codes
+      float w[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        // weights: plain for the sum and the minima, times scale and as two f16 terms for the codes
-        float w[4];
+      for (int x = 0; x < 4; ++x) {
+        w[x] = exp2_fast(s[x] - ref);
+        l += w[x];
+      }
+      uint32_t wh[NG][2], wl[NG][2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          w[x] = exp2_fast(s[4 * u + x] - ref);
-          l += w[x];
-        }
-        uint32_t wh[NG][2], wl[NG][2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint64_t ww = pair(w[2 * j], w[2 * j + 1]);
-          uint64_t sc[NG], mid[NG];
-          load_pairs<NG>(rows_f32 + 32 * NG + ((2 * u + j) * 4 + tig) * NG * 2, sc);
-          load_pairs<NG>(rows_f32 + 64 * NG + ((2 * u + j) * 4 + tig) * NG * 2, mid);
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            oz[g] = fma2(ww, mid[g], oz[g]);
-            split_pair(mul2(ww, sc[g]), wh[g][j], wl[g][j]);
-          }
-        }
-        // value codes of unit gid, rows in the same order
-        uint32_t vw[4][NG / 2];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int r = 8 * (x >> 1) + 4 * (x & 1) + tig;
-          const uint8_t* v = st + u * SH::CHUNK + SH::CODE + r * (HD / 2);
-          if constexpr (NG == 4) {
-            const uint2 y = *reinterpret_cast<const uint2*>(v + 16 * ((gid >> 1) ^ (r & 2)) + 8 * (gid & 1));
-            vw[x][0] = y.x; vw[x][1] = y.y;
-          } else {
-            vw[x][0] = *reinterpret_cast<const uint32_t*>(v + 4 * gid);
-          }
-        }
+      for (int j = 0; j < 2; ++j) {
+        const uint64_t ww = pair(w[2 * j], w[2 * j + 1]);
+        const float* v = rows_f32 + 2 * kKv4Chunk * NG + (j * 4 + tig) * NG * 2;
+        uint64_t sc[NG], mid[NG];
+        load_pairs<NG>(v, sc);
+        load_pairs<NG>(v + kKv4Chunk * NG, mid);
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          const uint32_t t0 = __byte_perm(vw[0][g / 2], vw[1][g / 2], (g & 1) ? 0x7632 : 0x5410);
-          const uint32_t t1 = __byte_perm(vw[2][g / 2], vw[3][g / 2], (g & 1) ? 0x7632 : 0x5410);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t u0 = e ? t0 >> 8 : t0, u1 = e ? t1 >> 8 : t1;
-            const uint32_t a0 = as_u32(centre_low(u0)), a1 = as_u32(centre_high(u0));
-            const uint32_t a2 = as_u32(centre_low(u1)), a3 = as_u32(centre_high(u1));
-            mma_f16(o[2 * g + e], a0, a1, a2, a3, wh[g][0], wh[g][1]);
-            mma_f16(o[2 * g + e], a0, a1, a2, a3, wl[g][0], wl[g][1]);
-          }
+          oz[g] = fma2(ww, mid[g], oz[g]);
+          split_pair(mul2(ww, sc[g]), wh[g][j], wl[g][j]);
         }
       }
-      row0 = next0;
-      row1 = next1;
+      // value codes of unit gid, rows in the same order
+      uint32_t vw[4][NG / 2];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = 8 * (x >> 1) + 4 * (x & 1) + tig;
+        const uint8_t* v = st + SH::CODE + r * (HD / 2);
+        if constexpr (NG == 4) {
+          const uint2 y = *reinterpret_cast<const uint2*>(v + 16 * ((gid >> 1) ^ (r & 2)) + 8 * (gid & 1));
+          vw[x][0] = y.x; vw[x][1] = y.y;
+        } else {
+          vw[x][0] = *reinterpret_cast<const uint32_t*>(v + 4 * gid);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const uint32_t t0 = __byte_perm(vw[0][g / 2], vw[1][g / 2], (g & 1) ? 0x7632 : 0x5410);
+        const uint32_t t1 = __byte_perm(vw[2][g / 2], vw[3][g / 2], (g & 1) ? 0x7632 : 0x5410);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t u0 = e ? t0 >> 8 : t0, u1 = e ? t1 >> 8 : t1;
+          const uint32_t a0 = as_u32(centre_low(u0)), a1 = as_u32(centre_high(u0));
+          const uint32_t a2 = as_u32(centre_low(u1)), a3 = as_u32(centre_high(u1));
+          mma_f16(o[2 * g + e], a0, a1, a2, a3, wh[g][0], wh[g][1]);
+          mma_f16(o[2 * g + e], a0, a1, a2, a3, wl[g][0], wl[g][1]);
+        }
+      }
     }
     cp_async_wait<0>();
 
