@@ -36,6 +36,10 @@ constexpr int kDThreads = 32 * kDWarps;
 constexpr int kDStages = 4;       // chunks of a warp's ring
 constexpr int kDRows = 512;       // query rows of one launch (their chunk counts are in shared memory)
 constexpr int kDItem = 18;        // what an item costs a CTA besides its chunks, in chunks
+constexpr int kDJoin = 12;        // parts that are joined at once, and in groups of how many where there are more
+constexpr int kDGroup = 10;
+constexpr int kDGroupMax = 32;    // (the larger of kDJoin, kDGroup and the groups of all CTAs)
+constexpr int kDCounters = 1 << 15;  // items' counters, then the groups'
 constexpr int kDSizes = 8;        // sizes of a part that are tried, kDWarps chunks apart
 
 template <int HD>
@@ -188,7 +192,6 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   float* wgt = reinterpret_cast<float*>(smem + kBody + kDRows * 16);    // [warp][head] combine weights
   float* total = wgt + 64;                                              // [head] max, [head] sum
   int* flag = reinterpret_cast<int*>(total + 16);
-  uint32_t* fits = reinterpret_cast<uint32_t*>(flag + 2);               // [kDSizes] parts of all rows
   int64_t* scan = reinterpret_cast<int64_t*>(total + 32);               // [8] warp sums
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   const Kv4View& c = a.c;
@@ -197,39 +200,63 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
   pdl_trigger();
   pdl_wait();
 
-  // chunk counts of the rows (a row that sees nothing counts one, for its output)
+  // chunk counts of the rows (a row that sees nothing counts one, for its output), and sums of costs or
+  // parts over the rows before each: up to 32 rows in every warp's registers, more by way of shared memory
   const int G = a.H / c.heads, nsub = (G + 7) / 8, HS = c.heads * nsub;
-  int counts[kDRows / kDThreads];
+  const bool few = a.M <= 32;
+  auto row_of = [&](int m, int& p, int& sl) -> int {
+    p = a.pos[m];
+    sl = a.slot[m];
+    const bool ok = p >= 0 && sl >= 0 && sl < c.slots && kv4_in_reach(c, p, a.window, 0);
+    if (p >= 0 && !ok && blockIdx.x == 0) atomicOr(a.err, SHD_DEVERR_ARG);
+    if (!ok) p = -1;
+    return max(kv4_spans(c, p, p, a.window).total, 1);
+  };
+  int my_p = -1, my_slot = 0;            // of row `lane`, where the rows are few
+  int64_t my_pre = 0, sum = 0;
+  int size = 0;                          // of a part, in chunks; 0: equal shares of all chunks
+  if (few) {
+    const int n = lane < a.M ? row_of(lane, my_p, my_slot) : 0;
+    auto prefix = [&](int64_t v) {
+      int64_t x = lane < a.M ? v : 0;
+      const int64_t own = x;
 #pragma unroll
-  for (int i = 0; i < kDRows / kDThreads; ++i) {
-    const int m = i * kDThreads + tid;
-    counts[i] = 0;
-    if (m < a.M) {
-      int p = a.pos[m];
-      const int sl = a.slot[m];
-      const bool ok = p >= 0 && sl >= 0 && sl < c.slots && kv4_in_reach(c, p, a.window, 0);
-      if (p >= 0 && !ok && blockIdx.x == 0) atomicOr(a.err, SHD_DEVERR_ARG);
-      if (!ok) p = -1;
-      rows[m] = make_int2(p, sl);
-      counts[i] = max(kv4_spans(c, p, p, a.window).total, 1);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      my_pre = x - own;
+      sum = __shfl_sync(0xffffffffu, x, 31);
+    };
+    prefix((int64_t)n + kDItem);
+    if (a.M * HS <= (int)gridDim.x) {
+      // the least size, in steps of kDWarps, that gives every CTA at most one part: lane y tries the y-th
+      const int64_t chunks = (sum - (int64_t)a.M * kDItem) * HS;
+      const uint32_t first = (uint32_t)(((chunks + gridDim.x - 1) / gridDim.x + kDWarps - 1) / kDWarps) * kDWarps;
+      const uint32_t mine = first + kDWarps * lane;
+      uint32_t all = 0;
+      for (int m = 0; m < a.M; ++m) all += ((uint32_t)__shfl_sync(0xffffffffu, n, m) + mine - 1) / mine;
+      const uint32_t fit = __ballot_sync(0xffffffffu, (uint64_t)all * HS <= gridDim.x) & ((1u << kDSizes) - 1u);
+      if (fit) {
+        size = (int)first + kDWarps * (__ffs(fit) - 1);
+        prefix((n + size - 1) / size);
+      }
     }
-  }
-  if (tid < kDSizes) fits[tid] = 0u;
-  // sums over the rows before each, of f(count), into pre; returns the sum over all
-  auto prefix = [&](auto f) -> int64_t {
-    int64_t sum = 0;
-#pragma unroll
-    for (int i = 0; i < kDRows / kDThreads; ++i) {
-      if (i * kDThreads >= a.M) break;
-      const int m = i * kDThreads + tid;
-      const int64_t n = m < a.M ? f(counts[i]) : 0;
+  } else {
+    for (int m0 = 0; m0 < a.M; m0 += kDThreads) {
+      const int m = m0 + tid;
+      int64_t n = 0;
+      if (m < a.M) {
+        int p, sl;
+        n = row_of(m, p, sl) + kDItem;
+        rows[m] = make_int2(p, sl);
+      }
       int64_t x = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
       }
-      __syncthreads();
       if (lane == 31) scan[warp] = x;
       __syncthreads();
       int64_t base = sum;
@@ -239,47 +266,40 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
         sum += scan[w];
       }
       if (m < a.M) pre[m] = base + x - n;
+      __syncthreads();
     }
-    return sum;
-  };
-  int64_t sum = prefix([](int n) { return (int64_t)n + kDItem; });
-  const int64_t share = ((sum - (int64_t)a.M * kDItem) * HS + gridDim.x - 1) / gridDim.x;  // chunks a CTA
-  int size = 0;  // of a part; 0: equal shares
-  if ((int64_t)a.M * HS <= gridDim.x) {
-    const uint32_t first = (uint32_t)((share + kDWarps - 1) / kDWarps) * kDWarps;
-#pragma unroll
-    for (int y = 0; y < kDSizes; ++y) {
-      uint32_t n = 0;
-#pragma unroll
-      for (int i = 0; i < kDRows / kDThreads; ++i) n += ((uint32_t)counts[i] + first + kDWarps * y - 1) / (first + kDWarps * y);
-      n = __reduce_add_sync(0xffffffffu, n);
-      if (lane == 0 && n) atomicAdd(fits + y, n);
-    }
-    __syncthreads();
-    for (int y = kDSizes - 1; y >= 0; --y)
-      if ((uint64_t)fits[y] * HS <= gridDim.x) size = (int)first + kDWarps * y;
-    if (size) sum = prefix([size](int n) { return (int64_t)((n + size - 1) / size); });
   }
-  __syncthreads();
   const int64_t T = sum * HS;
   const int64_t per = size ? 1 : (T + gridDim.x - 1) / gridDim.x;
   const int64_t t_begin = blockIdx.x * per, t_end = min(T, t_begin + per);
 
   for (int64_t t = t_begin; t < t_end;) {
     // the item that t falls into: its parts, or kDItem for its start and end, then its chunks
-    int lo = 0, hi = a.M - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pre[mid] * HS <= t) lo = mid; else hi = mid - 1;
+    int m, p, sl, cost;
+    int64_t row_t;
+    if (few) {
+      m = 31 - __clz(__ballot_sync(0xffffffffu, lane < a.M && my_pre * HS <= t));
+      p = __shfl_sync(0xffffffffu, my_p, m);
+      sl = __shfl_sync(0xffffffffu, my_slot, m);
+      const int64_t here = __shfl_sync(0xffffffffu, my_pre, m), next = __shfl_sync(0xffffffffu, my_pre, (m + 1) & 31);
+      row_t = here * HS;
+      cost = (int)((m + 1 < a.M ? next : sum) - here);
+    } else {
+      int lo = 0, hi = a.M - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] * HS <= t) lo = mid; else hi = mid - 1;
+      }
+      m = lo;
+      p = rows[m].x;
+      sl = rows[m].y;
+      row_t = pre[m] * HS;
+      cost = (int)((m + 1 < a.M ? pre[m + 1] : sum) - pre[m]);
     }
-    const int m = lo;
-    const int64_t row_t = pre[m] * HS;
-    const int cost = (int)((m + 1 < a.M ? pre[m + 1] : sum) - pre[m]);
     const uint64_t in_row = (uint64_t)(t - row_t);
     const int hs = in_row >> 32 ? (int)(in_row / (uint64_t)cost) : (int)((uint32_t)in_row / (uint32_t)cost);
     const int64_t item_t = row_t + (int64_t)hs * cost;
     const int64_t done = min(t_end, item_t + cost);
-    const int p = rows[m].x, sl = rows[m].y;
     const Kv4Spans sp = kv4_spans(c, p, p, a.window);
     int n, c0, c1, w0, parts;  // chunks, this CTA's of them, first CTA of the item and how many
     if (size) {
@@ -595,44 +615,57 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
       }
     }
     if (!whole) {
-      // the last CTA of the item joins the parts in CTA order
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        int* counter = counters + (size_t)m * HS + hs;
-        const int last = atomicAdd(counter, 1) == parts - 1;
-        if (last) *counter = 0;
-        *flag = last;
-      }
-      __syncthreads();
-      if (*flag) {
+      // The last CTA of the item to arrive joins the parts in CTA order; of many parts the last of each
+      // group of `group` CTAs first joins its group's (one SM takes in 64 bytes a clock).
+      const int mine_at = (int)blockIdx.x - w0;
+      const int group = parts > kDJoin ? kDGroup : parts, g0 = mine_at / group * group, members = min(group, parts - g0);
+      auto arrive = [&](int* counter, int n) -> bool {
         __threadfence();
-        // of part w: in its CTA the item is the first unless it begins there
-        const float* first_part = ws + ((size_t)w0 * 2 + ((int64_t)w0 * per >= item_t ? 0 : 1)) * SH::LEFT;
-        const float* next_parts = ws + (size_t)(w0 + 1) * 2 * SH::LEFT;
-        float* sm = reinterpret_cast<float*>(smem);  // [part][8] maxima, then weights
-        float* sl = sm + 8 * gridDim.x;
-        for (int x = tid; x < parts * 8; x += kDThreads) {
+        __syncthreads();
+        if (tid == 0) {
+          const int last = atomicAdd(counter, 1) == n - 1;
+          if (last) *counter = 0;
+          *flag = last;
+        }
+        __syncthreads();
+        const bool last = *flag != 0;
+        if (last) __threadfence();
+        return last;
+      };
+      // a part's place: in its CTA the item is the first unless it begins there
+      auto place_at = [&](int i) -> int { return (w0 + i) * 2 + ((int64_t)(w0 + i) * per >= item_t ? 0 : 1); };
+      auto place = [&](int i) -> float* { return ws + (size_t)place_at(i) * SH::LEFT; };
+      // parts g0, g0 + step, .. : n of them, into the first one's place or out
+      auto join = [&](int i0, int step, int n, bool last) {
+        float* sm = reinterpret_cast<float*>(smem);  // [part][8] maxima, then weights; sums
+        float* sl = sm + 8 * kDGroupMax;
+        float* first_part = place(i0);
+        const float* next_parts = n > 1 ? place(i0 + step) : first_part;
+        const size_t far = (size_t)step * 2 * SH::LEFT;
+        for (int x = tid; x < n * 8; x += kDThreads) {
           const int w = x / 8, h = x % 8;
-          const float* in = w == 0 ? first_part : next_parts + (size_t)(w - 1) * 2 * SH::LEFT;
+          const float* in = w == 0 ? first_part : next_parts + (w - 1) * far;
           sm[x] = h < nh ? __ldcg(in + 8 * HD + h) : -INFINITY;
           sl[x] = h < nh ? __ldcg(in + 8 * HD + 8 + h) : 0.0f;
         }
         __syncthreads();
-        if (warp < 8) {
+        {
           const int h = warp;
           float M = -INFINITY, L = 0.0f;
-          for (int w = lane; w < parts; w += 32) M = fmaxf(M, sm[w * 8 + h]);
+          for (int w = lane; w < n; w += 32) M = fmaxf(M, sm[w * 8 + h]);
 #pragma unroll
           for (int x = 16; x >= 1; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-          for (int w = lane; w < parts; w += 32) {
+          for (int w = lane; w < n; w += 32) {
             const float mw = sm[w * 8 + h], e = mw == -INFINITY ? 0.0f : exp2_fast(mw - M);
             L = fmaf(sl[w * 8 + h], e, L);
             sm[w * 8 + h] = e;
           }
 #pragma unroll
           for (int x = 16; x >= 1; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
-          if (lane == 0) total[8 + h] = L;
+          if (lane == 0) {
+            total[h] = M;
+            total[8 + h] = L;
+          }
         }
         __syncthreads();
         for (int x = tid; x < nh * (HD / 4); x += kDThreads) {
@@ -640,10 +673,27 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
           float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
           add_part4(y, __ldcg(reinterpret_cast<const float4*>(first_part + h * HD + d)), sm[h]);
 #pragma unroll 8
-          for (int w = 1; w < parts; ++w)
-            add_part4(y, __ldcg(reinterpret_cast<const float4*>(next_parts + (size_t)(w - 1) * 2 * SH::LEFT + h * HD + d)), sm[w * 8 + h]);
-          store_shares(a, (size_t)m * a.H * HD + (size_t)(h0 + h) * HD + d, y, total[8 + h]);
+          for (int w = 1; w < n; ++w)
+            add_part4(y, __ldcg(reinterpret_cast<const float4*>(next_parts + (w - 1) * far + h * HD + d)), sm[w * 8 + h]);
+          if (last) {
+            store_shares(a, (size_t)m * a.H * HD + (size_t)(h0 + h) * HD + d, y, total[8 + h]);
+          } else {
+            *reinterpret_cast<float4*>(first_part + h * HD + d) = y;
+            if (d == 0) {
+              first_part[8 * HD + h] = total[h];
+              first_part[8 * HD + 8 + h] = total[8 + h];
+            }
+          }
         }
+      };
+      int* counter = counters + (size_t)m * HS + hs;
+      if (group == parts) {
+        if (arrive(counter, parts)) join(0, 1, parts, true);
+      } else if (arrive(counters + kDCounters + place_at(g0), members)) {
+        join(g0, 1, members, false);
+        __syncthreads();
+        const int groups = (parts + group - 1) / group;
+        if (arrive(counter, groups)) join(0, group, groups, true);
       }
     }
     __syncthreads();  // the shared memory is used again
@@ -660,9 +710,10 @@ int launch_decode_t(shd_ctx* ctx, const Kv4AttnArgs& a0) {
     attr_devices |= 1u << (ctx->device & 31);
   }
   const int HS = a0.c.heads * ((a0.H / a0.c.heads + 7) / 8);
-  SHD_REQUIRE(ctx, HS <= ctx->n_counters, "shd_kv4_attn_decode: too many heads");
-  const int step = std::min(kDRows, ctx->n_counters / HS);
+  SHD_REQUIRE(ctx, HS <= kDCounters, "shd_kv4_attn_decode: too many heads");
+  const int step = std::min(kDRows, kDCounters / HS);
   const int grid = kv4_decode_ctas(ctx->num_sms);
+  SHD_REQUIRE(ctx, kDCounters + 2 * grid <= ctx->n_counters && grid <= kDGroup * kDGroupMax, "shd_kv4_attn_decode: unknown GPU size");
   for (int m = 0; m < a0.M; m += step) {
     Kv4AttnArgs a = a0;
     const size_t width = (size_t)a.H * HD;
