@@ -424,6 +424,13 @@ int shd_model_set_head(shd_model* m, const uint16_t* lm_head, const float* final
  * triple store: [0,h) input norm, [h, h+H*d) attention, [2h,3h) post-attention norm, [3h, 3h+I)
  * SwiGLU; the final norm uses layer L-1's [0,h). NULL clears (V3: reshare (y, 0)). */
 int shd_model_set_masks(shd_model* m, const float* masks, int64_t stride);
+/* Hold the key/value cache in 4 bits (the format of shd_kv4_cache above) instead of f32: `capacity`
+ * rows a slot (rounded up to a multiple of 16), attention limited to `window` positions (0: none) with
+ * the first `sinks` always visible. A capacity below max_seq makes the rows behind the sinks a ring and
+ * needs window + 511 <= capacity - sinks (prompts are taken in blocks of 512 positions). K and V are
+ * quantised from their shares as the q/k/v linear gives them; attention then reads the quantised values,
+ * of the prompt too. Only while no slot holds a sequence, and on single-GPU models. Frees the f32 cache. */
+int shd_model_set_kv4(shd_model* m, int capacity, int window, int sinks);
 /* Forget all sequences. */
 int shd_model_reset(shd_model* m);
 /* Prefill a prompt into sequence slot `slot` (chunks of up to 512 positions through the tensor-core

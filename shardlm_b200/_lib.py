@@ -99,6 +99,7 @@ SIGNATURES: dict[str, tuple] = {
     "shd_model_set_embedding": (I32, [P, P]),
     "shd_model_set_head": (I32, [P, P, P]),
     "shd_model_set_masks": (I32, [P, P, I64]),
+    "shd_model_set_kv4": (I32, [P, I32, I32, I32]),
     "shd_model_reset": (I32, [P]),
     "shd_model_prefill": (I32, [P, I32, P, I32, P]),
     "shd_model_decode_async": (I32, [P, I32]),

@@ -18,19 +18,9 @@ __device__ __forceinline__ void group_params(float lo, float hi, __half& s, __ha
   s = __float2half_rn(__fmul_rn(fmaxf(__fsub_rn(hi, __half2float(z)), 0.0f), 1.0f / 15.0f));
 }
 
-struct WriteArgs {
-  Kv4View c;
-  const float *kc, *ks, *vc, *vs;  // shares [M][ld]; the server's null: the client's hold the values
-  int ld;
-  const int32_t *slot, *pos;  // null: row m is position pos0 + m of slot0
-  int slot0, pos0, M;
-  float *k_val, *v_val;  // [M][heads * head_dim], nullable
-  int* err;
-};
-
 // Four channels a thread, so a group is 8 neighbouring lanes and its least and greatest value three
 // shuffles each.
-__global__ void __launch_bounds__(kWriteThreads) kv4_write_kernel(const WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads) kv4_write_kernel(const Kv4WriteArgs a) {
   pdl_trigger();
   pdl_wait();
   const int hd = a.c.head_dim, lanes = hd / 4, ng = hd / kKv4Group;
@@ -221,6 +211,7 @@ int check_attn(shd_ctx* ctx, const char* fn, const shd_kv4_cache* cache, const f
   a.window = window;
   a.scale = 1.0f / sqrtf((float)a.c.head_dim);
   a.mask = mask;
+  a.ldmask = (int64_t)H * a.c.head_dim;
   a.out_c = out_c;
   a.out_s = out_s;
   a.err = ctx->d_err;
@@ -228,6 +219,25 @@ int check_attn(shd_ctx* ctx, const char* fn, const shd_kv4_cache* cache, const f
 }
 
 }  // namespace
+
+int launch_kv4_write(shd_ctx* ctx, const Kv4WriteArgs& a) {
+  SHD_REQUIRE(ctx, (int64_t)a.M * a.c.heads <= 0x7fffffff, "shd_kv4_write: too many rows");
+  const int per_block = kWriteThreads / (a.c.head_dim / 4);
+  const int64_t blocks = ((int64_t)a.M * a.c.heads + per_block - 1) / per_block;
+  SHD_CHECK_CUDA(ctx, launch_pdl(kv4_write_kernel, dim3((unsigned)blocks), dim3(kWriteThreads), 0, ctx->stream, a));
+  ctx->launches++;
+  return SHD_OK;
+}
+
+int launch_kv4_read(shd_ctx* ctx, const Kv4View& c, int slot, int pos0, int n, float* k_out, float* v_out) {
+  SHD_REQUIRE(ctx, (int64_t)n * c.heads <= 0x7fffffff, "shd_kv4_read: too many rows");
+  const uint32_t units = (uint32_t)n * (uint32_t)c.heads, blocks = units / (kWriteThreads / 8) + (units % (kWriteThreads / 8) ? 1 : 0);
+  SHD_CHECK_CUDA(ctx, launch_pdl(c.head_dim == 128 ? kv4_read_kernel<4> : kv4_read_kernel<2>, dim3(blocks),
+                                 dim3(kWriteThreads), 0, ctx->stream, c, slot, pos0, units, k_out, v_out));
+  ctx->launches++;
+  return SHD_OK;
+}
+
 }  // namespace shd
 
 using namespace shd;
@@ -236,7 +246,7 @@ extern "C" int shd_kv4_write(shd_ctx* ctx, const shd_kv4_cache* cache, const flo
                              const float* vs, int ld, const int32_t* slot, const int32_t* pos, int slot0, int pos0,
                              int M, float* k_val, float* v_val) {
   if (!ctx) return SHD_ERR_ARG;
-  WriteArgs a{};
+  Kv4WriteArgs a{};
   const int rc = check_cache(ctx, "shd_kv4_write", cache, a.c);
   if (rc) return rc;
   SHD_REQUIRE(ctx, kc && vc && (ks == nullptr) == (vs == nullptr), "shd_kv4_write: null pointer");
@@ -256,12 +266,7 @@ extern "C" int shd_kv4_write(shd_ctx* ctx, const shd_kv4_cache* cache, const flo
   a.slot = slot; a.pos = pos; a.slot0 = slot0; a.pos0 = pos0; a.M = M;
   a.k_val = k_val; a.v_val = v_val;
   a.err = ctx->d_err;
-  SHD_REQUIRE(ctx, (int64_t)M * a.c.heads <= 0x7fffffff, "shd_kv4_write: too many rows");
-  const int per_block = kWriteThreads / (a.c.head_dim / 4);
-  const int64_t blocks = ((int64_t)M * a.c.heads + per_block - 1) / per_block;
-  SHD_CHECK_CUDA(ctx, launch_pdl(kv4_write_kernel, dim3((unsigned)blocks), dim3(kWriteThreads), 0, ctx->stream, a));
-  ctx->launches++;
-  return SHD_OK;
+  return launch_kv4_write(ctx, a);
 }
 
 extern "C" int shd_kv4_read(shd_ctx* ctx, const shd_kv4_cache* cache, int slot, int pos0, int n, float* k_out,
@@ -276,12 +281,7 @@ extern "C" int shd_kv4_read(shd_ctx* ctx, const shd_kv4_cache* cache, int slot, 
   SHD_REQUIRE(ctx, (int64_t)pos0 + n <= c.capacity || n <= c.capacity - c.sinks, "shd_kv4_read: more rows than the ring holds");
   SHD_REQUIRE(ctx, shd_aligned16(k_out) && shd_aligned16(v_out), "shd_kv4_read: tensors must be 16-byte aligned");
   SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
-  SHD_REQUIRE(ctx, (int64_t)n * c.heads <= 0x7fffffff, "shd_kv4_read: too many rows");
-  const uint32_t units = (uint32_t)n * (uint32_t)c.heads, blocks = units / (kWriteThreads / 8) + (units % (kWriteThreads / 8) ? 1 : 0);
-  SHD_CHECK_CUDA(ctx, launch_pdl(c.head_dim == 128 ? kv4_read_kernel<4> : kv4_read_kernel<2>, dim3(blocks),
-                                 dim3(kWriteThreads), 0, ctx->stream, c, slot, pos0, units, k_out, v_out));
-  ctx->launches++;
-  return SHD_OK;
+  return launch_kv4_read(ctx, c, slot, pos0, n, k_out, v_out);
 }
 
 extern "C" int shd_kv4_attn_decode(shd_ctx* ctx, const shd_kv4_cache* cache, const float* q, int ldq, int H,

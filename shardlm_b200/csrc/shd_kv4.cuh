@@ -181,10 +181,24 @@ struct Kv4AttnArgs {
   int slot0, pos0;
   int window;   // 0: every earlier position
   float scale;  // 1 / sqrt(head_dim)
-  const float* mask;       // [M][H * head_dim], nullable
+  const float* mask;       // [M][ldmask], H * head_dim used, nullable
+  int64_t ldmask;          // 0: one row for all
   float *out_c, *out_s;    // [M][H * head_dim]
   int* err;
 };
+
+// Rows of K and V into the cache and back (shd_kv4.cu; arguments as at the C entries, checked there).
+struct Kv4WriteArgs {
+  Kv4View c;
+  const float *kc, *ks, *vc, *vs;  // shares [M][ld]; the server's null: the client's hold the values
+  int ld;
+  const int32_t *slot, *pos;  // null: row m is position pos0 + m of slot0
+  int slot0, pos0, M;
+  float *k_val, *v_val;  // [M][heads * head_dim], nullable
+  int* err;
+};
+int launch_kv4_write(shd_ctx* ctx, const Kv4WriteArgs& a);
+int launch_kv4_read(shd_ctx* ctx, const Kv4View& c, int slot, int pos0, int n, float* k_out, float* v_out);
 
 // Single-token attention (shd_kv4_decode.cu): CTAs of a launch, and the context scratch they leave the
 // parts of cut items in, two a CTA.

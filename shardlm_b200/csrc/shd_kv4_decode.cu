@@ -172,8 +172,9 @@ __device__ __forceinline__ void add_part(float4& y, const float* p, float e) {
 }
 
 // (y / L - mask, mask); a row that sees nothing (L = 0) gives 0
-__device__ __forceinline__ void store_shares(const Kv4AttnArgs& a, size_t at, const float4& y, float L) {
-  const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+__device__ __forceinline__ void store_shares(const Kv4AttnArgs& a, int m, int col, const float4& y, float L) {
+  const size_t at = (size_t)m * a.H * a.c.head_dim + col;
+  const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + m * a.ldmask + col) : make_float4(0.f, 0.f, 0.f, 0.f);
   const float D = L == 0.0f ? 1.0f : L;
   *reinterpret_cast<float4*>(a.out_c + at) =
       make_float4(__fsub_rn(__fdiv_rn(y.x, D), mk.x), __fsub_rn(__fdiv_rn(y.y, D), mk.y),
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
 #pragma unroll
       for (int w = 0; w < kDWarps; ++w) add_part(y, part + (w * 8 + h) * PART + 4 + d, wgt[w * 8 + h]);
       if (whole) {
-        store_shares(a, (size_t)m * a.H * HD + (size_t)(h0 + h) * HD + d, y, total[8 + h]);
+        store_shares(a, m, (h0 + h) * HD + d, y, total[8 + h]);
       } else {
         *reinterpret_cast<float4*>(out + h * HD + d) = y;
         if (d == 0) {
@@ -676,7 +677,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
           for (int w = 1; w < n; ++w)
             add_part4(y, __ldcg(reinterpret_cast<const float4*>(next_parts + (w - 1) * far + h * HD + d)), sm[w * 8 + h]);
           if (last) {
-            store_shares(a, (size_t)m * a.H * HD + (size_t)(h0 + h) * HD + d, y, total[8 + h]);
+            store_shares(a, m, (h0 + h) * HD + d, y, total[8 + h]);
           } else {
             *reinterpret_cast<float4*>(first_part + h * HD + d) = y;
             if (d == 0) {
@@ -721,7 +722,7 @@ int launch_decode_t(shd_ctx* ctx, const Kv4AttnArgs& a0) {
     a.q += (size_t)m * a.ldq;
     a.slot += m;
     a.pos += m;
-    if (a.mask) a.mask += m * width;
+    if (a.mask) a.mask += m * a.ldmask;
     a.out_c += m * width;
     a.out_s += m * width;
     SHD_CHECK_CUDA(ctx, launch_pdl(kv4_decode_kernel<HD>, dim3(grid), dim3(kDThreads), SH::SMEM, ctx->stream, a,

@@ -613,8 +613,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           const float4 v = *reinterpret_cast<const float4*>(stage + i * STRIDE + 4 * f);
           if (whole) {
             const int mm = group_of(rr);
-            const size_t to = (size_t)mm * a.H * HD + (size_t)(sg.head * G + rr - mm * G) * HD + ch;
-            const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + to) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const int in_row = (sg.head * G + rr - mm * G) * HD + ch;
+            const size_t to = (size_t)mm * a.H * HD + in_row;
+            const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + mm * a.ldmask + in_row) : make_float4(0.f, 0.f, 0.f, 0.f);
             *reinterpret_cast<float4*>(a.out_c + to) =
                 make_float4(__fsub_rn(v.x, mk.x), __fsub_rn(v.y, mk.y), __fsub_rn(v.z, mk.z), __fsub_rn(v.w, mk.w));
             *reinterpret_cast<float4*>(a.out_s + to) = mk;
@@ -939,10 +940,11 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ P
     for (int i = 0; i < CPL; ++i) y[i] = fmaf(v[i], e, y[i]);
   }
   const float D = L == 0.0f ? 1.0f : L;
-  const size_t at = (size_t)(r / G) * a.H * HD + (size_t)(sg.head * G + r % G) * HD + CPL * lane;
+  const int in_row = (int)(sg.head * G + r % G) * HD + CPL * lane;
+  const size_t at = (size_t)(r / G) * a.H * HD + in_row;
 #pragma unroll
   for (int i = 0; i < CPL; ++i) {
-    const float mk = a.mask ? a.mask[at + i] : 0.0f;
+    const float mk = a.mask ? a.mask[(r / G) * a.ldmask + in_row + i] : 0.0f;
     a.out_c[at + i] = __fsub_rn(__fdiv_rn(y[i], D), mk);
     a.out_s[at + i] = mk;
   }
@@ -970,7 +972,7 @@ int launch_prefill_t(shd_ctx* ctx, const Kv4AttnArgs& a0) {
     pa.a.M = std::min(step, a0.M - m);
     pa.a.pos0 += m;
     pa.a.q += (size_t)m * a0.ldq;
-    if (a0.mask) pa.a.mask += m * width;
+    if (a0.mask) pa.a.mask += m * a0.ldmask;
     pa.a.out_c += m * width;
     pa.a.out_s += m * width;
     pa.last = a0.pos0 + a0.M - 1;

@@ -397,6 +397,94 @@ extern "C" int shd_model_set_masks(shd_model* m, const float* masks, int64_t str
   return SHD_OK;
 }
 
+extern "C" int shd_model_set_kv4(shd_model* m, int capacity, int window, int sinks) {
+  if (!m) return SHD_ERR_ARG;
+  shd_ctx* ctx = m->ctx;
+  const shd_model_config& c = m->cfg;
+  for (int n : m->len) SHD_REQUIRE(ctx, n == 0, "shd_model_set_kv4: the model holds sequences");
+  if (c.tp_world > 1) return shd_fail(ctx, SHD_ERR_UNSUPPORTED, "shd_model_set_kv4: single-GPU models only");
+  SHD_REQUIRE(ctx, capacity > 0 && window >= 0 && sinks >= 0, "shd_model_set_kv4: bad shape");
+  const int cap = (int)std::min<int64_t>(((int64_t)capacity + kKv4Chunk - 1) / kKv4Chunk * kKv4Chunk, 0x7ffffff0);
+  SHD_REQUIRE(ctx, sinks < cap, "shd_model_set_kv4: sinks must be below the capacity");
+  SHD_REQUIRE(ctx, cap >= c.max_seq || (window > 0 && (int64_t)window + kPrefillRows - 1 <= cap - sinks),
+              "shd_model_set_kv4: a cache shorter than max_seq needs a window, and room for it, a prompt block (512) and the sinks");
+  SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
+  SHD_CHECK_CUDA(ctx, cudaStreamSynchronize(m->stream));
+  if (m->graph) {
+    cudaGraphExecDestroy(m->graph);
+    m->graph = nullptr;
+  }
+  auto drop = [&](void* p) {
+    if (!p) return;
+    m->owned.erase(std::remove(m->owned.begin(), m->owned.end(), p), m->owned.end());
+    cudaFree(p);
+  };
+  // the f32 cache goes first: the two need not fit side by side
+  for (void* p : {(void*)m->kcache, (void*)m->vcache, (void*)m->kv4.kc, (void*)m->kv4.kp, (void*)m->kv4.vc, (void*)m->kv4.vp}) drop(p);
+  m->kcache = m->vcache = nullptr;
+  Kv4View v{};
+  v.slots = c.max_batch; v.heads = m->sh.kv_head_count; v.head_dim = c.head_dim; v.sinks = sinks;
+  const size_t rows = (size_t)c.n_layers * v.slots * v.heads * cap;
+  struct A {
+    void** p;
+    size_t bytes;
+  } allocs[] = {
+      {(void**)&v.kc, rows * (c.head_dim / 2)}, {(void**)&v.kp, rows * (c.head_dim / kKv4Group) * 4},
+      {(void**)&v.vc, rows * (c.head_dim / 2)}, {(void**)&v.vp, rows * (c.head_dim / kKv4Group) * 4},
+      {(void**)&m->kv4_rows, m->kv4_rows ? 0 : (size_t)2 * m->R * (m->qd + 2 * m->kvd) * 4},
+  };
+  m->kv4 = Kv4View{};
+  for (auto& a : allocs) {
+    if (!a.bytes) continue;
+    cudaError_t e = cudaMalloc(a.p, a.bytes);
+    if (e != cudaSuccess) {  // no cache is left: calls that need one are refused until this one succeeds
+      for (void* p : {(void*)v.kc, (void*)v.kp, (void*)v.vc, (void*)v.vp}) drop(p);
+      return shd_cuda_fail(ctx, e, "shd_model_set_kv4: cudaMalloc");
+    }
+    m->owned.push_back(*a.p);
+  }
+  v.capacity = cap;
+  m->kv4 = v;
+  m->kv4_window = window;
+  return SHD_OK;
+}
+
+Kv4View shd_model::kv4_layer(int l) const {
+  Kv4View v = kv4;
+  const size_t rows = (size_t)l * v.slots * v.heads * v.capacity;
+  v.kc += rows * (v.head_dim / 2);
+  v.vc += rows * (v.head_dim / 2);
+  v.kp += rows * (v.head_dim / kKv4Group) * 2;
+  v.vp += rows * (v.head_dim / kKv4Group) * 2;
+  return v;
+}
+
+// Quantise the M rows that the q/k/v linear left in kv4_rows, then attend: Qbuf -> Abuf.
+int shd_model::kv4_attention(int l, int M, const int* d_pos, const int* d_seq, const float* mask, bool decode) {
+  const int ld = qd + 2 * kvd;
+  Kv4WriteArgs w{};
+  w.c = kv4_layer(l);
+  w.kc = kv4_rows + qd; w.ks = w.kc + (size_t)M * ld;
+  w.vc = w.kc + kvd; w.vs = w.ks + kvd;
+  w.ld = ld; w.slot = d_seq; w.pos = d_pos; w.M = M; w.err = ctx->d_err;
+  const int rc = launch_kv4_write(ctx, w);
+  if (rc) return rc;
+  Kv4AttnArgs a{};
+  a.c = w.c;
+  a.q = Qbuf; a.ldq = qd; a.H = sh.q_head_count; a.M = M;
+  a.window = kv4_window;
+  a.scale = 1.0f / sqrtf((float)cfg.head_dim);
+  a.mask = mask; a.ldmask = 0;
+  a.out_c = Abuf; a.out_s = Abuf + (size_t)M * qd;
+  a.err = ctx->d_err;
+  if (decode) {
+    a.slot = d_seq; a.pos = d_pos;
+    return launch_kv4_decode(ctx, a);
+  }
+  a.slot0 = prompt_slot; a.pos0 = prompt_pos;
+  return launch_kv4_prefill(ctx, a);
+}
+
 extern "C" int shd_model_reset(shd_model* m) {
   if (!m) return SHD_ERR_ARG;
   std::fill(m->len.begin(), m->len.end(), 0);
@@ -477,8 +565,13 @@ int shd_model::enqueue_layers(int M, const int* d_pos, const int* d_seq, int var
     g.rope_cos = rope_cos; g.rope_sin = rope_sin; g.rope_max_seq = cfg.max_seq;
     g.pos = d_pos; g.seq = d_seq;
     g.Q = Qbuf; g.ldq = qd;
-    g.Kcache = kcache + (size_t)l * kv_layer; g.Vcache = vcache + (size_t)l * kv_layer;
-    g.kv_seq_stride = (int64_t)c.max_seq * kvd;
+    if (kv4.capacity) {  // shares of the rows, which kv4_attention quantises into the cache
+      g.ldy = qd + 2 * kvd;
+      g.Yc = kv4_rows; g.Ys = kv4_rows + (size_t)M * g.ldy;
+    } else {
+      g.Kcache = kcache + (size_t)l * kv_layer; g.Vcache = vcache + (size_t)l * kv_layer;
+      g.kv_seq_stride = (int64_t)c.max_seq * kvd;
+    }
     g.trace = trace_slot(0);
     if ((rc = prof_mark(0, Lw.qkv, true))) return rc;
     if ((rc = op_gemv(Lw.qkv, M, EPI_QKV, g, fused))) return rc;
@@ -499,9 +592,11 @@ int shd_model::enqueue_layers(int M, const int* d_pos, const int* d_seq, int var
       at.n_groups = n_groups8;
       at.group_cap = 8;
     }
-    at.trace = trace_slot(5);
+    if (!kv4.capacity) at.trace = trace_slot(5);
     if ((rc = prof_mark(5, nullptr, true))) return rc;
-    if (!decode && M >= kFlashRows && flash_prefill_supported(at, M))
+    if (kv4.capacity)
+      rc = kv4_attention(l, M, d_pos, d_seq, at.mask, decode);
+    else if (!decode && M >= kFlashRows && flash_prefill_supported(at, M))
       rc = launch_flash_prefill(ctx, at, M);  // a prompt block: consecutive positions of one slot
     else
       rc = launch_attention(ctx, at, M);
@@ -593,6 +688,7 @@ int shd_model::enqueue_head_rows(int M, int cur, int variant, float* logits) {
 
 int shd_model::check_ready() {
   SHD_REQUIRE(ctx, embed && lm_head, "model: embedding and head must be set");
+  SHD_REQUIRE(ctx, kcache || kv4.capacity, "model: no key/value cache");
   for (auto& L : layers) SHD_REQUIRE(ctx, L.qkv && L.o && L.gateup && L.down, "model: a layer has no weights");
   return SHD_OK;
 }
@@ -640,6 +736,8 @@ int shd_model::prefill_impl(int slot, int n, const int32_t* tokens_host, const f
       ea.Dc = Dbuf; ea.Ds = Dbuf + (size_t)M * h; ea.amax = amax; ea.err = ctx->d_err;
       if ((rc = launch_embed(ctx, ea, M))) break;
     }
+    prompt_slot = slot;
+    prompt_pos = len[slot] + p0;
     if ((rc = enqueue_layers(M, p_pos, p_seq, cfg.variant_prefill, cur, false))) break;
     if (p0 + M == n) {
       if ((rc = enqueue_head(M, M - 1, cur, cfg.variant_prefill, logits_c_host != nullptr, 0))) break;
@@ -732,6 +830,29 @@ extern "C" int shd_model_read_kv(shd_model* m, int slot, int pos0, int n, float*
               "shd_model_read_kv: positions beyond the slot's length");
   SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
   const size_t kvd = (size_t)m->kvd, row = kvd * 4;
+  if (m->kv4.capacity) {
+    const Kv4View& v = m->kv4;
+    SHD_REQUIRE(ctx, m->len[slot] <= v.capacity || pos0 >= m->len[slot] - (v.capacity - v.sinks) || pos0 + n <= v.sinks,
+                "shd_model_read_kv: positions that the cache no longer holds");
+    // the context's launches go to the model's stream meanwhile
+    struct Scope {
+      shd_model* m;
+      explicit Scope(shd_model* x) : m(x) { m->use_stream(); }
+      ~Scope() { m->restore_stream(); }
+    } scope(m);
+    for (int l = 0; l < m->cfg.n_layers; ++l)
+      for (int p = 0; p < n; p += kPrefillRows) {
+        const int rows = std::min(kPrefillRows, n - p);
+        float *k = m->kv4_rows, *w = k + (size_t)rows * kvd;
+        const int rc = launch_kv4_read(ctx, m->kv4_layer(l), slot, pos0 + p, rows, k, w);
+        if (rc) return rc;
+        const size_t to = ((size_t)l * n + p) * kvd;
+        SHD_CHECK_CUDA(ctx, cudaMemcpyAsync(k_host + to, k, rows * row, cudaMemcpyDeviceToHost, m->stream));
+        SHD_CHECK_CUDA(ctx, cudaMemcpyAsync(v_host + to, w, rows * row, cudaMemcpyDeviceToHost, m->stream));
+      }
+    SHD_CHECK_CUDA(ctx, cudaStreamSynchronize(m->stream));
+    return SHD_OK;
+  }
   const size_t layer = (size_t)m->cfg.max_batch * m->cfg.max_seq * kvd;
   for (int l = 0; l < m->cfg.n_layers; ++l) {
     const size_t src = (size_t)l * layer + ((size_t)slot * m->cfg.max_seq + pos0) * kvd;

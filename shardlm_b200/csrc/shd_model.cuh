@@ -6,6 +6,7 @@
 #include "shd_gemv.cuh"
 #include "shd_nonlinear.cuh"
 #include "shd_planes.cuh"
+#include "shd_kv4.cuh"
 
 struct LayerW {
   shd_weight* qkv = nullptr;     // fused q|k|v, SHD_ROWS_QKV
@@ -35,7 +36,14 @@ struct shd_model {
   float *Dbuf = nullptr, *Xbuf = nullptr, *Qbuf = nullptr, *Abuf = nullptr, *ACTbuf = nullptr;
   float *LOGbuf = nullptr, *LOGfull = nullptr;
   float* gather_buf = nullptr;  // TP logit all-gather staging
-  float *kcache = nullptr, *vcache = nullptr;  // [L][slots][T][kvd]
+  float *kcache = nullptr, *vcache = nullptr;  // [L][slots][T][kvd]; null once the cache is in 4 bits
+  // 4-bit cache (shd_model_set_kv4): a layer's part follows the last one's
+  shd::Kv4View kv4{};  // of layer 0; capacity 0: the cache is f32
+  int kv4_window = 0;
+  float* kv4_rows = nullptr;             // [2][rows][qd + 2 kvd] shares of q, k, v (with RoPE)
+  int prompt_slot = 0, prompt_pos = 0;   // of the block that enqueue_layers works on (not decode)
+  shd::Kv4View kv4_layer(int l) const;
+  int kv4_attention(int l, int M, const int* d_pos, const int* d_seq, const float* mask, bool decode);
   int *tokens = nullptr, *pos = nullptr, *seq = nullptr;
   int *p_tokens = nullptr, *p_pos = nullptr, *p_seq = nullptr;
   int4* attn_groups_dev = nullptr;  // attention head groups (kv head, first q head, count), <= 4 q heads

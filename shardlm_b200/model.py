@@ -174,6 +174,12 @@ class SecureModel:
         m = masks.float().contiguous()
         check(lib().shd_model_set_masks(self.handle, ptr(m), m.shape[-1]), self.ctx.ptr)
 
+    def set_kv4(self, capacity: int | None = None, window: int = 0, sinks: int = 0) -> None:
+        """Hold the key/value cache in 4 bits: `capacity` rows a slot (default max_seq), attention over the last
+        `window` positions (0: all) and the first `sinks`. A capacity below max_seq is used as a ring."""
+        check(lib().shd_model_set_kv4(self.handle, self.max_seq if capacity is None else capacity, window, sinks),
+              self.ctx.ptr)
+
     def reset(self) -> None:
         check(lib().shd_model_reset(self.handle), self.ctx.ptr)
 
