@@ -66,9 +66,8 @@ struct PromptShape {
   static constexpr uint32_t ROWBUF = 2 * kPKV * 4;
   static constexpr uint32_t OF32 = ROW + 8 * ROWBUF;           // [8][2][4], of 32 rows: 2^(key e), e, 2^-e, seen by every query
   static constexpr uint32_t RED = OF32 + 8 * 2 * 16;                   // [3][2 halves][128]: maxima of even and odd steps, sums
-  static constexpr uint32_t QEXP = RED + 6 * kPRows * 4;       // [128] exponents that the queries are scaled by
-  static constexpr uint32_t QSUM = QEXP + kPRows * 4;          // [128][4] sums of their groups
-  static constexpr uint32_t BAR = QSUM + kPRows * 16;
+  static constexpr uint32_t RFAC = RED + 6 * kPRows * 4;       // [128] queries' scale
+  static constexpr uint32_t BAR = RFAC + kPRows * 4;
   static constexpr uint32_t PRE = BAR + 256;                   // [kPTiles] cost of the tiles before
   static constexpr size_t SMEM = PRE + kPTiles * 4 + 1024;     // + alignment slack
   static constexpr int PART = HD + 4;                          // of a row: reference, sum, 2 unused, weighted values
@@ -331,8 +330,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_row = tbase + ((uint32_t)((warp & 3) * 32) << 16);
     float* red = reinterpret_cast<float*>(smem + SH::RED);
-    int* qexp = reinterpret_cast<int*>(smem + SH::QEXP);
-    float* qsum = reinterpret_cast<float*>(smem + SH::QSUM);
+    float* rfac = reinterpret_cast<float*>(smem + SH::RFAC);
     int it = 0;
     bool ok = true;
     Segment sg;
@@ -359,78 +357,70 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           tmem_wait_st();
           named_bar_sync(1, 256);
         };
-        // four rows' loads at a time; the low terms' pass takes the rows from L2 again (kept in registers, they
-        // made this straight-line code that is fetched anew for every item: 15 k clocks against 9 k)
-#pragma unroll 1
-        for (int x = 0; x < 2 * N; x += 4) {
-          const bool low = x >= N;
-          if (x == N) high_terms();
-          const int y1 = y0 + (low ? x - N : x) * RPW;
-          float4 v[4];
+        uint2 low[N];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = r0 + y1 + i * RPW, mm = group_of(r);
+        for (int i0 = 0; i0 < N; i0 += 8) {
+          float4 v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = r0 + y0 + (i0 + i) * RPW;
             v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows) v[i] = *reinterpret_cast<const float4*>(a.q + (size_t)mm * a.ldq + (size_t)(sg.head * G + r - mm * G) * HD + 4 * ql);
+            if (r < rows)
+              v[i] = *reinterpret_cast<const float4*>(a.q + (size_t)group_of(r) * a.ldq + (size_t)(sg.head * G + r - group_of(r) * G) * HD + 4 * ql);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int y = y1 + i * RPW;
-            int k;
-            if (!low) {
-              const float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
-              int e = ceil_exp2(top);
-              if constexpr (LPR == 32) {
-                e = __reduce_max_sync(0xffffffffu, e);
-              } else {
+          for (int i = 0; i < 8; ++i) {
+            const int y = y0 + (i0 + i) * RPW;
+            float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
+            float qs = __fadd_rn(__fadd_rn(v[i].x, v[i].y), __fadd_rn(v[i].z, v[i].w));
 #pragma unroll
-                for (int o = 1; o < LPR; o <<= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
-              }
-              float qs = __fadd_rn(__fadd_rn(v[i].x, v[i].y), __fadd_rn(v[i].z, v[i].w));
+            for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
-              for (int o = 1; o < 8; o <<= 1) qs = __fadd_rn(qs, __shfl_xor_sync(0xffffffffu, qs, o));
-              k = max(min(7 - e, 60), -60);  // 2^-k times a power of two of the keys stays normal
-              if (ql % 8 == 0) qsum[4 * y + ql / 8] = qs;
-              if (ql == 0) qexp[y] = k;
-            } else {
-              k = qexp[y];
-            }
+            for (int o = 1; o < 8; o <<= 1) qs = __fadd_rn(qs, __shfl_xor_sync(0xffffffffu, qs, o));
+            const int k = max(min(7 - ceil_exp2(top), 60), -60);  // 2^-k times a power of two of the keys stays normal
             const float up = pow2i(k);
             // of 8 channels the even lane makes pairs (0, 4), (1, 5), the odd one (2, 6), (3, 7)
             const bool odd = lane & 1;
             const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[i].x : v[i].z, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v[i].y : v[i].w, 1);
-            uint2 hi, lo;
-            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, lo.x);
-            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, lo.y);
-            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = low ? lo : hi;
-          }
-        }
-        if (half == 0) {  // 7.5 x and 1 x the groups' sums of this thread's row
-          const float up = pow2i(qexp[row]);
-          uint32_t h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};
+            uint2 hi;
+            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, low[i0 + i].x);
+            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, low[i0 + i].y);
+            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = hi;
+            float q4[NG];
 #pragma unroll
-          for (int g = 0; g < NG; g += 2) {
-            const float s0 = qsum[4 * row + g] * up, s1 = qsum[4 * row + g + 1] * up;
-            split_f16(s0 * 7.5f, s1 * 7.5f, h[g / 2], l[g / 2]);
-            split_f16(s0, s1, h[NG / 2 + g / 2], l[NG / 2 + g / 2]);
+            for (int g = 0; g < NG; ++g) q4[g] = __shfl_sync(0xffffffffu, qs, (lane & ~(LPR - 1)) + 8 * g) * up;
+            if (ql == 0) {
+              uint32_t h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};  // 7.5 x and 1 x the groups' sums
+#pragma unroll
+              for (int g = 0; g < NG; g += 2) {
+                split_f16(q4[g] * 7.5f, q4[g + 1] * 7.5f, h[g / 2], l[g / 2]);
+                split_f16(q4[g], q4[g + 1], h[NG / 2 + g / 2], l[NG / 2 + g / 2]);
+              }
+              *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(y, 0)) = make_uint4(h[0], h[1], h[2], h[3]);
+              *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(y, 1)) = make_uint4(l[0], l[1], l[2], l[3]);
+              rfac[y] = a.scale * 1.44269504088896341f * pow2i(-k);
+            }
           }
-          *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(row, 0)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(row, 1)) = make_uint4(l[0], l[1], l[2], l[3]);
         }
+        high_terms();
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y0 + i * RPW, (4 * ql) & 63)) = low[i];
       }
       tc_fence_before();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar + B_QFULL);
+      named_bar_sync(1, 256);  // rfac
 
       const bool live = r0 + row < rows;
       const int p = a.pos0 + (live ? group_of(r0 + row) : a.M - 1);
-      const float rowf = a.scale * 1.44269504088896341f * pow2i(-qexp[row]);
+      const float rowf = rfac[row];
       float ref = kKv4Never, l = 0.0f;
       bool summed = false;  // the second accumulator holds something
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
         const int b = it & 1;
-        ok = ok && wait(B_SFULL + b, (it >> 1) & 1);
+        ok = ok && wait(B_EFULL + (it & 3), (it >> 2) & 1) && wait(B_SFULL + b, (it >> 1) & 1);
         tc_fence_after();
         const int* rp = reinterpret_cast<const int*>(smem + SH::ROW + (it & 7) * SH::ROWBUF) + 32 * half;
         const float4 of32 = *reinterpret_cast<const float4*>(smem + SH::OF32 + ((it & 7) * 2 + half) * 16);
@@ -820,8 +810,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     bool ok = true;
     auto scores = [&](int i) -> bool {
       const int b = __shfl_sync(0xffffffffu, i & 1, 0);
-      // the softmax needs what the value rows' prelude writes with these scores: one wait less for it
-      if (!wait(B_KFULL + b, (i >> 1) & 1) || !wait(B_EFULL + (i & 3), (i >> 2) & 1)) return false;
+      if (!wait(B_KFULL + b, (i >> 1) & 1)) return false;
       tc_fence_after();
       if (elect_one()) {
         const uint32_t d = tb + kColS + b * kPKV;
