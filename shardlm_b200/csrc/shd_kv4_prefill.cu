@@ -43,6 +43,10 @@ constexpr int kPRows = 128;    // (position, head) pairs of a tile
 constexpr int kPKV = 64;       // cache rows of a step
 constexpr int kPThreads = 576;
 constexpr int kPTiles = 2048;  // tiles a launch (their step counts are in shared memory)
+// steps of rows on their way as stored: three, since a step's values are unpacked only when the product
+// before the last has let go of their buffer, and the keys of the step after next must not wait for that
+// (512 positions after 8191, 40 heads, 8 kv heads: 296 us, with two 302; shorter items the same)
+constexpr int kPRaw = 3;
 constexpr int kPItem = 8;      // cost of an item's queries and results, in steps
 constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
 constexpr float kRoom = 8.0f, kHead = 6.0f;  // weights are 2^(score' - ref + 6), score' - ref <= 8
@@ -60,9 +64,9 @@ struct PromptShape {
   static constexpr uint32_t KXBUF = kPKV * 32;
   static constexpr uint32_t VX = KX + 2 * KXBUF;               // [2 buffers][64 rows / 8][16 columns][16 B]: value middles
   static constexpr uint32_t VXBUF = kPKV * 32;
-  static constexpr uint32_t RAW = VX + 2 * VXBUF;              // [2 buffers][keys, values] codes, then parameters, as stored
+  static constexpr uint32_t RAW = VX + 2 * VXBUF;              // [kPRaw][keys, values] codes, then parameters, as stored
   static constexpr uint32_t RAWC = kPKV * HD / 2, RAWP = kPKV * 4 * NG, RAWBUF = 2 * (RAWC + RAWP);
-  static constexpr uint32_t ROW = RAW + 2 * RAWBUF;            // [8][2][64]: a row's position, out of sight from
+  static constexpr uint32_t ROW = RAW + kPRaw * RAWBUF;        // [8][2][64]: a row's position, out of sight from
   static constexpr uint32_t ROWBUF = 2 * kPKV * 4;
   static constexpr uint32_t OF32 = ROW + 8 * ROWBUF;           // [8][2][4], of 32 rows: 2^(key e), e, 2^-e, seen by every query
   static constexpr uint32_t RED = OF32 + 8 * 2 * 16;                   // [3][2 halves][128]: maxima of even and odd steps, sums
@@ -77,7 +81,7 @@ struct PromptShape {
 // Tensor memory columns. Of each 16 columns of scores, 8 take the weights' high terms and 8 the low ones.
 constexpr uint32_t kColS = 0, kColO = 128, kColSum = 272, kColQ = 416, kCols = 512;
 
-enum Bar { B_QFULL = 0, B_KFULL = 1, B_KFREE = 3, B_VFULL = 5, B_VFREE = 7, B_SFULL = 9, B_PFULL = 11, B_PDONE = 13, B_EFULL = 15, B_RFULL = 19, B_RFREE = 21, B_END = 23 };
+enum Bar { B_QFULL = 0, B_KFULL = 1, B_KFREE = 3, B_VFULL = 5, B_VFREE = 7, B_SFULL = 9, B_PFULL = 11, B_PDONE = 13, B_EFULL = 15, B_RFULL = 19, B_RFREE = 19 + kPRaw, B_END = 19 + 2 * kPRaw };
 
 // D f32, A and B f16, both K-major
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int m, int n) {
@@ -279,7 +283,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
   if (tid == 0) {
     abort_word = 0;
     for (int i = 0; i <= B_END; ++i) {
-      const bool eight = i == B_QFULL || i == B_PFULL || i == B_PFULL + 1 || i == B_RFREE || i == B_RFREE + 1;
+      const bool eight = i == B_QFULL || i == B_PFULL || i == B_PFULL + 1 || (i >= B_RFREE && i < B_RFREE + kPRaw);
       const bool four = i == B_KFULL || i == B_KFULL + 1 || i == B_VFULL || i == B_VFULL + 1 || (i >= B_EFULL && i < B_EFULL + 4);
       mbar_init(bar + i, eight ? 8 : four ? 4 : 1);
     }
@@ -639,11 +643,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     for (int64_t t = t_begin; ok && next_segment(sg, pre, pa.tiles, sum, c.heads, t, t_end); t = sg.next) {
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
         const int b = it & 1;
-        const uint8_t* raw = smem + SH::RAW + b * SH::RAWBUF + (vals ? SH::RAWC : 0);
-        const uint8_t* rawp = smem + SH::RAW + b * SH::RAWBUF + 2 * SH::RAWC + (vals ? SH::RAWP : 0);
+        const int st = it % kPRaw;
+        const uint8_t* raw = smem + SH::RAW + st * SH::RAWBUF + (vals ? SH::RAWC : 0);
+        const uint8_t* rawp = smem + SH::RAW + st * SH::RAWBUF + 2 * SH::RAWC + (vals ? SH::RAWP : 0);
         const int* rp = reinterpret_cast<const int*>(smem + SH::ROW + (it & 7) * SH::ROWBUF);
         float* of32 = reinterpret_cast<float*>(smem + SH::OF32 + ((it & 7) * 2 + (warp & 1)) * 16);
-        if (!(ok = wait(B_RFULL + b, (it >> 1) & 1))) break;
+        if (!(ok = wait(B_RFULL + st, (it / kPRaw) & 1))) break;
         uint32_t w[NG];
         if constexpr (NG == 4) {
           const uint4 v = *reinterpret_cast<const uint4*>(rawp + r * 16);
@@ -731,7 +736,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(bar + (vals ? B_VFULL : B_KFULL) + b);
-          mbar_arrive(bar + B_RFREE + b);
+          mbar_arrive(bar + B_RFREE + st);
         }
       }
     }
@@ -759,8 +764,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         }
       }
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
-        const int b = it & 1;
-        if (it >= 2 && !(ok = wait(B_RFREE + b, ((it - 2) >> 1) & 1))) break;
+        const int st = it % kPRaw;
+        if (it >= kPRaw && !(ok = wait(B_RFREE + st, (it / kPRaw - 1) & 1))) break;
         const int x0 = j * (kPKV / kKv4Chunk), chunks = min(kPKV / kKv4Chunk, sp.total - x0);
         int* rp = reinterpret_cast<int*>(smem + SH::ROW + (it & 7) * SH::ROWBUF);
 #pragma unroll
@@ -783,23 +788,23 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         }
         constexpr uint32_t CODE = kKv4Chunk * HD / 2, PAR = kKv4Chunk * 4 * NG;
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(bar + B_RFULL + b, chunks * 2 * (CODE + PAR));
+        if (lane == 0) mbar_arrive_expect_tx(bar + B_RFULL + st, chunks * 2 * (CODE + PAR));
         __syncwarp();
         if (lane < 16 && (lane & 3) < chunks) {
           const size_t row0 = base + (size_t)kv4_span_chunk(sp, x0 + (lane & 3)) * kKv4Chunk;
           const int kind = lane >> 2;  // key codes, value codes, key and value parameters
-          uint8_t* raw = smem + SH::RAW + b * SH::RAWBUF;
+          uint8_t* raw = smem + SH::RAW + st * SH::RAWBUF;
           if (kind < 2)
-            bulk_copy(raw + kind * SH::RAWC + (lane & 3) * CODE, (kind ? c.vc : c.kc) + row0 * (HD / 2), CODE, bar + B_RFULL + b);
+            bulk_copy(raw + kind * SH::RAWC + (lane & 3) * CODE, (kind ? c.vc : c.kc) + row0 * (HD / 2), CODE, bar + B_RFULL + st);
           else
             bulk_copy(raw + 2 * SH::RAWC + (kind - 2) * SH::RAWP + (lane & 3) * PAR,
-                      reinterpret_cast<const uint8_t*>(kind == 3 ? c.vp : c.kp) + row0 * (4 * NG), PAR, bar + B_RFULL + b);
+                      reinterpret_cast<const uint8_t*>(kind == 3 ? c.vp : c.kp) + row0 * (4 * NG), PAR, bar + B_RFULL + st);
         }
       }
     }
     // no copy is in flight when the block ends
-    for (int i = max(it - 2, 0); i < it; ++i)
-      if (lane == 0 && !mbar_wait_bounded(bar + B_RFULL + (i & 1), (i >> 1) & 1)) atomicOr(a.err, SHD_DEVERR_TIMEOUT_DRAIN);
+    for (int i = max(it - kPRaw, 0); i < it; ++i)
+      if (lane == 0 && !mbar_wait_bounded(bar + B_RFULL + i % kPRaw, (i / kPRaw) & 1)) atomicOr(a.err, SHD_DEVERR_TIMEOUT_DRAIN);
   } else {
     // ---- MMAs: the whole warp walks, one elected thread issues --------------------------------------
     // Operands that the compiler knows to be the same in the warp (by way of the shuffles) keep an issue
