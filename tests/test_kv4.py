@@ -322,6 +322,51 @@ def test_decode_many_sequences(ctx):
 
 
 @pytest.mark.gpu
+def test_decode_rows_of_several_launches(ctx):
+    """More rows than a launch takes, some of them empty, several on one sequence, each with its mask."""
+    rng = np.random.default_rng(12)
+    n, slots_n, heads, heads_q, d = 1100, 40, 1, 3, 64
+    lengths = [1 + (i * 29) % 48 for i in range(slots_n)]
+    b = Built(ctx, rng, slots_n, heads, 48, d, 2, lengths)
+    slots = [int(x) for x in rng.integers(0, slots_n, n)]
+    pos = [-1 if m % 97 == 5 else int(rng.integers(0, lengths[s])) for m, s in enumerate(slots)]
+    q = rng.standard_normal((n, heads_q * d)).astype(np.float32)
+    mask = rng.standard_normal((n, heads_q * d)).astype(np.float32)
+    got = b.cache.attend(dev(q), slot=dev(np.array(slots, np.int32)), pos=dev(np.array(pos, np.int32)), window=20, mask=dev(mask))
+    ctx.sync()
+    check_rows(got, b, q, slots, pos, 20, heads_q, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("parts_of", [1, 3])
+def test_decode_long_beside_short(ctx, parts_of):
+    """Items cut into many parts, joined in groups, next to items of one chunk."""
+    rng = np.random.default_rng(13 + parts_of)
+    heads, heads_q, d, length = 1, 5, 128, 12007
+    lengths = [length - 1000 * i for i in range(parts_of)] + [1, 17, 2]
+    b = Built(ctx, rng, len(lengths), heads, 12016, d, 0, lengths)
+    slots, pos = list(range(len(lengths))), [n - 1 for n in lengths]
+    q = rng.standard_normal((len(lengths), heads_q * d)).astype(np.float32)
+    got = b.cache.attend(dev(q), slot=dev(np.array(slots, np.int32)), pos=dev(np.array(pos, np.int32)))
+    ctx.sync()
+    check_rows(got, b, q, slots, pos, 0, heads_q)
+
+
+@pytest.mark.gpu
+def test_prompt_of_several_launches(ctx):
+    """More (position, head) tiles than a launch takes: the second launch's positions, masks and outputs."""
+    rng = np.random.default_rng(14)
+    heads, heads_q, d, n = 1, 64, 64, 4200
+    b = Built(ctx, rng, 1, heads, 4208, d, 3, [n])
+    q = rng.standard_normal((n, heads_q * d)).astype(np.float32)
+    mask = rng.standard_normal((n, heads_q * d)).astype(np.float32)
+    got = b.cache.attend_prompt(dev(q), slot=0, pos0=0, window=90, mask=dev(mask))
+    ctx.sync()
+    some = [0, 1, 2047, 4094, 4095, 4096, 4097, n - 1]
+    check_rows((got[0][some], got[1][some]), b, q[some], [0] * len(some), some, 90, heads_q, mask[some])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("prompt", [False, True])
 @pytest.mark.parametrize("k_gain,q_gain,v_gain", [
     (1.0, 0.0, None),                                  # equal weights
