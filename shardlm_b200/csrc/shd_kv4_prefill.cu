@@ -69,9 +69,8 @@ struct PromptShape {
   static constexpr uint32_t ROW = RAW + kPRaw * RAWBUF;        // [8][2][64]: a row's position, out of sight from
   static constexpr uint32_t ROWBUF = 2 * kPKV * 4;
   static constexpr uint32_t OF32 = ROW + 8 * ROWBUF;           // [8][2][4], of 32 rows: 2^(key e), e, 2^-e, seen by every query
-  static constexpr uint32_t RED = OF32 + 8 * 2 * 16;                   // [3][2 halves][128]: maxima of even and odd steps, sums
-  static constexpr uint32_t RFAC = RED + 6 * kPRows * 4;       // [128] queries' scale
-  static constexpr uint32_t BAR = RFAC + kPRows * 4;
+  static constexpr uint32_t RED = OF32 + 8 * 2 * 16;                   // [3][2 halves][128]: maxima of even and odd steps; the query's, then the sums
+  static constexpr uint32_t BAR = RED + 6 * kPRows * 4;
   static constexpr uint32_t PRE = BAR + 256;                   // [kPTiles] cost of the tiles before
   static constexpr size_t SMEM = PRE + kPTiles * 4 + 1024;     // + alignment slack
   static constexpr int PART = HD + 4;                          // of a row: reference, sum, 2 unused, weighted values
@@ -334,92 +333,77 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
     const int half = warp >> 2, row = (warp & 3) * 32 + lane;
     const uint32_t t_row = tbase + ((uint32_t)((warp & 3) * 32) << 16);
     float* red = reinterpret_cast<float*>(smem + SH::RED);
-    float* rfac = reinterpret_cast<float*>(smem + SH::RFAC);
     int it = 0;
     bool ok = true;
     Segment sg;
     for (int64_t t = t_begin; next_segment(sg, pre, pa.tiles, sum, c.heads, t, t_end); t = sg.next) {
       const int r0 = sg.tile * kPRows, rows = a.M * G;  // at most kPTiles * kPRows
-      // queries as two terms of q * 2^k, |q| 2^k < 2^7, channels in the order of the key words: a warp
-      // takes 16 rows, HD / 4 lanes a row; the high terms go to tensor memory by way of the low terms' place
+      // queries as two terms of q * 2^k, |q| 2^k < 2^7, channels in the order of the key words; a thread takes
+      // its row's half, so that nothing but the exponent crosses threads
+      const bool live = r0 + row < rows;
+      float rowf;
       {
-        constexpr int LPR = HD / 4, RPW = 32 / LPR, N = 16 / RPW;
-        const int ql = lane % LPR, y0 = warp * 16 + lane / LPR;
-        auto high_terms = [&]() {
-          named_bar_sync(1, 256);
+        constexpr int N = HD / 8;
+        const int mm = live ? group_of(r0 + row) : 0;
+        const float* src = a.q + (size_t)mm * a.ldq + (size_t)(sg.head * G + (live ? r0 + row - mm * G : 0)) * HD + half * (HD / 2);
+        float4 v[N];
+        float top = 0.0f, sums[HD / 64];
 #pragma unroll
-          for (int x = 0; x < HD / 64; ++x) {
-            const int ch = half * (HD / 2) + 32 * x;  // 32 channels: 16 columns
-            uint32_t h[16];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint4 v = *reinterpret_cast<const uint4*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(row, (ch & 63) + 8 * y));
-              h[4 * y] = v.x; h[4 * y + 1] = v.y; h[4 * y + 2] = v.z; h[4 * y + 3] = v.w;
-            }
-            tmem_st16(t_row + kColQ + ch / 2, h);
-          }
-          tmem_wait_st();
-          named_bar_sync(1, 256);
-        };
-        uint2 low[N];
-#pragma unroll
-        for (int i0 = 0; i0 < N; i0 += 8) {
-          float4 v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = r0 + y0 + (i0 + i) * RPW;
-            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < rows)
-              v[i] = *reinterpret_cast<const float4*>(a.q + (size_t)group_of(r) * a.ldq + (size_t)(sg.head * G + r - group_of(r) * G) * HD + 4 * ql);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int y = y0 + (i0 + i) * RPW;
-            float top = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w)));
-            float qs = __fadd_rn(__fadd_rn(v[i].x, v[i].y), __fadd_rn(v[i].z, v[i].w));
-#pragma unroll
-            for (int o = 1; o < LPR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) qs = __fadd_rn(qs, __shfl_xor_sync(0xffffffffu, qs, o));
-            const int k = max(min(7 - ceil_exp2(top), 60), -60);  // 2^-k times a power of two of the keys stays normal
-            const float up = pow2i(k);
-            // of 8 channels the even lane makes pairs (0, 4), (1, 5), the odd one (2, 6), (3, 7)
-            const bool odd = lane & 1;
-            const float s0 = __shfl_xor_sync(0xffffffffu, odd ? v[i].x : v[i].z, 1), s1 = __shfl_xor_sync(0xffffffffu, odd ? v[i].y : v[i].w, 1);
-            uint2 hi;
-            split_f16((odd ? s0 : v[i].x) * up, (odd ? v[i].z : s0) * up, hi.x, low[i0 + i].x);
-            split_f16((odd ? s1 : v[i].y) * up, (odd ? v[i].w : s1) * up, hi.y, low[i0 + i].y);
-            *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y, (4 * ql) & 63)) = hi;
-            float q4[NG];
-#pragma unroll
-            for (int g = 0; g < NG; ++g) q4[g] = __shfl_sync(0xffffffffu, qs, (lane & ~(LPR - 1)) + 8 * g) * up;
-            if (ql == 0) {
-              uint32_t h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};  // 7.5 x and 1 x the groups' sums
-#pragma unroll
-              for (int g = 0; g < NG; g += 2) {
-                split_f16(q4[g] * 7.5f, q4[g + 1] * 7.5f, h[g / 2], l[g / 2]);
-                split_f16(q4[g], q4[g + 1], h[NG / 2 + g / 2], l[NG / 2 + g / 2]);
-              }
-              *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(y, 0)) = make_uint4(h[0], h[1], h[2], h[3]);
-              *reinterpret_cast<uint4*>(smem + SH::QX + plain16_offset(y, 1)) = make_uint4(l[0], l[1], l[2], l[3]);
-              rfac[y] = a.scale * 1.44269504088896341f * pow2i(-k);
-            }
-          }
+        for (int i = 0; i < N; ++i) {
+          v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (live) v[i] = *reinterpret_cast<const float4*>(src + 4 * i);
         }
-        high_terms();
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          *reinterpret_cast<uint2*>(smem + SH::QL + (ql >> 4) * (kPRows * 128) + sw128_offset(y0 + i * RPW, (4 * ql) & 63)) = low[i];
+        for (int g = 0; g < HD / 64; ++g) {
+          float4 t = v[8 * g], y = make_float4(fabsf(t.x), fabsf(t.y), fabsf(t.z), fabsf(t.w));
+#pragma unroll
+          for (int i = 8 * g + 1; i < 8 * g + 8; ++i) {
+            t.x = __fadd_rn(t.x, v[i].x); t.y = __fadd_rn(t.y, v[i].y); t.z = __fadd_rn(t.z, v[i].z); t.w = __fadd_rn(t.w, v[i].w);
+            y.x = fmaxf(y.x, fabsf(v[i].x)); y.y = fmaxf(y.y, fabsf(v[i].y)); y.z = fmaxf(y.z, fabsf(v[i].z)); y.w = fmaxf(y.w, fabsf(v[i].w));
+          }
+          sums[g] = __fadd_rn(__fadd_rn(t.x, t.y), __fadd_rn(t.z, t.w));
+          top = fmaxf(top, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+        }
+        red[(4 + half) * kPRows + row] = top;
+        named_bar_sync(4 + (warp & 3), 64);
+        top = fmaxf(top, red[(4 + (half ^ 1)) * kPRows + row]);
+        const int k = max(min(7 - ceil_exp2(top), 60), -60);  // 2^-k times a power of two of the keys stays normal
+        const float up = pow2i(k);
+        rowf = a.scale * 1.44269504088896341f * pow2i(-k);
+#pragma unroll
+        for (int x = 0; x < HD / 64; ++x) {
+          const int ch = half * (HD / 2) + 32 * x;  // 32 channels: 16 columns
+          uint32_t h[16];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {  // of 8 channels the pairs (0, 4), (1, 5), (2, 6), (3, 7)
+            const float4 f = v[8 * x + 2 * y], g = v[8 * x + 2 * y + 1];
+            uint4 lo;
+            split_f16(f.x * up, g.x * up, h[4 * y], lo.x);
+            split_f16(f.y * up, g.y * up, h[4 * y + 1], lo.y);
+            split_f16(f.z * up, g.z * up, h[4 * y + 2], lo.z);
+            split_f16(f.w * up, g.w * up, h[4 * y + 3], lo.w);
+            *reinterpret_cast<uint4*>(smem + SH::QL + (ch >> 6) * (kPRows * 128) + sw128_offset(row, (ch & 63) + 8 * y)) = lo;
+          }
+          tmem_st16(t_row + kColQ + ch / 2, h);
+          // 7.5 x and 1 x the group's sum, as elements g and NG + g of the high terms' 8 and the low terms'
+          uint32_t hi, lo;
+          split_f16(sums[x] * up * 7.5f, sums[x] * up, hi, lo);
+          uint16_t* to = reinterpret_cast<uint16_t*>(smem + SH::QX + plain16_offset(row, 0)) + ch / 32;
+          to[0] = (uint16_t)hi; to[NG] = (uint16_t)(hi >> 16);
+          to[64] = (uint16_t)lo; to[64 + NG] = (uint16_t)(lo >> 16);
+        }
+        if (HD == 64 && half == 0) {
+          *reinterpret_cast<uint2*>(smem + SH::QX + plain16_offset(row, 0) + 8) = make_uint2(0u, 0u);
+          *reinterpret_cast<uint2*>(smem + SH::QX + plain16_offset(row, 1) + 8) = make_uint2(0u, 0u);
+        }
+        tmem_wait_st();
       }
       tc_fence_before();
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar + B_QFULL);
-      named_bar_sync(1, 256);  // rfac
 
-      const bool live = r0 + row < rows;
       const int p = a.pos0 + (live ? group_of(r0 + row) : a.M - 1);
-      const float rowf = rfac[row];
       float ref = kKv4Never, l = 0.0f;
       bool summed = false;  // the second accumulator holds something
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
