@@ -72,9 +72,13 @@ struct PromptShape {
   static constexpr uint32_t RED = OF32 + 8 * 2 * 16;                   // [3][2 halves][128]: maxima of even and odd steps; the query's, then the sums
   static constexpr uint32_t BAR = RED + 6 * kPRows * 4;
   static constexpr uint32_t PRE = BAR + 256;                   // [kPTiles] cost of the tiles before
-  static constexpr size_t SMEM = PRE + kPTiles * 4 + 1024;     // + alignment slack
+  // [8 warps][32 rows][32 channels] of queries on their way to their threads: the low terms' place, where it is wide enough
+  static constexpr uint32_t TURN = HD == 128 ? QL : PRE + kPTiles * 4, TURNBUF = 32 * 32 * 4;
+  static constexpr size_t SMEM = PRE + kPTiles * 4 + (HD == 128 ? 0 : 8 * TURNBUF) + 1024;  // + alignment slack
+  static_assert(TURN != QL || 8 * TURNBUF <= QX - QL, "turned queries run over");
   static constexpr int PART = HD + 4;                          // of a row: reference, sum, 2 unused, weighted values
   static constexpr int SC = HD / 4;                            // channels of a row staged together on the way out
+  static_assert(8 * 32 * (SC + 4) * 4 <= K - QL, "staged results run over");
 };
 
 // Tensor memory columns. Of each 16 columns of scores, 8 take the weights' high terms and 8 the low ones.
@@ -344,14 +348,29 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       float rowf;
       {
         constexpr int N = HD / 8;
-        const int mm = live ? group_of(r0 + row) : 0;
-        const float* src = a.q + (size_t)mm * a.ldq + (size_t)(sg.head * G + (live ? r0 + row - mm * G : 0)) * HD + half * (HD / 2);
+        // as they lie, 8 lanes a row, and by way of shared memory to their threads
+        float* turn = reinterpret_cast<float*>(smem + SH::TURN + warp * SH::TURNBUF);
         float4 v[N];
         float top = 0.0f, sums[HD / 64];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (live) v[i] = *reinterpret_cast<const float4*>(src + 4 * i);
+        for (int i = 0; i < 8; ++i) {
+          const int r = r0 + (warp & 3) * 32 + 4 * i + lane / 8, mm = group_of(r);
+          const float* src = a.q + (size_t)mm * a.ldq + (size_t)(sg.head * G + r - mm * G) * HD + half * (HD / 2) + 4 * (lane & 7);
+#pragma unroll
+          for (int g = 0; g < HD / 64; ++g) {
+            v[8 * g + i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rows) v[8 * g + i] = *reinterpret_cast<const float4*>(src + 32 * g);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < HD / 64; ++g) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)  // column ^ row: both sides without bank conflicts
+            *reinterpret_cast<float4*>(turn + (4 * i + lane / 8) * 32 + 4 * ((lane & 7) ^ ((4 * i + lane / 8) & 7))) = v[8 * g + i];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[8 * g + i] = *reinterpret_cast<const float4*>(turn + lane * 32 + 4 * (i ^ (lane & 7)));
+          __syncwarp();
         }
 #pragma unroll
         for (int g = 0; g < HD / 64; ++g) {
@@ -365,7 +384,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           top = fmaxf(top, fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
         }
         red[(4 + half) * kPRows + row] = top;
-        named_bar_sync(4 + (warp & 3), 64);
+        named_bar_sync(1, 256);  // also: every warp's queries have left their place
         top = fmaxf(top, red[(4 + (half ^ 1)) * kPRows + row]);
         const int k = max(min(7 - ceil_exp2(top), 60), -60);  // 2^-k times a power of two of the keys stays normal
         const float up = pow2i(k);
@@ -592,23 +611,44 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         // SC / 2 channels of each group from 4 * (first unit)
         const int unit = (col & 63) / 8;
         constexpr int LPR = SC / 4;
+        constexpr int RPI = 32 / LPR, B = 4;
+        const int f = lane % LPR, g = g0 + f / (LPR / 2), ch = 32 * g + 4 * unit + 4 * (f % (LPR / 2));
+        const int y0 = (warp & 3) * 32;
+        if (whole && a.mask) {  // of four rows on their way at a time: one by one, their latency is most of a short item
 #pragma unroll 1
-        for (int i = lane / LPR; i < 32; i += 32 / LPR) {
-          const int f = lane % LPR, g = g0 + f / (LPR / 2), ch = 32 * g + 4 * unit + 4 * (f % (LPR / 2));
-          const int y = (warp & 3) * 32 + i;
-          const int rr = r0 + y;
-          if (rr >= rows) continue;
-          const float4 v = *reinterpret_cast<const float4*>(stage + i * STRIDE + 4 * f);
-          if (whole) {
-            const int mm = group_of(rr);
-            const int in_row = (sg.head * G + rr - mm * G) * HD + ch;
-            const size_t to = (size_t)mm * a.H * HD + in_row;
-            const float4 mk = a.mask ? *reinterpret_cast<const float4*>(a.mask + mm * a.ldmask + in_row) : make_float4(0.f, 0.f, 0.f, 0.f);
-            *reinterpret_cast<float4*>(a.out_c + to) =
-                make_float4(__fsub_rn(v.x, mk.x), __fsub_rn(v.y, mk.y), __fsub_rn(v.z, mk.z), __fsub_rn(v.w, mk.w));
-            *reinterpret_cast<float4*>(a.out_s + to) = mk;
-          } else {
-            *reinterpret_cast<float4*>(parts + (size_t)y * SH::PART + 4 + ch) = v;
+          for (int i0 = lane / LPR; i0 < 32; i0 += B * RPI) {
+            float4 mk[B];
+#pragma unroll
+            for (int x = 0; x < B; ++x) {
+              const int rr = r0 + y0 + i0 + x * RPI, mm = group_of(rr);
+              mk[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (rr < rows) mk[x] = *reinterpret_cast<const float4*>(a.mask + mm * a.ldmask + (sg.head * G + rr - mm * G) * HD + ch);
+            }
+#pragma unroll
+            for (int x = 0; x < B; ++x) {
+              const int i = i0 + x * RPI, rr = r0 + y0 + i, mm = group_of(rr);
+              if (rr >= rows) continue;
+              const float4 v = *reinterpret_cast<const float4*>(stage + i * STRIDE + 4 * f);
+              const size_t to = (size_t)mm * a.H * HD + (sg.head * G + rr - mm * G) * HD + ch;
+              *reinterpret_cast<float4*>(a.out_c + to) =
+                  make_float4(__fsub_rn(v.x, mk[x].x), __fsub_rn(v.y, mk[x].y), __fsub_rn(v.z, mk[x].z), __fsub_rn(v.w, mk[x].w));
+              *reinterpret_cast<float4*>(a.out_s + to) = mk[x];
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int i = lane / LPR; i < 32; i += RPI) {
+            const int rr = r0 + y0 + i;
+            if (rr >= rows) continue;
+            const float4 v = *reinterpret_cast<const float4*>(stage + i * STRIDE + 4 * f);
+            if (whole) {
+              const int mm = group_of(rr);
+              const size_t to = (size_t)mm * a.H * HD + (sg.head * G + rr - mm * G) * HD + ch;
+              *reinterpret_cast<float4*>(a.out_c + to) = v;
+              *reinterpret_cast<float4*>(a.out_s + to) = make_float4(0.f, 0.f, 0.f, 0.f);
+            } else {
+              *reinterpret_cast<float4*>(parts + (size_t)(y0 + i) * SH::PART + 4 + ch) = v;
+            }
           }
         }
         __syncwarp();
