@@ -190,6 +190,7 @@ struct RowParams {
 struct PromptArgs {
   Kv4AttnArgs a;
   float* parts;    // [CTA][2][128][PART]
+  int4* cuts;      // [CTA]: of the item first cut at the CTA's end, tile, head, parts (0: none) and which of the CTA's two parts is its first
   int tiles;       // of a kv head
   int last;        // newest position written
   uint32_t per_group;  // 2^32 / G, rounded up (0 for G = 1): r / G = high word of the product for r < 2^18
@@ -826,6 +827,15 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         }
       }
     }
+    if (lane == 0) {
+      int4 cut = make_int4(0, 0, 0, 0);
+      if (t_end < T && t_begin < t_end) {
+        const Segment at = find_segment(pre, pa.tiles, sum, c.heads, t_end, T);
+        if (at.begin > 0 && (at.item + kPItem) / per == (int64_t)blockIdx.x)
+          cut = make_int4(at.tile, at.head, (int)((at.item + kPItem + at.steps - 1) / per) - (int)blockIdx.x + 1, t_begin >= at.item ? 0 : 1);
+      }
+      pa.cuts[blockIdx.x] = cut;
+    }
     // no copy is in flight when the block ends
     for (int i = max(it - kPRaw, 0); i < it; ++i)
       if (lane == 0 && !mbar_wait_bounded(bar + B_RFULL + i % kPRaw, (i / kPRaw) & 1)) atomicOr(a.err, SHD_DEVERR_TIMEOUT_DRAIN);
@@ -918,36 +928,32 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
 }
 
 // Items that a share boundary cuts, joined in CTA order: block (b, y) takes rows 8 y .. + 7 of the item
-// whose first cut is boundary b + 1; a warp takes a row.
+// whose first cut is the end of CTA b's share; a warp takes a row.
 template <int HD>
-__global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ PromptArgs pa, int ctas) {
+__global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ PromptArgs pa) {
   using SH = PromptShape<HD>;
+  constexpr int CPL = HD / 32;  // channels a lane
   const Kv4AttnArgs& a = pa.a;
-  __shared__ int pre[kPTiles];
-  __shared__ int scratch[32];
   pdl_trigger();
   pdl_wait();
-  const int G = a.H / a.c.heads;
-  const int sum = plan_tiles(a, pa.tiles, G, pre, scratch);
-  const int64_t T = (int64_t)sum * a.c.heads, per = (T + ctas - 1) / ctas, t = (blockIdx.x + 1) * per;
-  if (t >= T) return;
-  const Segment sg = find_segment(pre, pa.tiles, sum, a.c.heads, t, T);
-  // not cut here, or not for the first time
-  if (sg.begin == 0 || (sg.item + kPItem) / per != (int64_t)blockIdx.x) return;
-  const int64_t item = sg.item;
-  const int w0 = (int)blockIdx.x, parts = (int)((item + kPItem + sg.steps - 1) / per) - w0 + 1;
+  const int4 cut = __ldcg(pa.cuts + blockIdx.x);
+  const int parts = cut.z, G = a.H / a.c.heads;
   const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int64_t r = (int64_t)sg.tile * kPRows + row;
-  if (r >= (int64_t)a.M * G) return;
+  const int r = cut.x * kPRows + row, mm = pa.per_group ? (int)__umulhi((uint32_t)r, pa.per_group) : r;
+  if (parts == 0 || mm >= a.M) return;
+  const int in_row = (cut.y * G + r - mm * G) * HD + CPL * lane;
+  const size_t at = (size_t)mm * a.H * HD + in_row;
+  float mk[CPL];
+#pragma unroll
+  for (int i = 0; i < CPL; ++i) mk[i] = a.mask ? a.mask[mm * a.ldmask + in_row + i] : 0.0f;
   const size_t step = (size_t)2 * kPRows * SH::PART;
-  const float* first = pa.parts + ((size_t)w0 * 2 + (w0 * per >= item ? 0 : 1)) * kPRows * SH::PART + (size_t)row * SH::PART;
-  const float* next = pa.parts + (size_t)(w0 + 1) * step + (size_t)row * SH::PART;
+  const float* first = pa.parts + ((size_t)blockIdx.x * 2 + cut.w) * kPRows * SH::PART + (size_t)row * SH::PART;
+  const float* next = pa.parts + (size_t)(blockIdx.x + 1) * step + (size_t)row * SH::PART;
   auto part = [&](int w) { return w == 0 ? first : next + (size_t)(w - 1) * step; };
   float M = -INFINITY, L = 0.0f;
   for (int w = lane; w < parts; w += 32) M = fmaxf(M, __ldcg(part(w)));
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  constexpr int CPL = HD / 32;  // channels a lane
   float y[CPL];
 #pragma unroll
   for (int i = 0; i < CPL; ++i) y[i] = 0.0f;
@@ -969,13 +975,14 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ P
     for (int i = 0; i < CPL; ++i) y[i] = fmaf(v[i], e, y[i]);
   }
   const float D = L == 0.0f ? 1.0f : L;
-  const int in_row = (int)(sg.head * G + r % G) * HD + CPL * lane;
-  const size_t at = (size_t)(r / G) * a.H * HD + in_row;
 #pragma unroll
-  for (int i = 0; i < CPL; ++i) {
-    const float mk = a.mask ? a.mask[(r / G) * a.ldmask + in_row + i] : 0.0f;
-    a.out_c[at + i] = __fsub_rn(__fdiv_rn(y[i], D), mk);
-    a.out_s[at + i] = mk;
+  for (int i = 0; i < CPL; ++i) y[i] = __fsub_rn(__fdiv_rn(y[i], D), mk[i]);
+  if constexpr (CPL == 4) {
+    *reinterpret_cast<float4*>(a.out_c + at) = make_float4(y[0], y[1], y[2], y[3]);
+    *reinterpret_cast<float4*>(a.out_s + at) = make_float4(mk[0], mk[1], mk[2], mk[3]);
+  } else {
+    *reinterpret_cast<float2*>(a.out_c + at) = make_float2(y[0], y[1]);
+    *reinterpret_cast<float2*>(a.out_s + at) = make_float2(mk[0], mk[1]);
   }
 }
 
@@ -989,7 +996,7 @@ int launch_prefill_t(shd_ctx* ctx, const Kv4AttnArgs& a0) {
   }
   const int ctas = ctx->num_sms;
   const size_t need = (size_t)ctas * 2 * kPRows * PromptShape<128>::PART;
-  if (!ctx->d_kv4_parts) SHD_CHECK_CUDA(ctx, cudaMalloc(&ctx->d_kv4_parts, need * 4));
+  if (!ctx->d_kv4_parts) SHD_CHECK_CUDA(ctx, cudaMalloc(&ctx->d_kv4_parts, need * 4 + ctas * sizeof(int4)));
   const int G = a0.H / a0.c.heads;
   // launches of at most kPTiles tiles: whole positions
   const int step = (int)std::min<int64_t>(a0.M, (int64_t)kPTiles * kPRows / G);
@@ -1007,9 +1014,10 @@ int launch_prefill_t(shd_ctx* ctx, const Kv4AttnArgs& a0) {
     pa.last = a0.pos0 + a0.M - 1;
     pa.per_group = G == 1 ? 0u : (uint32_t)(((1ull << 32) + G - 1) / G);
     pa.parts = ctx->d_kv4_parts;
+    pa.cuts = reinterpret_cast<int4*>(ctx->d_kv4_parts + need);
     pa.tiles = (int)(((int64_t)pa.a.M * G + kPRows - 1) / kPRows);
     SHD_CHECK_CUDA(ctx, launch_pdl(kv4_prefill_kernel<HD>, dim3(ctas), dim3(kPThreads), SH::SMEM, ctx->stream, pa));
-    SHD_CHECK_CUDA(ctx, launch_pdl(kv4_join_kernel<HD>, dim3(ctas - 1, kPRows / 8), dim3(256), 0, ctx->stream, pa, ctas));
+    SHD_CHECK_CUDA(ctx, launch_pdl(kv4_join_kernel<HD>, dim3(ctas - 1, kPRows / 8), dim3(256), 0, ctx->stream, pa));
     ctx->launches += 2;
   }
   return SHD_OK;
