@@ -305,7 +305,8 @@ int shd_kv4_attn_decode(shd_ctx* ctx, const shd_kv4_cache* cache, const float* q
                         const int32_t* slot, const int32_t* pos, int M, int window,
                         const float* mask, float* out_c, float* out_s);
 /* The same attention for M consecutive positions pos0 .. pos0 + M - 1 of one slot, all of whose K/V
- * rows are written; past the capacity the ring must hold window + M - 1 positions. */
+ * rows are written; past the capacity the ring must hold window + M - 1 positions. A context's first
+ * call allocates its scratch (20 MB): make one before capturing it in a graph. */
 int shd_kv4_attn_prefill(shd_ctx* ctx, const shd_kv4_cache* cache, const float* q, int ldq, int H,
                          int slot, int pos0, int M, int window, const float* mask, float* out_c,
                          float* out_s);

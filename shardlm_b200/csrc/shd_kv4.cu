@@ -19,7 +19,8 @@ __device__ __forceinline__ void group_params(float lo, float hi, __half& s, __ha
 }
 
 // Four channels a thread, so a group is 8 neighbouring lanes and its least and greatest value three
-// shuffles each.
+// shuffles each. Bound by memory: 4096 rows of 8 heads of 128 with shares and values out, 106 MB, in 19.2 us,
+// 5.5 TB/s (a plain copy measures 6.5). Few rows cost a launch: 333 rows of 2 heads of 64, 2.6 us.
 __global__ void __launch_bounds__(kWriteThreads) kv4_write_kernel(const Kv4WriteArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -100,7 +101,8 @@ __global__ void __launch_bounds__(kWriteThreads) kv4_write_kernel(const Kv4Write
 
 // 8 threads a row (slot, head): thread u reads 2 NG bytes of the keys' codes (words of NG / 2 groups) and
 // unit u of the values, and writes both. A value unit's NG pieces of 4 channels go out 128 bytes at a time;
-// of the keys neighbouring threads exchange halves, so that theirs do too.
+// of the keys neighbouring threads exchange halves, so that theirs do too. Bound by memory: 32768 rows of 8
+// heads of 128, 310 MB, in 48.7 us, 6.4 TB/s.
 template <int NG>
 __global__ void __launch_bounds__(kWriteThreads) kv4_read_kernel(const Kv4View c, int slot, int pos0, uint32_t units,
                                                                  float* k_out, float* v_out) {

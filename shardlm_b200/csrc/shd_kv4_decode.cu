@@ -7,8 +7,9 @@
 // the subnormal c * 2^-24 (its bits under a mask, one instruction for two codes; the nibble above it
 // is c * 2^-20), centred to (c - 7.5) * 2^-9, also exact, by one more: weights add up to 1 over many rows
 // whose values cancel, and sums of codes that are all positive would lose what cancels (measured
-// against 64 bits at 131000 positions: 5e-4 of the result). The other operand is split into two f16 terms (22 bits): the queries, scaled by a power
-// of two of their head, and the weights p_t s_tg, scaled by a running power of two of the scales.
+// against 64 bits at 131000 positions: 5e-4 of the result). The other operand is split into two f16 terms
+// (22 bits): the queries, scaled by a power of two of their head, and the weights p_t s_tg, scaled by a
+// running power of two of the scales.
 // Sums are f32. Rows of the first product's A are the 8 heads' high terms and the 8 heads' low terms;
 // the second takes the two terms one after the other:
 //   S [8 + 8 heads x 8 rows]      += Q [16 x 16 channels] K^T   per group, then scaled by s
@@ -18,12 +19,20 @@
 // read below is free of bank conflicts.
 //
 // Work: an item is (query row, kv head, up to 8 query heads) with its visible 16-row chunks (kv4_spans).
-// When the items are few, each is cut evenly into as many parts as give every CTA at most one; else the
+// When the items are few, each is cut evenly into as many parts as give every CTA at most one (one sequence
+// at 554 positions: 11.4 us where equal shares took 14.7); else the
 // chunks of all items, with kDItem for an item's start and end, are laid end to end and cut into equal
 // shares, whatever the lengths. In a CTA the 8 warps take chunks in turn, each with its own ring
 // of asynchronous copies and its own online softmax, and are combined in warp order. An item that is cut
 // leaves partial results; the CTA that arrives last joins them in CTA order, so results do not depend on
 // timing.
+//
+// Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 42.6 us (2.0 TB/s of cache); 64
+// ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 73.7 us (2.3 TB/s); 8 at 1041 to 1280
+// positions 15.1 us; one at 554 positions 10.3 us. Long ones are bound by integer and conversion
+// instructions: some 215 of the 500 a chunk of 16 rows costs a warp, 395 clocks a chunk of a CTA with two
+// CTAs an SM, where the tensor instructions take 107 clocks an SM. Short ones are bound by the chain of
+// launch, plan, first rows from memory, combine and join, one after the other.
 #include <cmath>
 
 #include "shd_kv4.cuh"
@@ -35,7 +44,9 @@ constexpr int kDWarps = 8;
 constexpr int kDThreads = 32 * kDWarps;
 constexpr int kDStages = 4;       // chunks of a warp's ring
 constexpr int kDRows = 512;       // query rows of one launch (their chunk counts are in shared memory)
-constexpr int kDItem = 18;        // what an item costs a CTA besides its chunks, in chunks
+// what an item costs a CTA besides its chunks, in chunks: at 12, 18 and 24 the windowed batch above takes 82.5,
+// 72.8 and 72.4 us
+constexpr int kDItem = 18;
 constexpr int kDJoin = 12;        // parts that are joined at once, and in groups of how many where there are more
 constexpr int kDGroup = 10;
 constexpr int kDGroupMax = 32;    // (the larger of kDJoin, kDGroup and the groups of all CTAs)
