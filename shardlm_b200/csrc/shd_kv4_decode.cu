@@ -29,10 +29,11 @@
 //
 // Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 42.6 us (2.0 TB/s of cache); 64
 // ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 73.7 us (2.3 TB/s); 8 at 1041 to 1280
-// positions 15.1 us; one at 554 positions 10.3 us. Long ones are bound by integer and conversion
-// instructions: some 215 of the 500 a chunk of 16 rows costs a warp, 395 clocks a chunk of a CTA with two
-// CTAs an SM, where the tensor instructions take 107 clocks an SM. Short ones are bound by the chain of
-// launch, plan, first rows from memory, combine and join, one after the other.
+// positions 15.1 us; one at 554 positions 10.3 us. No pipe is full in the long ones (of the windowed batch's
+// time on the SMs the integer pipe is busy 38 %, tensor 23 %, issue slots 56 %, memory 27 %): a chunk of 16
+// rows is some 500 instructions of a warp in dependent steps, and the registers hold four warps a scheduler.
+// It takes 198 clocks of an SM, where its 215 integer and conversion instructions alone take 107. Short ones
+// are bound by the chain of launch, plan, first rows from memory, combine and join, one after the other.
 #include <cmath>
 
 #include "shd_kv4.cuh"
