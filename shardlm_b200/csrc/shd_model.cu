@@ -389,11 +389,24 @@ extern "C" int shd_model_set_masks(shd_model* m, const float* masks, int64_t str
   SHD_REQUIRE(ctx, stride >= 3LL * h + m->cfg.intermediate &&
                        stride >= (int64_t)h + (int64_t)m->cfg.n_heads * m->cfg.head_dim,
               "shd_model_set_masks: stride shorter than 3*hidden + intermediate");
-  const size_t bytes = (size_t)m->cfg.n_layers * stride * 4;
-  SHD_CHECK_CUDA(ctx, cudaMalloc(&m->masks, bytes));
-  SHD_CHECK_CUDA(ctx, cudaMemcpyAsync(m->masks, masks, bytes, cudaMemcpyDeviceToDevice, ctx->stream));
-  SHD_CHECK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-  m->mask_stride = stride;
+  return m->lay_masks(masks, stride, m->kv4.capacity ? (stride + 3) / 4 * 4 : stride);
+}
+
+// The layers' masks from rows of `stride` floats into an allocation with rows of `to`, which replaces the
+// present one. Attention over the 4-bit cache reads its masks 16 bytes at a time: there the rows are a
+// multiple of 4 floats apart.
+int shd_model::lay_masks(const float* from, int64_t stride, int64_t to) {
+  float* laid = nullptr;
+  SHD_CHECK_CUDA(ctx, cudaMalloc(&laid, (size_t)cfg.n_layers * to * 4));
+  cudaError_t e = cudaMemcpy2DAsync(laid, to * 4, from, stride * 4, stride * 4, cfg.n_layers, cudaMemcpyDeviceToDevice, ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+  if (e != cudaSuccess) {
+    cudaFree(laid);
+    return shd_cuda_fail(ctx, e, "masks: cudaMemcpy2DAsync");
+  }
+  cudaFree(masks);
+  masks = laid;
+  mask_stride = to;
   return SHD_OK;
 }
 
@@ -413,6 +426,10 @@ extern "C" int shd_model_set_kv4(shd_model* m, int capacity, int window, int sin
   if (m->graph) {
     cudaGraphExecDestroy(m->graph);
     m->graph = nullptr;
+  }
+  if (m->masks && m->mask_stride % 4) {
+    const int rc = m->lay_masks(m->masks, m->mask_stride, (m->mask_stride + 3) / 4 * 4);
+    if (rc) return rc;
   }
   auto drop = [&](void* p) {
     if (!p) return;
@@ -462,6 +479,7 @@ Kv4View shd_model::kv4_layer(int l) const {
 // Quantise the M rows that the q/k/v linear left in kv4_rows, then attend: Qbuf -> Abuf.
 int shd_model::kv4_attention(int l, int M, const int* d_pos, const int* d_seq, const float* mask, bool decode) {
   const int ld = qd + 2 * kvd;
+  SHD_REQUIRE(ctx, shd_aligned16(mask), "attention over the 4-bit cache: masks must be 16-byte aligned");
   Kv4WriteArgs w{};
   w.c = kv4_layer(l);
   w.kc = kv4_rows + qd; w.ks = w.kc + (size_t)M * ld;

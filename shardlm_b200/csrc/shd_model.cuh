@@ -43,6 +43,7 @@ struct shd_model {
   float* kv4_rows = nullptr;             // [2][rows][qd + 2 kvd] shares of q, k, v (with RoPE)
   int prompt_slot = 0, prompt_pos = 0;   // of the block that enqueue_layers works on (not decode)
   shd::Kv4View kv4_layer(int l) const;
+  int lay_masks(const float* from, int64_t stride, int64_t to);
   int kv4_attention(int l, int M, const int* d_pos, const int* d_seq, const float* mask, bool decode);
   int *tokens = nullptr, *pos = nullptr, *seq = nullptr;
   int *p_tokens = nullptr, *p_pos = nullptr, *p_seq = nullptr;
