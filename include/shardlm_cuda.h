@@ -56,6 +56,11 @@ int shd_init(int device, shd_ctx** out);
 int shd_destroy(shd_ctx* ctx);
 /* Use the caller's stream (a cudaStream_t) for all later work; NULL = the legacy default stream. */
 int shd_set_stream(shd_ctx* ctx, void* stream);
+/* The same for a caller whose calls change streams: later work on `stream` starts after all that the
+ * context has enqueued before, whichever streams it went to, as the context's scratch needs. A stream
+ * that is left must live until this call or until a shd_sync on it. Work captured into a graph is ordered
+ * with other calls only within its capture: whoever launches the graph orders the launch. */
+int shd_switch_stream(shd_ctx* ctx, void* stream);
 const char* shd_last_error(shd_ctx* ctx);
 /* Synchronise the stream and report any error a kernel recorded in the context's error word
  * (a bounded wait that ran out -> SHD_ERR_TIMEOUT). Clears the word. */

@@ -43,6 +43,7 @@ SIGNATURES: dict[str, tuple] = {
     "shd_init": (I32, [I32, PP]),
     "shd_destroy": (I32, [P]),
     "shd_set_stream": (I32, [P, P]),
+    "shd_switch_stream": (I32, [P, P]),
     "shd_last_error": (C.c_char_p, [P]),
     "shd_sync": (I32, [P]),
     "shd_launch_count": (I64, [P]),

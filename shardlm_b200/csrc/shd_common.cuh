@@ -37,6 +37,10 @@ struct shd_ctx {
   size_t stage_bytes = 0;
   int num_sms = 148;
   int64_t launches = 0;
+  int64_t launches_synced = 0;   // of those, how many the last shd_sync saw finish
+  cudaEvent_t ev_switch = nullptr;  // end of the work of streams left (shd_switch_stream)
+  cudaEvent_t ev_branch = nullptr;  // the same within one stream capture
+  bool switch_waits = false;        // and whether a stream bound later has still to wait for it
   // RoPE table (host-built with libm, as the reference's RopeFrequencies::new)
   float* d_rope_cos = nullptr;
   float* d_rope_sin = nullptr;

@@ -52,6 +52,8 @@ extern "C" int shd_init(int device, shd_ctx** out) {
   if ((e = cudaMalloc(&ctx->d_partials, ctx->partial_floats * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMalloc(&ctx->d_counters, (size_t)ctx->n_counters * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMalloc(&ctx->d_kv4, kv4_scratch_floats(ctx->num_sms) * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
+  if ((e = cudaEventCreateWithFlags(&ctx->ev_switch, cudaEventDisableTiming)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
+  if ((e = cudaEventCreateWithFlags(&ctx->ev_branch, cudaEventDisableTiming)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMemset(ctx->d_err, 0, 16)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaMemset(ctx->d_counters, 0, (size_t)ctx->n_counters * 4)) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
   if ((e = cudaDeviceSynchronize()) != cudaSuccess) { shd_destroy(ctx); return SHD_ERR_CUDA; }
@@ -77,6 +79,8 @@ extern "C" int shd_destroy(shd_ctx* ctx) {
   if (!ctx) return SHD_OK;
   cudaSetDevice(ctx->device);
   if (ctx->stream) cudaStreamSynchronize(ctx->stream);
+  if (ctx->ev_switch) cudaEventDestroy(ctx->ev_switch);
+  if (ctx->ev_branch) cudaEventDestroy(ctx->ev_branch);
   cudaFree(ctx->d_err);
   cudaFree(ctx->d_partials);
   cudaFree(ctx->d_counters);
@@ -97,6 +101,45 @@ extern "C" int shd_destroy(shd_ctx* ctx) {
 extern "C" int shd_set_stream(shd_ctx* ctx, void* stream) {
   if (!ctx) return SHD_ERR_ARG;
   ctx->stream = reinterpret_cast<cudaStream_t>(stream);
+  return SHD_OK;
+}
+
+// The capture a stream takes part in; 0: none, ~0: it cannot be asked now.
+static unsigned long long capture_id(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+    cudaGetLastError();
+    return ~0ull;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
+// Scratch and counters are the context's, so work on the stream bound next starts after all that went
+// before. A stream under capture is outside that order (an event of another stream would break the
+// capture, and what is captured runs at a time of the caller's choosing), but branches of one capture
+// are ordered as streams are. A stream with nothing enqueued since shd_sync is not touched: it may be gone.
+extern "C" int shd_switch_stream(shd_ctx* ctx, void* stream) {
+  if (!ctx) return SHD_ERR_ARG;
+  const cudaStream_t from = ctx->stream, to = reinterpret_cast<cudaStream_t>(stream);
+  if (from == to) return SHD_OK;
+  SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
+  const bool used = ctx->launches != ctx->launches_synced;
+  const unsigned long long was = used ? capture_id(from) : 0, now = capture_id(to);
+  if (used && was == 0) {
+    if (ctx->switch_waits) SHD_CHECK_CUDA(ctx, cudaStreamWaitEvent(from, ctx->ev_switch, 0));
+    SHD_CHECK_CUDA(ctx, cudaEventRecord(ctx->ev_switch, from));
+    ctx->switch_waits = true;
+  }
+  if (now == 0 && ctx->switch_waits) {
+    SHD_CHECK_CUDA(ctx, cudaStreamWaitEvent(to, ctx->ev_switch, 0));
+    ctx->switch_waits = false;
+  }
+  if (now != 0 && now != ~0ull && now == was) {
+    SHD_CHECK_CUDA(ctx, cudaEventRecord(ctx->ev_branch, from));
+    SHD_CHECK_CUDA(ctx, cudaStreamWaitEvent(to, ctx->ev_branch, 0));
+  }
+  ctx->stream = to;
   return SHD_OK;
 }
 
@@ -133,7 +176,9 @@ extern "C" int shd_wait_selftest(shd_ctx* ctx, int limit_ms) {
 extern "C" int shd_sync(shd_ctx* ctx) {
   if (!ctx) return SHD_ERR_ARG;
   SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
+  const int64_t launches = ctx->launches;
   SHD_CHECK_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+  ctx->launches_synced = launches;
   int h = 0;
   SHD_CHECK_CUDA(ctx, cudaMemcpy(&h, ctx->d_err, 4, cudaMemcpyDeviceToHost));
   if (h == 0) return SHD_OK;

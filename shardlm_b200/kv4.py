@@ -6,7 +6,8 @@ secure_inference.rs:2452-2471) a position takes 5/32 of the memory. Rows are qua
 written, straight from the K and V shares; queries may be limited to a sliding window, the first
 `sinks` positions staying visible, and a cache smaller than its sequences is then used as a ring.
 
-Device tensors in, device tensors out, asynchronous on torch's current stream; errors that only the
+Device tensors in, device tensors out, asynchronous on torch's current stream, after the context's calls
+on other streams (Context.bind_stream says what holds for graphs); errors that only the
 device sees (a slot outside the cache, values that the format cannot hold) surface at Context.sync().
 """
 from __future__ import annotations

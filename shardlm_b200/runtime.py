@@ -42,10 +42,14 @@ class Context:
 
     # -- plumbing ------------------------------------------------------------------------------
     def bind_stream(self, stream: torch.cuda.Stream | None = None) -> None:
+        """Later calls go to `stream` (torch's current one by default). Scratch and counters are the
+        context's: on a change the new stream waits for what was enqueued on the old one. Graphs are
+        outside that order: launches of a graph that holds calls are ordered by whoever launches it."""
         # the raw handle: a Stream object would cost 2 us a call
         raw = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(self.device)
         if raw != self._bound_stream:
-            check(lib().shd_set_stream(self.ptr, raw), self.ptr)
+            bind = lib().shd_set_stream if self._bound_stream is None else lib().shd_switch_stream
+            check(bind(self.ptr, raw), self.ptr)
             self._bound_stream = raw
 
     def call(self, name: str, *args) -> None:
