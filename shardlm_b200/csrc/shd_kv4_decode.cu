@@ -8,8 +8,10 @@
 // is c * 2^-20), centred to (c - 7.5) * 2^-9, also exact, by one more: weights add up to 1 over many rows
 // whose values cancel, and sums of codes that are all positive would lose what cancels (measured
 // against 64 bits at 131000 positions: 5e-4 of the result). The other operand is split into two f16 terms
-// (22 bits): the queries, scaled by a power of two of their head, and the weights p_t s_tg, scaled by a
-// running power of two of the scales.
+// (22 bits, or 2^-37 of the largest beside them): the queries, scaled by a power of two of their head, and the
+// weights p_t s_tg, scaled by a running power of two of the largest of their head: the largest over rows
+// of weight times the row's largest scale, so that a row which weighs nothing has no say however large its values
+// are. A group whose scales are 2^-k of the row's largest loses bits from k = 15 on, to 2^-37 of that largest part.
 // Sums are f32. Rows of the first product's A are the 8 heads' high terms and the 8 heads' low terms;
 // the second takes the two terms one after the other:
 //   S [8 + 8 heads x 8 rows]      += Q [16 x 16 channels] K^T   per group, then scaled by s
@@ -27,8 +29,8 @@
 // leaves partial results; the CTA that arrives last joins them in CTA order, so results do not depend on
 // timing.
 //
-// Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 42.6 us (2.0 TB/s of cache); 64
-// ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 73.7 us (2.3 TB/s); 8 at 1041 to 1280
+// Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 42.5 us (2.0 TB/s of cache); 64
+// ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 74.1 us (2.3 TB/s); 8 at 1041 to 1280
 // positions 15.1 us; one at 554 positions 10.3 us. No pipe is full in the long ones (of the windowed batch's
 // time on the SMs the integer pipe is busy 38 %, tensor 23 %, issue slots 56 %, memory 27 %): a chunk of 16
 // rows is some 500 instructions of a warp in dependent steps, and the registers hold four warps a scheduler.
@@ -53,6 +55,9 @@ constexpr int kDGroup = 10;
 constexpr int kDGroupMax = 32;    // (the larger of kDJoin, kDGroup and the groups of all CTAs)
 constexpr int kDCounters = 1 << 15;  // items' counters, then the groups'
 constexpr int kDSizes = 8;        // sizes of a part that are tried, kDWarps chunks apart
+// stands for the exponent of scales that are all 0 (such a row adds its minima only, in f32): low enough that the row
+// has no say where another has, and 2^-kFlat sums of 2^17 rows of any minima stay in f32
+constexpr float kFlat = -60.0f;
 
 template <int HD>
 struct DecodeShape {
@@ -63,8 +68,8 @@ struct DecodeShape {
   static constexpr int PART = HD + 4;                  // of one head: running max, sum, 2 unused, weighted V
   static constexpr int LEFT = 8 * HD + 16;             // of a cut item: weighted V of 8 heads, maxima, sums
   // a chunk's parameters in f32: [keys, values][scale, middle][half of the chunk][tig][group][row sigma(2 tig),
-  // sigma(2 tig + 1)]
-  static constexpr int ROWS = 4 * kKv4Chunk * NG * 4;
+  // sigma(2 tig + 1)], then the exponents of the rows' largest value scales: [half of the chunk][tig][the two rows]
+  static constexpr int ROWS = 4 * kKv4Chunk * NG * 4 + kKv4Chunk * 4;
   static constexpr int RING = kDWarps * (kDStages * STAGE + ROWS);
   static constexpr int JOIN = kDWarps * 8 * PART * 4;  // per warp and head, over the rings
   static constexpr size_t SMEM = (RING > JOIN ? RING : JOIN) + kDRows * 16 + 64 * 4 + 16 * 4 + 256;
@@ -404,11 +409,9 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     uint64_t oz[NG];  // head gid's minima, even and odd rows
 #pragma unroll
     for (int g = 0; g < NG; ++g) oz[g] = pair(0.0f, 0.0f);
-    // weights are 2^(score - ref), ref = running maximum - (13 - ev): every value scale so far (the
-    // largest is vbound, f16 bits) is below 2^ev, so that weight times scale is at most 2^13
+    // weights are 2^(score - ref), ref = mx - 13, mx the running maximum of score + exponent of the row's largest
+    // value scale: weight times scale is at most 2^13, and at least 2^12 for the row that adds most
     float mx = kKv4Never, ref = kKv4Never, l = 0.0f;
-    uint32_t vbound = 0u;
-    int ev = 0;
 
 #pragma unroll 1
     for (int i = 0; i < mine; ++i) {
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
       const uint8_t* st = ring + at * SH::STAGE;
       // lanes 0-15: the rows' key parameters, 16-31: their value parameters, in f32 for the 8 heads' lanes; a
       // row out of sight has them 0, whatever its memory holds
-      uint32_t sight, vtop;
+      uint32_t sight;
       {
         const int r = lane & 15, kind = lane >> 4;
         const bool ok = seen.row(kv4_span_chunk(sp, first + i * kDWarps) * kKv4Chunk + r);
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
           }
         }
         float* out = rows_f32 + kind * (2 * kKv4Chunk * NG) + (((r >> 3) * 4 + (r & 3)) * NG) * 2 + ((r >> 2) & 1);
-        uint32_t top = 0u;
+        float top = 0.0f;
 #pragma unroll
         for (int g = 0; g < NG / 2; ++g) {
           const float2 v = unpack_f16(w[g]), z = unpack_f16(w[NG / 2 + g]);
@@ -453,9 +456,12 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
           out[4 * g + 2] = v.y;
           out[kKv4Chunk * NG + 4 * g] = fmaf(7.5f, v.x, z.x);
           out[kKv4Chunk * NG + 4 * g + 2] = fmaf(7.5f, v.y, z.y);
-          top = max(top, max(w[g] & 0xffffu, w[g] >> 16));  // positive f16 order as integers
+          top = fmaxf(top, fmaxf(v.x, v.y));
         }
-        vtop = __reduce_max_sync(0xffffffffu, kind ? top : 0u);
+        // the exponent e with top < 2^e as f32: 2^23 + n has n in its low bits
+        if (kind)
+          rows_f32[4 * kKv4Chunk * NG + ((r >> 3) * 4 + (r & 3)) * 2 + ((r >> 2) & 1)] =
+              fmaxf(__uint_as_float(0x4b000000u | (__float_as_uint(top) >> 23)) - (8388608.0f + 126.0f), kFlat);
       }
       __syncwarp();
 
@@ -496,18 +502,17 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
         for (int x = 0; x < 4; ++x)
           if (!(sight >> (4 * x + tig) & 1u)) s[x] = -INFINITY;
       }
-      float tm = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+      const float* ex = rows_f32 + 4 * kKv4Chunk * NG + 2 * tig;
+      const float2 t0 = unpair(add2(pair(s[0], s[1]), *reinterpret_cast<const uint64_t*>(ex)));
+      const float2 t1 = unpair(add2(pair(s[2], s[3]), *reinterpret_cast<const uint64_t*>(ex + 8)));
+      float tm = fmaxf(fmaxf(t0.x, t0.y), fmaxf(t1.x, t1.y));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
 
-      // rescale when the head's maximum or the bound of the value scales grows
-      if (__any_sync(0xffffffffu, tm > mx || vtop > vbound)) {
+      // rescale when a head's maximum grows
+      if (__any_sync(0xffffffffu, tm > mx)) {
         mx = fmaxf(mx, tm);
-        if (vtop > vbound) {  // the same in every lane
-          ev = ceil_exp2(__half2float(__ushort_as_half((unsigned short)vtop))) + 1;
-          vbound = vtop;
-        }
-        const float now = mx == kKv4Never ? kKv4Never : mx - (float)(13 - ev);
+        const float now = mx == kKv4Never ? kKv4Never : mx - 13.0f;
         const float al = exp2_fast(ref - now);
         ref = now;
         l *= al;
