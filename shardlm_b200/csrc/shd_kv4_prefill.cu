@@ -5,10 +5,11 @@
 // share every unpacked row. It walks the rows that any of its positions sees, 64 at a time:
 //   S [128 x 64]       = Q [128 x HD] K^T      O [128 x HD] += P [128 x 64] V
 // Operands are f16 in two terms. The keys of 32 rows are divided by a power of two of theirs and
-// s (c - 7.5) is then exactly two terms (11 + 5 bits; of a row 2^19 smaller than the largest of the 32
-// the error is 2^-34 of the largest); queries, weights and minima keep 22 bits of theirs. Three of the
+// s (c - 7.5) is then exactly two terms (11 + 5 bits); queries, weights and minima keep 22 bits of theirs. Three of the
 // four term products are formed (the fourth is below 2^-22 of the sum), accumulated in f32 in
-// tensor memory. What the minima add,
+// tensor memory. Where the 32 rows' sizes are more than 2^6 apart, each row has a power of two of its own
+// and the softmax goes row by row (a large row that weighs nothing would else take the bits of the others).
+// Within a row a group 2^-k of the largest loses bits from k = 12 on. What the minima add,
 //   sum_g (z_tg + 7.5 s_tg) (sum_(i in g) q_i)    and    sum_t p_t (z_tg + 7.5 s_tg),
 // is one more step of 16 along the first product's depth (a row's parameters against the groups' query
 // sums) and 16 more columns of the second's width. 32 value rows are divided by a power of two 2^e of
@@ -60,6 +61,9 @@ constexpr int kPRaw = 3;
 constexpr int kPItem = 8;
 constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
 constexpr float kRoom = 8.0f, kHead = 6.0f;  // weights are 2^(score' - ref + 6), score' - ref <= 8
+// rows of 32 whose sizes lie within 2^6 share a power of two, else each has its own: the weight of the row that adds
+// most is then at least 1, which leaves its two f16 terms their 22 bits
+constexpr int kSpread = 6;
 
 template <int HD>
 struct PromptShape {
@@ -78,8 +82,10 @@ struct PromptShape {
   static constexpr uint32_t RAWC = kPKV * HD / 2, RAWP = kPKV * 4 * NG, RAWBUF = 2 * (RAWC + RAWP);
   static constexpr uint32_t ROW = RAW + kPRaw * RAWBUF;        // [8][2][64]: a row's position, out of sight from
   static constexpr uint32_t ROWBUF = 2 * kPKV * 4;
-  static constexpr uint32_t OF32 = ROW + 8 * ROWBUF;           // [8][2][4], of 32 rows: 2^(key e), e, 2^-e, seen by every query
-  static constexpr uint32_t RED = OF32 + 8 * 2 * 16;           // [3][2 halves][128]: maxima of even and odd steps; the query's, then the sums
+  // [8][2][4], of 32 rows: 2^(key e), e, 2^-e, seen by every query; 2^(key e) or 2^-e is 0 where rows have their own
+  static constexpr uint32_t OF32 = ROW + 8 * ROWBUF;
+  static constexpr uint32_t OWN = OF32 + 8 * 2 * 16;           // [8][2][64], of rows that have their own: 2^(key e), e
+  static constexpr uint32_t RED = OWN + 8 * ROWBUF;            // [3][2 halves][128]: maxima of even and odd steps; the query's, then the sums
   static constexpr uint32_t BAR = RED + 6 * kPRows * 4;
   static constexpr uint32_t PRE = BAR + 256;                   // [kPTiles] cost of the tiles before
   // [8 warps][32 rows][32 channels] of queries on their way to their threads: the low terms' place, where it is wide enough
@@ -161,6 +167,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {  // and waits
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // no use of the loaded values moves above the wait before this
 __device__ __forceinline__ void tmem_loaded16(uint32_t (&r)[16]) {
@@ -176,13 +195,15 @@ __device__ __forceinline__ void scale_pair(__half2 c, __half2 s, uint32_t& hi, u
   lo = as_u32(__hfma2(s, c, __hneg2(h)));
 }
 
-// A row's parameters and the power of two that it is divided by, which is that of its warp's 32 rows:
-// 8 s and |z| (values: |z + 7.5 s|) come to at most 2^9.
+// A row's parameters and the power of two that it is divided by: 8 s and |z| (values: |z + 7.5 s|) come to at
+// most 2^9. It is that of its warp's 32 rows where they are of like size, else the row's own (set gives true): keys
+// of 0 fit any size, but a value row of 0 does not, since its weight follows the power of two. Rows that
+// no query sees come as zeros and do not count.
 template <int NG>
 struct RowParams {
   float s[NG], z[NG];
   int e;
-  __device__ __forceinline__ void set(const uint32_t (&w)[NG], bool middle) {  // NG scales, NG minima
+  __device__ __forceinline__ bool set(const uint32_t (&w)[NG], bool middle, bool seen) {  // NG scales, NG minima
     float top = 0.0f;
 #pragma unroll
     for (int g = 0; g < NG; g += 2) {
@@ -193,9 +214,43 @@ struct RowParams {
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) top = fmaxf(top, fmaxf(8.0f * s[g], fabsf(z[g])));
-    e = max(__reduce_max_sync(0xffffffffu, ceil_exp2(top)), -40) - 9;
+    const int own = max(ceil_exp2(top), -40) - 9;
+    e = __reduce_max_sync(0xffffffffu, own);
+    const bool wide = __any_sync(0xffffffffu, (middle ? seen : top > 0.0f) && own < e - kSpread);
+    if (wide) e = own;
+    return wide;
   }
 };
+
+// Where rows have their own powers of two, seldom: score + e row by row, or out of sight, in the scores' place (apart
+// from the walk, whose code this would spread out)
+__device__ __noinline__ void own_scores(uint32_t t_s, const float* own, const int* rp, float4 of32, float rowf, int p) {
+#pragma unroll 1
+  for (int y = 0; y < 32; y += 8) {
+    uint32_t w[8];
+    tmem_ld8(t_s + y, w);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const bool in_sight = rp[y + x] <= p && p < rp[64 + y + x];
+      const float f = of32.x == 0.0f ? own[y + x] : of32.x, e = of32.z == 0.0f ? own[64 + y + x] : of32.y;
+      w[x] = in_sight ? __float_as_uint(fmaf(__uint_as_float(w[x]), rowf * f, e)) : 0xff800000u;
+    }
+    tmem_st8(t_s + y, w);
+  }
+  tmem_wait_st();
+}
+// The weights' sum of such rows without 2^e.
+__device__ __noinline__ float own_sum(uint32_t t_s, const float* own, float4 of32, float shift) {
+  float part = 0.0f;
+#pragma unroll 1
+  for (int y = 0; y < 32; y += 8) {
+    uint32_t w[8];
+    tmem_ld8(t_s + y, w);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) part += exp2_fast(__uint_as_float(w[x]) - (of32.z == 0.0f ? own[64 + y + x] : of32.y) + shift);
+  }
+  return part;
+}
 
 struct PromptArgs {
   Kv4AttnArgs a;
@@ -444,10 +499,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         tc_fence_after();
         const int* rp = reinterpret_cast<const int*>(smem + SH::ROW + (it & 7) * SH::ROWBUF) + 32 * half;
         const float4 of32 = *reinterpret_cast<const float4*>(smem + SH::OF32 + ((it & 7) * 2 + half) * 16);
-        const bool masked = of32.w == 0.0f;
         const uint32_t t_s = t_row + kColS + b * kPKV + 32 * half;
-        // this half's 32 scores: score + e in log2 units is fac * v + of32.y
-        const float fac = rowf * of32.x;
+        // this half's 32 scores: score + e in log2 units is fac * v + add
+        const bool wide = of32.x == 0.0f || of32.z == 0.0f, masked = of32.w == 0.0f && !wide;
+        const float fac = wide ? 1.0f : rowf * of32.x, add = wide ? 0.0f : of32.y;
+        const float* own = reinterpret_cast<const float*>(smem + SH::OWN + (it & 7) * SH::ROWBUF) + 32 * half;
+        if (wide) own_scores(t_s, own, rp, of32, rowf, p);
         uint32_t v[2][16];
         tmem_ld16(t_s, v[0]);
         tmem_ld16(t_s + 16, v[1]);
@@ -476,12 +533,12 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             const float e = y + 4 + x < 32 ? __uint_as_float(v[((y + 4 + x) % 32) / 16][(y + 4 + x) % 16]) : -INFINITY;
             t4[x] = fmaxf(t4[x], fmaxf(__uint_as_float(v[(y + x) / 16][(y + x) % 16]), e));
           }
-        float top = fmaf(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), fac, of32.y);
+        float top = fmaf(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])), fac, add);
         red[(2 * b + half) * kPRows + row] = top;
         // weights as two f16 terms (in the scores' places: high terms of 16 first), and their sum without 2^e
         float part = 0.0f;
         auto weigh = [&]() {
-          const float sh = of32.y + (kHead - ref);
+          const float sh = add + (kHead - ref);
           const uint64_t shift = pair(sh, sh), fac2 = pair(fac, fac);
           uint64_t s0 = pair(0.0f, 0.0f), s1 = s0;
 #pragma unroll
@@ -527,7 +584,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           }
           weigh();
         }
-        l = fmaf(part, of32.z, l);
+        if (wide) part = own_sum(t_s, own, of32, kHead - ref);
+        l = fmaf(part, wide ? 1.0f : of32.z, l);
         tmem_st16(t_s, v[0]);
         tmem_st16(t_s + 16, v[1]);
         // every kPDrain steps the sums so far go to the second accumulator; both follow the reference
@@ -694,18 +752,24 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           const uint2 v = *reinterpret_cast<const uint2*>(rawp + r * 8);
           w[0] = v.x; w[1] = v.y;
         }
-        if (rp[64 + r] == 0) {  // no query sees it: its parameters may be anything
+        const bool seen = rp[64 + r] != 0;
+        if (!seen) {  // no query sees it: its parameters may be anything
 #pragma unroll
           for (int g = 0; g < NG; ++g) w[g] = 0u;
         }
         RowParams<NG> q;
-        q.set(w, vals);
+        const bool wide = q.set(w, vals, seen);
+        float* own = reinterpret_cast<float*>(smem + SH::OWN + (it & 7) * SH::ROWBUF) + (vals ? kPKV : 0);
         const float down = pow2i(-q.e), up9 = down * 512.0f;
         if (vals) {
+          if (wide) {
+            if (kh == 0) own[r] = (float)q.e;
+            __syncwarp();
+          }
           if (lane == 0) {
             if (kh == 0) {
               of32[1] = (float)q.e;
-              of32[2] = pow2i(-q.e);
+              of32[2] = wide ? 0.0f : pow2i(-q.e);
             }
             mbar_arrive(bar + B_EFULL + (it & 3));
           }
@@ -722,7 +786,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
             uint8_t* kx = smem + SH::KX + b * SH::KXBUF;
             *reinterpret_cast<uint4*>(kx + plain16_offset(r, 0)) = make_uint4(y[0], y[1], y[2], y[3]);
             *reinterpret_cast<uint4*>(kx + plain16_offset(r, 1)) = make_uint4(y[0], y[1], y[2], y[3]);
-            if (lane == 0) of32[0] = pow2i(q.e);
+            if (wide) own[r] = pow2i(q.e);
+            if (lane == 0) of32[0] = wide ? 0.0f : pow2i(q.e);
           } else {
             // middles: column g the high term, 4 + g the low one
             __half* vx = reinterpret_cast<__half*>(smem + SH::VX + b * SH::VXBUF + (r >> 3) * 256 + (r & 7) * 2);
