@@ -29,9 +29,9 @@
 // leaves partial results; the CTA that arrives last joins them in CTA order, so results do not depend on
 // timing.
 //
-// Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 42.5 us (2.0 TB/s of cache); 64
-// ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 74.1 us (2.3 TB/s); 8 at 1041 to 1280
-// positions 15.1 us; one at 554 positions 10.3 us. No pipe is full in the long ones (of the windowed batch's
+// Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 41.7 us (2.0 TB/s of cache); 64
+// ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 73.5 us (2.3 TB/s); 8 at 1041 to 1280
+// positions 14.9 us; one at 554 positions 10.2 us. No pipe is full in the long ones (of the windowed batch's
 // time on the SMs the integer pipe is busy 38 %, tensor 23 %, issue slots 56 %, memory 27 %): a chunk of 16
 // rows is some 500 instructions of a warp in dependent steps, and the registers hold four warps a scheduler.
 // It takes 198 clocks of an SM, where its 215 integer and conversion instructions alone take 107. Short ones
@@ -68,7 +68,7 @@ struct DecodeShape {
   static constexpr int PART = HD + 4;                  // of one head: running max, sum, 2 unused, weighted V
   static constexpr int LEFT = 8 * HD + 16;             // of a cut item: weighted V of 8 heads, maxima, sums
   // a chunk's parameters in f32: [keys, values][scale, middle][half of the chunk][tig][group][row sigma(2 tig),
-  // sigma(2 tig + 1)], then the exponents of the rows' largest value scales: [half of the chunk][tig][the two rows]
+  // sigma(2 tig + 1)], then of each row 13 less the exponent of its largest value scale: [half of the chunk][tig][the two rows]
   static constexpr int ROWS = 4 * kKv4Chunk * NG * 4 + kKv4Chunk * 4;
   static constexpr int RING = kDWarps * (kDStages * STAGE + ROWS);
   static constexpr int JOIN = kDWarps * 8 * PART * 4;  // per warp and head, over the rings
@@ -375,8 +375,8 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // |q| 2^k <= 2^13; the limits keep 2^k and 2^(9 - k) normal
-      const int k = max(min(13 - ceil_exp2(top), 100), -100);
+      // |q| 2^k <= 2^13, k at least -115 for a finite query; the limit keeps 2^(9 - k) normal
+      const int k = min(13 - ceil_exp2(top), 100);
       const float up = pow2i(k);
       const float sc = a.scale * 1.44269504088896341f;
       factor = sc * pow2i(9 - k);
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
         }
       }
       // the query sums against a row's parameters (scales, then minima): word tig of the row
-      const int kz = max(min(12 - ceil_exp2(ztop), 100), -100);  // 7.5 |sum| 2^kz < 2^15
+      const int kz = min(12 - ceil_exp2(ztop), 100);  // 7.5 |sum| 2^kz < 2^15
       zfactor = sc * pow2i(-kz);
       const float zup = pow2i(kz) * (tig < NG / 2 ? 7.5f : (tig < NG ? 1.0f : 0.0f));
       float za = qs[0], zb = qs[1];
@@ -409,9 +409,9 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
     uint64_t oz[NG];  // head gid's minima, even and odd rows
 #pragma unroll
     for (int g = 0; g < NG; ++g) oz[g] = pair(0.0f, 0.0f);
-    // weights are 2^(score - ref), ref = mx - 13, mx the running maximum of score + exponent of the row's largest
+    // weights are 2^(score - mx), mx the running maximum of score + e - 13, e the exponent of the row's largest
     // value scale: weight times scale is at most 2^13, and at least 2^12 for the row that adds most
-    float mx = kKv4Never, ref = kKv4Never, l = 0.0f;
+    float mx = kKv4Never, l = 0.0f;
 
 #pragma unroll 1
     for (int i = 0; i < mine; ++i) {
@@ -458,10 +458,10 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
           out[kKv4Chunk * NG + 4 * g + 2] = fmaf(7.5f, v.y, z.y);
           top = fmaxf(top, fmaxf(v.x, v.y));
         }
-        // the exponent e with top < 2^e as f32: 2^23 + n has n in its low bits
+        // 13 less the exponent e with top < 2^e, as f32: 2^23 + n has n in its low bits
         if (kind)
           rows_f32[4 * kKv4Chunk * NG + ((r >> 3) * 4 + (r & 3)) * 2 + ((r >> 2) & 1)] =
-              fmaxf(__uint_as_float(0x4b000000u | (__float_as_uint(top) >> 23)) - (8388608.0f + 126.0f), kFlat);
+              fminf((8388608.0f + 126.0f + 13.0f) - __uint_as_float(0x4b000000u | (__float_as_uint(top) >> 23)), 13.0f - kFlat);
       }
       __syncwarp();
 
@@ -502,19 +502,21 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
         for (int x = 0; x < 4; ++x)
           if (!(sight >> (4 * x + tig) & 1u)) s[x] = -INFINITY;
       }
-      const float* ex = rows_f32 + 4 * kKv4Chunk * NG + 2 * tig;
-      const float2 t0 = unpair(add2(pair(s[0], s[1]), *reinterpret_cast<const uint64_t*>(ex)));
-      const float2 t1 = unpair(add2(pair(s[2], s[3]), *reinterpret_cast<const uint64_t*>(ex + 8)));
+      // score + e - 13, and below back to the score from its difference to mx: the difference has no rounding, so that
+      // scores of any size leave the weights in range
+      const uint64_t* less = reinterpret_cast<const uint64_t*>(rows_f32 + 4 * kKv4Chunk * NG + 2 * tig);
+      const uint64_t less0 = less[0], less1 = less[4], minus = pair(-1.0f, -1.0f);
+      const uint64_t sum0 = fma2(less0, minus, pair(s[0], s[1])), sum1 = fma2(less1, minus, pair(s[2], s[3]));
+      const float2 t0 = unpair(sum0), t1 = unpair(sum1);
       float tm = fmaxf(fmaxf(t0.x, t0.y), fmaxf(t1.x, t1.y));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
       tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
 
       // rescale when a head's maximum grows
       if (__any_sync(0xffffffffu, tm > mx)) {
-        mx = fmaxf(mx, tm);
-        const float now = mx == kKv4Never ? kKv4Never : mx - 13.0f;
-        const float al = exp2_fast(ref - now);
-        ref = now;
+        const float now = fmaxf(mx, tm);
+        const float al = exp2_fast(mx - now);
+        mx = now;
         l *= al;
 #pragma unroll
         for (int g = 0; g < NG; ++g) oz[g] = mul2(oz[g], pair(al, al));
@@ -527,10 +529,17 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
 
       // weights: plain for the sum and the minima, times scale and as two f16 terms for the codes
       float w[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        w[x] = exp2_fast(s[x] - ref);
-        l += w[x];
+      {
+        const uint64_t low = pair(-mx, -mx);
+        const float2 x0 = unpair(add2(add2(sum0, low), less0)), x1 = unpair(add2(add2(sum1, low), less1));
+        w[0] = exp2_fast(x0.x);
+        w[1] = exp2_fast(x0.y);
+        w[2] = exp2_fast(x1.x);
+        w[3] = exp2_fast(x1.y);
+        l += w[0];
+        l += w[1];
+        l += w[2];
+        l += w[3];
       }
       uint32_t wh[NG][2], wl[NG][2];
 #pragma unroll
@@ -598,7 +607,7 @@ __global__ void __launch_bounds__(kDThreads, 2) kv4_decode_kernel(const Kv4AttnA
       }
     }
     if (tig == 0) {
-      part[(warp * 8 + gid) * PART] = ref == kKv4Never ? -INFINITY : ref;
+      part[(warp * 8 + gid) * PART] = mx == kKv4Never ? -INFINITY : mx;
       part[(warp * 8 + gid) * PART + 1] = l;
     }
     __syncthreads();

@@ -23,7 +23,7 @@
 // that S of the next 64 rows and O of the last run while the softmax works; the queries' high terms are
 // an A operand in tensor memory too, which spares shared memory most of the first product's reads. A
 // value row is unpacked as it lies (the second product's B operand is the wide dimension's major). O
-// stays in tensor memory; it is rescaled only when a row's reference has to grow by more than 2^8, which
+// stays in tensor memory; it is rescaled only when a row's reference has to grow by more than 2^7.75, which
 // the f16 range of the weights leaves room for. The tensor core's f32 sums round toward 0, so every
 // kPDrain steps the softmax threads add O to a second accumulator, rounding to nearest, and the MMAs
 // start afresh: without it the error grows with the length (2.3e-5 of the result at 8700 positions; a
@@ -60,7 +60,8 @@ constexpr int kPRaw = 3;
 // 32.3 and 32.3 us, the windowed one 61.0, 57.3, 56.2 and 55.6, the long one 284.1, 283.3, 282.8 and 284.5
 constexpr int kPItem = 8;
 constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
-constexpr float kRoom = 8.0f, kHead = 6.0f;  // weights are 2^(score' - ref + 6), score' - ref <= 8
+// weights are 2^(score' - ref + 6), score' - ref <= 7.75, and with what is rounded of scores up to 2^23 below 2^15.5
+constexpr float kRoom = 7.75f, kHead = 6.0f;
 // rows of 32 whose sizes lie within 2^6 share a power of two, else each has its own: the weight of the row that adds
 // most is then at least 1, which leaves its two f16 terms their 22 bits
 constexpr int kSpread = 6;
@@ -222,7 +223,8 @@ struct RowParams {
   }
 };
 
-// Where rows have their own powers of two, seldom: score + e row by row, or out of sight, in the scores' place (apart
+// Where rows have their own powers of two, or scores may pass 2^23 and a reference that is rounded would be off by more
+// than the weights' room (here they are rounded as it is), seldom: score + e row by row, or out of sight, in the scores' place (apart
 // from the walk, whose code this would spread out)
 __device__ __noinline__ void own_scores(uint32_t t_s, const float* own, const int* rp, float4 of32, float rowf, int p) {
 #pragma unroll 1
@@ -239,15 +241,15 @@ __device__ __noinline__ void own_scores(uint32_t t_s, const float* own, const in
   }
   tmem_wait_st();
 }
-// The weights' sum of such rows without 2^e.
-__device__ __noinline__ float own_sum(uint32_t t_s, const float* own, float4 of32, float shift) {
+// The weights' sum without 2^e where value rows have their own.
+__device__ __noinline__ float own_sum(uint32_t t_s, const float* own, float shift) {
   float part = 0.0f;
 #pragma unroll 1
   for (int y = 0; y < 32; y += 8) {
     uint32_t w[8];
     tmem_ld8(t_s + y, w);
 #pragma unroll
-    for (int x = 0; x < 8; ++x) part += exp2_fast(__uint_as_float(w[x]) - (of32.z == 0.0f ? own[64 + y + x] : of32.y) + shift);
+    for (int x = 0; x < 8; ++x) part = fmaf(exp2_fast(__uint_as_float(w[x]) + shift), exp2_fast(-own[64 + y + x]), part);
   }
   return part;
 }
@@ -454,7 +456,9 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         red[(4 + half) * kPRows + row] = top;
         named_bar_sync(1, 256);  // also: every warp's queries have left their place
         top = fmaxf(top, red[(4 + (half ^ 1)) * kPRows + row]);
-        const int k = max(min(7 - ceil_exp2(top), 60), -60);  // 2^-k times a power of two of the keys stays normal
+        // at least -121 for a finite query, whose group sums times 7.5 then stay below 2^15; the upper limit keeps 2^-k
+        // times a power of two of the keys normal
+        const int k = min(7 - ceil_exp2(top), 60);
         const float up = pow2i(k);
         rowf = a.scale * 1.44269504088896341f * pow2i(-k);
 #pragma unroll
@@ -491,6 +495,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
       if (lane == 0) mbar_arrive(bar + B_QFULL);
 
       const int p = a.pos0 + (live ? group_of(r0 + row) : a.M - 1);
+      // 2^(key e) from which a score of the warp's may pass 2^23: queries are below 2^7, keys 3 x 2^9
+      const float large = 0.25f / (__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(rowf))) * (HD / 128.0f));
       float ref = kKv4Never, l = 0.0f;
       bool summed = false;  // the second accumulator holds something
       for (int j = sg.begin; j < sg.end; ++j, ++it) {
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         const float4 of32 = *reinterpret_cast<const float4*>(smem + SH::OF32 + ((it & 7) * 2 + half) * 16);
         const uint32_t t_s = t_row + kColS + b * kPKV + 32 * half;
         // this half's 32 scores: score + e in log2 units is fac * v + add
-        const bool wide = of32.x == 0.0f || of32.z == 0.0f, masked = of32.w == 0.0f && !wide;
+        const bool wide = of32.x * of32.z == 0.0f || of32.x >= large, masked = of32.w == 0.0f && !wide;
         const float fac = wide ? 1.0f : rowf * of32.x, add = wide ? 0.0f : of32.y;
         const float* own = reinterpret_cast<const float*>(smem + SH::OWN + (it & 7) * SH::ROWBUF) + 32 * half;
         if (wide) own_scores(t_s, own, rp, of32, rowf, p);
@@ -566,7 +572,7 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
         named_bar_sync(4 + (warp & 3), 64);
         top = fmaxf(top, red[(2 * b + (half ^ 1)) * kPRows + row]);
         float al = 1.0f;
-        const bool grow = __any_sync(0xffffffffu, top > ref + kRoom);  // alike in both halves
+        const bool grow = __any_sync(0xffffffffu, top - ref > kRoom);  // alike in both halves
         if (grow) {
           const float now = fmaxf(ref, top);
           al = exp2_fast(ref - now);
@@ -584,8 +590,8 @@ __global__ void __launch_bounds__(kPThreads, 1) kv4_prefill_kernel(const __grid_
           }
           weigh();
         }
-        if (wide) part = own_sum(t_s, own, of32, kHead - ref);
-        l = fmaf(part, wide ? 1.0f : of32.z, l);
+        if (of32.z == 0.0f) part = own_sum(t_s, own, kHead - ref);
+        l = fmaf(part, of32.z == 0.0f ? 1.0f : of32.z, l);
         tmem_st16(t_s, v[0]);
         tmem_st16(t_s + 16, v[1]);
         // every kPDrain steps the sums so far go to the second accumulator; both follow the reference
