@@ -100,9 +100,20 @@ __host__ __device__ __forceinline__ int kv4_held(const Kv4View& c, int r, int la
   return last - back;
 }
 
-// Whether a query at position p sees the row r that holds position t.
-__host__ __device__ __forceinline__ bool kv4_sees(const Kv4View& c, int p, int r, int t, int window) {
-  return t <= p && (window <= 0 || r < c.sinks || (int64_t)t > (int64_t)p - window);
+// A block of positions (shd_kv4_prefill.cu) is planned in tiles of kKv4Tile (position, head) pairs of a kv head, whose
+// cost is that of the steps of kKv4Step cache rows they walk and kKv4Item more.
+constexpr int kKv4Tile = 128, kKv4Step = 64, kKv4Item = 8;
+
+__host__ __device__ __forceinline__ int kv4_tile_cost(const Kv4View& c, int lo, int hi, int window) {
+  return (kv4_spans(c, lo, hi, window).total * kKv4Chunk + kKv4Step - 1) / kKv4Step + kKv4Item;
+}
+// Positions of one launch, of at most `tiles` tiles and M positions: plans are kept in 31 bits, the sum of the tiles'
+// costs and one tile's cost over all kv heads. 0: not even one position fits.
+inline int kv4_launch_positions(const Kv4View& c, int M, int G, int last, int tiles) {
+  const int64_t rows = last < c.capacity ? (int64_t)last + 1 : c.capacity;
+  const int64_t cost = (rows + kKv4Chunk - 1 + kKv4Step - 1) / kKv4Step + kKv4Item;  // no tile's is above
+  if (cost * c.heads > 0x7fffffff) return 0;
+  return (int)std::min<int64_t>(M, std::min<int64_t>(tiles, 0x7fffffff / cost) * kKv4Tile / G);
 }
 
 #ifdef __CUDACC__

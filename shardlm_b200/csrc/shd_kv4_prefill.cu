@@ -48,8 +48,8 @@
 namespace shd {
 namespace {
 
-constexpr int kPRows = 128;    // (position, head) pairs of a tile
-constexpr int kPKV = 64;       // cache rows of a step
+constexpr int kPRows = kKv4Tile;  // (position, head) pairs of a tile
+constexpr int kPKV = kKv4Step;    // cache rows of a step
 constexpr int kPThreads = 576;
 constexpr int kPTiles = 2048;  // tiles a launch (their step counts are in shared memory)
 // steps of rows on their way as stored: three, since a step's values are unpacked only when the product
@@ -58,7 +58,7 @@ constexpr int kPTiles = 2048;  // tiles a launch (their step counts are in share
 constexpr int kPRaw = 3;
 // cost of an item's queries and results, in steps: at 4, 6, 8 and 11 the short prompt above takes 34.0, 31.8,
 // 32.3 and 32.3 us, the windowed one 61.0, 57.3, 56.2 and 55.6, the long one 284.1, 283.3, 282.8 and 284.5
-constexpr int kPItem = 8;
+constexpr int kPItem = kKv4Item;
 constexpr int kPDrain = 4;     // steps that the tensor core sums up on its own
 // weights are 2^(score' - ref + 6), score' - ref <= 7.75, and with what is rounded of scores up to 2^23 below 2^15.5
 constexpr float kRoom = 7.75f, kHead = 6.0f;
@@ -271,7 +271,7 @@ __device__ __forceinline__ void tile_positions(const Kv4AttnArgs& a, int tile, i
 __device__ __forceinline__ int tile_cost(const Kv4AttnArgs& a, int tile, int G) {
   int lo, hi;
   tile_positions(a, tile, G, lo, hi);
-  return (kv4_spans(a.c, lo, hi, a.window).total * kKv4Chunk + kPKV - 1) / kPKV + kPItem;
+  return kv4_tile_cost(a.c, lo, hi, a.window);
 }
 
 // Costs of the tiles before each into pre[0 .. tiles), their sum returned; all threads of the block.
@@ -1082,8 +1082,8 @@ int launch_prefill_t(shd_ctx* ctx, const Kv4AttnArgs& a0) {
   const size_t need = (size_t)ctas * 2 * kPRows * PromptShape<128>::PART;
   if (!ctx->d_kv4_parts) SHD_CHECK_CUDA(ctx, cudaMalloc(&ctx->d_kv4_parts, need * 4 + ctas * sizeof(int4)));
   const int G = a0.H / a0.c.heads;
-  // launches of at most kPTiles tiles: whole positions
-  const int step = (int)std::min<int64_t>(a0.M, (int64_t)kPTiles * kPRows / G);
+  // launches of whole positions, of at most kPTiles tiles and a plan that fits
+  const int step = kv4_launch_positions(a0.c, a0.M, G, a0.pos0 + a0.M - 1, kPTiles);
   SHD_REQUIRE(ctx, step > 0, "shd_kv4_attn_prefill: too many heads");
   for (int m = 0; m < a0.M; m += step) {
     PromptArgs pa{};
