@@ -470,7 +470,8 @@ int shd_model_prefill_hidden(shd_model* m, int slot, const float* hc_host, const
                              float* final_s_host, int32_t* next_token_host);
 /* The reconstructed K and V rows of positions [pos0, pos0 + n) of a slot, every layer, as the
  * reference's prefill response carries them: host [n_layers][n][kv_dim] each (this rank's kv
- * heads under tensor parallelism). Synchronous. */
+ * heads under tensor parallelism). Positions that the ring of a 4-bit cache no longer holds are refused.
+ * Synchronous. */
 int shd_model_read_kv(shd_model* m, int slot, int pos0, int n, float* k_host, float* v_host);
 /* shd_model_forward_host that also returns the position's output hidden state shares [h]
  * (BinaryDecodeResponse.hidden_*); hidden outputs nullable (as a pair). */
@@ -486,7 +487,8 @@ int shd_model_forward_host_hidden(shd_model* m, int slot, const float* hc_host, 
  * the slot's length) and returns a BinaryDecodeResponse. *resp_len receives the response size;
  * a NULL or too small `resp` fails with SHD_ERR_ARG before any work, naming the size needed.
  * Malformed requests (truncated, trailing bytes, wrong dimensions) fail with SHD_ERR_ARG
- * ("Invalid binary request: ..."), as the route's InvalidRequest. Single-GPU models only. */
+ * ("Invalid binary request: ..."), as the route's InvalidRequest; so does a prompt whose K and V are asked
+ * for and of which the ring of a 4-bit cache would not hold every row. Single-GPU models only. */
 int shd_bincode_prefill(shd_model* m, int slot, const uint8_t* req, size_t req_len, int include_kv,
                         uint8_t* resp, size_t resp_cap, size_t* resp_len);
 int shd_bincode_decode(shd_model* m, int slot, const uint8_t* req, size_t req_len, uint8_t* resp,

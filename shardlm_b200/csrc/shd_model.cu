@@ -466,6 +466,12 @@ extern "C" int shd_model_set_kv4(shd_model* m, int capacity, int window, int sin
   return SHD_OK;
 }
 
+// Whether the rows of positions [pos0, pos0 + n) are in the cache of a sequence of `length`.
+bool shd_model::kv_holds(int64_t pos0, int64_t n, int64_t length) const {
+  const int64_t ring = kv4.capacity - kv4.sinks;
+  return !kv4.capacity || length <= kv4.capacity || pos0 >= length - ring || pos0 + n <= kv4.sinks;
+}
+
 Kv4View shd_model::kv4_layer(int l) const {
   Kv4View v = kv4;
   const size_t rows = (size_t)l * v.slots * v.heads * v.capacity;
@@ -849,9 +855,7 @@ extern "C" int shd_model_read_kv(shd_model* m, int slot, int pos0, int n, float*
   SHD_CHECK_CUDA(ctx, cudaSetDevice(ctx->device));
   const size_t kvd = (size_t)m->kvd, row = kvd * 4;
   if (m->kv4.capacity) {
-    const Kv4View& v = m->kv4;
-    SHD_REQUIRE(ctx, m->len[slot] <= v.capacity || pos0 >= m->len[slot] - (v.capacity - v.sinks) || pos0 + n <= v.sinks,
-                "shd_model_read_kv: positions that the cache no longer holds");
+    SHD_REQUIRE(ctx, m->kv_holds(pos0, n, m->len[slot]), "shd_model_read_kv: positions that the cache no longer holds");
     // the context's launches go to the model's stream meanwhile
     struct Scope {
       shd_model* m;

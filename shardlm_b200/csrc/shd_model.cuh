@@ -42,6 +42,7 @@ struct shd_model {
   int kv4_window = 0;
   float* kv4_rows = nullptr;             // [2][rows][qd + 2 kvd] shares of q, k, v (with RoPE)
   int prompt_slot = 0, prompt_pos = 0;   // of the block that enqueue_layers works on (not decode)
+  bool kv_holds(int64_t pos0, int64_t n, int64_t length) const;
   shd::Kv4View kv4_layer(int l) const;
   int lay_masks(const float* from, int64_t stride, int64_t to);
   int kv4_attention(int l, int M, const int* d_pos, const int* d_seq, const float* mask, bool decode);

@@ -102,6 +102,9 @@ extern "C" int shd_bincode_prefill(shd_model* m, int slot, const uint8_t* req, s
   if (seq_len == 0) return wire_fail(m, "Invalid binary request: empty prompt");
   if (nc != (uint64_t)seq_len * h || ns != nc)
     return wire_fail(m, "Invalid binary request: hidden states are not seq_len x hidden_dim");
+  // before any work: the rows of the response have to be there when the prompt has been taken in
+  if (include_kv && !m->kv_holds(m->len[slot], seq_len, (int64_t)m->len[slot] + seq_len))
+    return wire_fail(m, "shd_bincode_prefill: the cache's ring holds fewer rows than the prompt, which a response with K and V needs");
   const int L = m->cfg.n_layers, kvd = m->kvd, V = m->cfg.vocab;
   const uint64_t kv_count = include_kv ? (uint64_t)L * seq_len * kvd : 0;
   const size_t need = 4 * 8 + 2 * (size_t)h * 4 + 8 + 2 * (8 + kv_count * 4) + 2 * (size_t)V * 4;
