@@ -3,14 +3,17 @@ holds for it: slots other than the first, mask rows at strides that are not a mu
 several sequences in one pass.
 
 Every layer's K and V rows of a position are checked against the oracle's projections of that layer's
-input (tests/test_kv4_model.py states what a rounding of a code may do), so rows of another layer or slot,
-which are unrelated numbers, do not pass. Logits are held to the model tests' tolerance.
+input, so rows of another layer or slot, which are unrelated numbers, do not pass. The bounds are those
+of tests/test_kv4_model.py: an element may be off by its group's step where its code rounds the other way,
+which is rare: of all elements checked (one row of 128 holds too few to say) less than 2e-3. Logits are
+held to the model tests' tolerance.
 """
 import numpy as np
 import pytest
 import torch
 
-from test_kv4_model import LOGIT_RTOL, OneLayer, check_rows, visible
+from test_kv4 import quantise
+from test_kv4_model import LOGIT_RTOL, OneLayer, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -62,6 +65,16 @@ def held_rows(m, slot, p, window, sinks):
     return np.concatenate(ks, 1), np.concatenate(vs, 1)
 
 
+def other_codes(x, got, d):
+    """Which elements of a row read back are more than the f32 tolerance off; none by more than a step."""
+    _, params, want = quantise(x.reshape(-1, d))
+    step = np.repeat(params[:, 0].astype(np.float32), 32, axis=-1)
+    off = np.abs(got.reshape(-1, d) - want)
+    scale = np.maximum(np.abs(x).max(), 1e-3)
+    assert np.all(off <= step * 1.01 + 2e-3 * scale)
+    return (off > 2e-3 * scale).reshape(-1)
+
+
 def hidden(rng, n, h):
     x = (rng.standard_normal((n, h)) * 0.5).astype(np.float32)
     s = rng.uniform(0, 1, x.shape).astype(np.float32)
@@ -102,4 +115,50 @@ def test_mask_rows_at_any_stride(ctx, orc, odd, before):
                 lc, ls = m.forward_host(hc[p], hs[p], slot=slot)
             want, _ = ref.walk(hc[p], hs[p], p, *held_rows(m, slot, p, 24, 3))
             assert np.max(np.abs(lc + ls - want)) <= LOGIT_RTOL * np.max(np.abs(want)), (slot, p)
+    m.close()
+
+
+@pytest.mark.parametrize("name,window,sinks,cap", [("tiny", 0, 0, None), ("tiny", 40, 2, None), ("qwen2.5-1.5b", 0, 0, None),
+                                                   ("tiny", 60, 5, 592)])
+def test_every_layer_and_slot_holds_its_own_rows(ctx, orc, name, window, sinks, cap):
+    """Prompts in the slots of a model of three layers, then several sequences a pass (forward_host_rows), slots out of
+    order: K and V of every layer and the logits against the oracle."""
+    from shardlm_b200.model import SHAPES, SecureModel
+
+    orc.set_threads(orc.max_threads())
+    shape = SHAPES[name].replace(n_layers=3, vocab=1000)
+    max_seq = 80 if cap is None else 700
+    m = SecureModel(ctx, shape, max_seq=max_seq, max_batch=3)
+    host = m.load_random_weights(seed=3, host_copy=True)
+    m.set_kv4(cap, window=window, sinks=sinks)
+    prompt, token = Layers(orc, shape, host, max_seq, orc.NL_GPU), Layers(orc, shape, host, max_seq, orc.NL_APPROX)
+    rng = np.random.default_rng(4)
+    lengths = [23, 50 if cap is None else 610, 37]
+    seqs = [hidden(rng, n + 2, shape.hidden) for n in lengths]
+    differ = []
+
+    def check(slot, p, got, ref):
+        hc, hs = seqs[slot]
+        want, own = ref.walk(hc[p], hs[p], p, *held_rows(m, slot, p, window, sinks))
+        assert np.max(np.abs(got - want)) <= LOGIT_RTOL * np.max(np.abs(want)), (slot, p)
+        k, v = m.read_kv(p, 1, slot=slot)
+        for l, (kx, vx) in enumerate(own):
+            differ.append(other_codes(kx, k[l, 0], shape.head_dim))
+            differ.append(other_codes(vx, v[l, 0], shape.head_dim))
+
+    for slot in (2, 0, 1):
+        n = lengths[slot]
+        before = [m.read_kv(0, m.seq_len(s), slot=s) for s in range(3) if s != slot and m.seq_len(s) <= 592]
+        _, lc, ls, _, _ = m.prefill_hidden(seqs[slot][0][:n], seqs[slot][1][:n], slot=slot)
+        check(slot, n - 1, lc + ls, prompt)
+        after = [m.read_kv(0, m.seq_len(s), slot=s) for s in range(3) if s != slot and m.seq_len(s) <= 592]
+        for a, b in zip(before, after):
+            assert all(np.array_equal(x, y) for x, y in zip(a, b))
+    for slots in ([1, 0, 2], [2, 1]):
+        at = [m.seq_len(s) for s in slots]
+        lc, ls = m.forward_host_rows(slots, np.stack([seqs[s][0][p] for s, p in zip(slots, at)]),
+                                     np.stack([seqs[s][1][p] for s, p in zip(slots, at)]))
+        for i, (s, p) in enumerate(zip(slots, at)):
+            check(s, p, lc[i] + ls[i], token)
+    assert np.mean(np.concatenate(differ)) < 2e-3
     m.close()
