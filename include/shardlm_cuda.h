@@ -435,7 +435,11 @@ int shd_model_set_masks(shd_model* m, const float* masks, int64_t stride);
  * the first `sinks` always visible. A capacity below max_seq makes the rows behind the sinks a ring and
  * needs window + 511 <= capacity - sinks (prompts are taken in blocks of 512 positions). K and V are
  * quantised from their shares as the q/k/v linear gives them; attention then reads the quantised values,
- * of the prompt too. Only while no slot holds a sequence, and on single-GPU models. Frees the f32 cache. */
+ * of the prompt too, with an exact softmax (the clamp of the V3 variants' scores goes with the f32 cache).
+ * Positions keep their RoPE angles, the sinks' among them, however far the window has moved. Only while no
+ * slot holds a sequence, and on single-GPU models. Frees the f32 cache, which no call brings back; may be
+ * called again with another shape. Where the memory does not suffice (SHD_ERR_CUDA) the model keeps the
+ * kind of cache that it had. */
 int shd_model_set_kv4(shd_model* m, int capacity, int window, int sinks);
 /* Forget all sequences. */
 int shd_model_reset(shd_model* m);

@@ -431,39 +431,63 @@ extern "C" int shd_model_set_kv4(shd_model* m, int capacity, int window, int sin
     const int rc = m->lay_masks(m->masks, m->mask_stride, (m->mask_stride + 3) / 4 * 4);
     if (rc) return rc;
   }
+  // what a failure must not touch comes before the f32 cache goes; that goes first, as the two need not fit side by side
+  auto hold = [&](void** p, size_t bytes) -> cudaError_t {
+    const cudaError_t e = cudaMalloc(p, bytes);
+    if (e == cudaSuccess) m->owned.push_back(*p);
+    else *p = nullptr, cudaGetLastError();
+    return e;
+  };
   auto drop = [&](void* p) {
     if (!p) return;
     m->owned.erase(std::remove(m->owned.begin(), m->owned.end(), p), m->owned.end());
     cudaFree(p);
   };
-  // the f32 cache goes first: the two need not fit side by side
+  auto hold4 = [&](Kv4View& v) -> cudaError_t {
+    const size_t rows = (size_t)c.n_layers * v.slots * v.heads * v.capacity;
+    const size_t codes = rows * (c.head_dim / 2), params = rows * (c.head_dim / kKv4Group) * 4;
+    v.kc = v.vc = nullptr;
+    v.kp = v.vp = nullptr;
+    cudaError_t e = hold((void**)&v.kc, codes);
+    if (e == cudaSuccess) e = hold((void**)&v.kp, params);
+    if (e == cudaSuccess) e = hold((void**)&v.vc, codes);
+    if (e == cudaSuccess) e = hold((void**)&v.vp, params);
+    if (e != cudaSuccess)
+      for (void* p : {(void*)v.kc, (void*)v.kp, (void*)v.vc, (void*)v.vp}) drop(p);
+    return e;
+  };
+  if (!m->kv4_rows) {
+    const cudaError_t e = hold((void**)&m->kv4_rows, (size_t)2 * m->R * (m->qd + 2 * m->kvd) * 4);
+    if (e != cudaSuccess) return shd_cuda_fail(ctx, e, "shd_model_set_kv4: cudaMalloc");
+  }
+  const bool was_f32 = m->kcache != nullptr;
+  Kv4View before = m->kv4;
   for (void* p : {(void*)m->kcache, (void*)m->vcache, (void*)m->kv4.kc, (void*)m->kv4.kp, (void*)m->kv4.vc, (void*)m->kv4.vp}) drop(p);
   m->kcache = m->vcache = nullptr;
-  Kv4View v{};
-  v.slots = c.max_batch; v.heads = m->sh.kv_head_count; v.head_dim = c.head_dim; v.sinks = sinks;
-  const size_t rows = (size_t)c.n_layers * v.slots * v.heads * cap;
-  struct A {
-    void** p;
-    size_t bytes;
-  } allocs[] = {
-      {(void**)&v.kc, rows * (c.head_dim / 2)}, {(void**)&v.kp, rows * (c.head_dim / kKv4Group) * 4},
-      {(void**)&v.vc, rows * (c.head_dim / 2)}, {(void**)&v.vp, rows * (c.head_dim / kKv4Group) * 4},
-      {(void**)&m->kv4_rows, m->kv4_rows ? 0 : (size_t)2 * m->R * (m->qd + 2 * m->kvd) * 4},
-  };
   m->kv4 = Kv4View{};
-  for (auto& a : allocs) {
-    if (!a.bytes) continue;
-    cudaError_t e = cudaMalloc(a.p, a.bytes);
-    if (e != cudaSuccess) {  // no cache is left: calls that need one are refused until this one succeeds
-      for (void* p : {(void*)v.kc, (void*)v.kp, (void*)v.vc, (void*)v.vp}) drop(p);
-      return shd_cuda_fail(ctx, e, "shd_model_set_kv4: cudaMalloc");
-    }
-    m->owned.push_back(*a.p);
+  Kv4View v{};
+  v.slots = c.max_batch; v.heads = m->sh.kv_head_count; v.capacity = cap; v.head_dim = c.head_dim; v.sinks = sinks;
+  const cudaError_t e = hold4(v);
+  if (e == cudaSuccess) {
+    m->kv4 = v;
+    m->kv4_window = window;
+    return SHD_OK;
   }
-  v.capacity = cap;
-  m->kv4 = v;
-  m->kv4_window = window;
-  return SHD_OK;
+  // the memory of the former cache is free again; should it be gone, calls that need a cache are refused
+  if (was_f32) {
+    const size_t bytes = (size_t)c.n_layers * c.max_batch * c.max_seq * m->kvd * 4;
+    if (hold((void**)&m->kcache, bytes) == cudaSuccess && hold((void**)&m->vcache, bytes) != cudaSuccess) {
+      drop(m->kcache);
+      m->kcache = nullptr;
+    }
+    if (m->kcache) {
+      cudaMemset(m->kcache, 0, bytes);
+      cudaMemset(m->vcache, 0, bytes);
+    }
+  } else if (before.capacity && hold4(before) == cudaSuccess) {
+    m->kv4 = before;
+  }
+  return shd_cuda_fail(ctx, e, "shd_model_set_kv4: cudaMalloc");
 }
 
 // Whether the rows of positions [pos0, pos0 + n) are in the cache of a sequence of `length`.

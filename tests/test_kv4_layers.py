@@ -162,3 +162,24 @@ def test_every_layer_and_slot_holds_its_own_rows(ctx, orc, name, window, sinks, 
             check(s, p, lc[i] + ls[i], token)
     assert np.mean(np.concatenate(differ)) < 2e-3
     m.close()
+
+
+@pytest.mark.parametrize("had_kv4", [False, True])
+def test_a_cache_too_large_leaves_the_model_as_it_was(ctx, had_kv4):
+    """More rows than the GPU's memory: the call fails, and the model goes on with the cache it had."""
+    from shardlm_b200._lib import SHD_ERR_CUDA, ShdError
+    from shardlm_b200.model import TINY, SecureModel
+
+    m = SecureModel(ctx, TINY, max_seq=64, max_batch=2)
+    m.load_random_weights(seed=1)
+    if had_kv4:
+        m.set_kv4(window=9, sinks=2)
+    want = [m.prefill([5, 6, 7, 8] * 6), *m.decode(4)[:, 0]]
+    rows = m.read_kv(0, 24)
+    m.reset()
+    with pytest.raises(ShdError) as e:
+        m.set_kv4(2 ** 31 - 16)  # 2 layers x 2 slots x 2 heads x 2^31 rows x 80 bytes and more
+    assert e.value.code == SHD_ERR_CUDA
+    assert [m.prefill([5, 6, 7, 8] * 6), *m.decode(4)[:, 0]] == want
+    assert all(np.array_equal(a, b) for a, b in zip(rows, m.read_kv(0, 24)))
+    m.close()
