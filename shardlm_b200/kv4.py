@@ -23,6 +23,14 @@ from .sharing import SharingError
 GROUP = 32
 CHUNK = 16
 _F32, _I32 = torch.float32, torch.int32
+_INT_MAX = 0x7FFFFFFF
+
+
+def _fits(**values: int) -> None:
+    """Refuses what the C entries' 32-bit arguments would cut off."""
+    for name, v in values.items():
+        if not -_INT_MAX <= v <= _INT_MAX:
+            raise SharingError(f"{name}: {v} does not fit 32 bits")
 
 
 class Kv4Cache:
@@ -63,6 +71,7 @@ class Kv4Cache:
             raise SharingError("head_dim must be 64 or 128")
         if cap % CHUNK or not 0 <= sinks < cap:
             raise SharingError("capacity must be a multiple of 16 and above the sinks")
+        _fits(slots=slots, n_kv_heads=heads, capacity=cap)
         self.ctx, self._device = ctx, ctx.torch_device
         self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
         self.slots, self.n_kv_heads, self.capacity, self.head_dim, self.sinks = slots, heads, cap, 2 * half, sinks
@@ -150,12 +159,14 @@ class Kv4Cache:
 
     def write_prompt(self, k_client, k_server, v_client, v_server, *, slot: int, pos0: int, values: bool = False):
         """Quantise consecutive positions pos0, pos0 + 1, .. of one slot."""
+        _fits(slot=slot, pos0=pos0)
         return self._write(k_client, k_server, v_client, v_server, None, None, slot, pos0, values)
 
     def read(self, slot: int, pos0: int, n: int):
         """Positions [pos0, pos0 + n) of a slot as (K, V), f32 [n, kv_dim]."""
         if n <= 0:
             raise SharingError("read: n must be positive")
+        _fits(slot=slot, pos0=pos0, n=n)
         k, v = self._f32.new_empty(n, self.kv_dim), self._f32.new_empty(n, self.kv_dim)
         self._call(lib().shd_kv4_read, slot, pos0, n, k.data_ptr(), v.data_ptr())
         return k, v
@@ -184,6 +195,7 @@ class Kv4Cache:
     def attend(self, q: torch.Tensor, *, slot: torch.Tensor, pos: torch.Tensor, window: int = 0, mask: torch.Tensor | None = None):
         """One token for each sequence: q [M, heads * head_dim] reconstructed, row m at position pos[m] of
         slot[m] (device int32), whose K/V row is written. Output shares (attn - mask, mask), or (attn, 0)."""
+        _fits(window=window)
         q, ldq, rows, width, mask_at, mask = self._queries(q, mask)
         c, s = self._f32.new_empty(rows, width), self._f32.new_empty(rows, width)
         self._call(lib().shd_kv4_attn_decode, q.data_ptr(), ldq, width // self.head_dim, self._index(slot, rows, "slot"),
@@ -192,6 +204,7 @@ class Kv4Cache:
 
     def attend_prompt(self, q: torch.Tensor, *, slot: int, pos0: int, window: int = 0, mask: torch.Tensor | None = None):
         """Consecutive positions pos0, pos0 + 1, .. of one slot, all of whose K/V rows are written."""
+        _fits(slot=slot, pos0=pos0, window=window)
         q, ldq, rows, width, mask_at, mask = self._queries(q, mask)
         c, s = self._f32.new_empty(rows, width), self._f32.new_empty(rows, width)
         self._call(lib().shd_kv4_attn_prefill, q.data_ptr(), ldq, width // self.head_dim, slot, pos0, rows, window, mask_at,

@@ -14,7 +14,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import ModelConfigC, NL_APPROX, NL_GPU, ShardInfoC, check, lib
+from ._lib import ModelConfigC, NL_APPROX, NL_GPU, ShardInfoC, ShdError, check, lib
 from .runtime import Context, ptr
 
 
@@ -177,6 +177,8 @@ class SecureModel:
     def set_kv4(self, capacity: int | None = None, window: int = 0, sinks: int = 0) -> None:
         """Hold the key/value cache in 4 bits: `capacity` rows a slot (default max_seq), attention over the last
         `window` positions (0: all) and the first `sinks`. A capacity below max_seq is used as a ring."""
+        if any(abs(x or 0) > 0x7FFFFFFF for x in (capacity, window, sinks)):
+            raise ShdError(_lib.SHD_ERR_ARG, "set_kv4: an argument does not fit 32 bits")
         check(lib().shd_model_set_kv4(self.handle, self.max_seq if capacity is None else capacity, window, sinks),
               self.ctx.ptr)
 
