@@ -178,7 +178,7 @@ int check_cache(shd_ctx* ctx, const char* fn, const shd_kv4_cache* cache, Kv4Vie
   const std::string f(fn);
   SHD_REQUIRE(ctx, cache && cache->k_codes && cache->k_params && cache->v_codes && cache->v_params, f + ": null cache");
   SHD_REQUIRE(ctx, cache->head_dim == 64 || cache->head_dim == 128, f + ": head_dim must be 64 or 128");
-  SHD_REQUIRE(ctx, cache->slots > 0 && cache->n_kv_heads > 0, f + ": bad cache shape");
+  SHD_REQUIRE(ctx, cache->slots > 0 && cache->n_kv_heads > 0 && (int64_t)cache->n_kv_heads * cache->head_dim <= 0x7fffffff, f + ": bad cache shape");
   SHD_REQUIRE(ctx, cache->capacity > 0 && cache->capacity % kKv4Chunk == 0, f + ": capacity must be a multiple of 16");
   SHD_REQUIRE(ctx, cache->sinks >= 0 && cache->sinks < cache->capacity, f + ": sinks must be below the capacity");
   SHD_REQUIRE(ctx, shd_aligned16(cache->k_codes) && shd_aligned16(cache->k_params) && shd_aligned16(cache->v_codes) &&
@@ -203,7 +203,7 @@ int check_attn(shd_ctx* ctx, const char* fn, const shd_kv4_cache* cache, const f
   SHD_REQUIRE(ctx, q && out_c && out_s, f + ": null pointer");
   SHD_REQUIRE(ctx, H > 0 && H % a.c.heads == 0, f + ": num_heads must be a multiple of num_kv_heads");
   SHD_REQUIRE(ctx, M > 0 && window >= 0, f + ": bad shape");
-  SHD_REQUIRE(ctx, ldq >= H * a.c.head_dim && ldq % 4 == 0, f + ": query rows must be 16-byte aligned");
+  SHD_REQUIRE(ctx, ldq >= (int64_t)H * a.c.head_dim && ldq % 4 == 0, f + ": query rows must be 16-byte aligned");
   SHD_REQUIRE(ctx, shd_aligned16(q) && shd_aligned16(out_c) && shd_aligned16(out_s) && shd_aligned16(mask),
               f + ": tensors must be 16-byte aligned");
   a.q = q;
@@ -253,7 +253,7 @@ extern "C" int shd_kv4_write(shd_ctx* ctx, const shd_kv4_cache* cache, const flo
   if (rc) return rc;
   SHD_REQUIRE(ctx, kc && vc && (ks == nullptr) == (vs == nullptr), "shd_kv4_write: null pointer");
   SHD_REQUIRE(ctx, (slot == nullptr) == (pos == nullptr), "shd_kv4_write: slot and pos are given together");
-  SHD_REQUIRE(ctx, M > 0 && ld >= a.c.heads * a.c.head_dim && ld % 4 == 0, "shd_kv4_write: bad shape");
+  SHD_REQUIRE(ctx, M > 0 && ld >= (int64_t)a.c.heads * a.c.head_dim && ld % 4 == 0, "shd_kv4_write: bad shape");
   SHD_REQUIRE(ctx, shd_aligned16(kc) && shd_aligned16(ks) && shd_aligned16(vc) && shd_aligned16(vs) &&
                        shd_aligned16(k_val) && shd_aligned16(v_val), "shd_kv4_write: tensors must be 16-byte aligned");
   if (!pos) {

@@ -42,3 +42,32 @@ def test_model_arguments_past_32_bits_are_refused():
         with pytest.raises(ShdError) as e:
             m.set_kv4(**kw)
         assert e.value.code == SHD_ERR_ARG
+
+
+@pytest.mark.gpu
+def test_heads_whose_width_passes_32_bits_are_refused(ctx):
+    """Head counts whose rows would be 2^32 channels wide, which is no width in 32 bits, at every C entry."""
+    from shardlm_b200._lib import SHD_ERR_ARG, Kv4CacheC, ShdError
+    from shardlm_b200.kv4 import Kv4Cache
+
+    import ctypes
+
+    c = Kv4Cache(ctx, 1, 2, 32, 64)
+    x = torch.zeros(4, 256, device="cuda")
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    X, I, many = x.data_ptr(), i.data_ptr(), 2 ** 26
+    wide = Kv4CacheC(*[getattr(c._c, f) for f, _ in Kv4CacheC._fields_])
+    wide.n_kv_heads = many
+    W = ctypes.byref(wide)
+    for name, *args in (
+        ("shd_kv4_attn_decode", c._ref, X, 256, many, I, I, 1, 0, None, X, X),
+        ("shd_kv4_attn_prefill", c._ref, X, 256, many, 0, 0, 1, 0, None, X, X),
+        ("shd_kv4_write", W, X, None, X, None, 256, None, None, 0, 0, 1, None, None),
+        ("shd_kv4_read", W, 0, 0, 1, X, X),
+        ("shd_kv4_attn_decode", W, X, 256, many, I, I, 1, 0, None, X, X),
+        ("shd_kv4_attn_prefill", W, X, 256, many, 0, 0, 1, 0, None, X, X),
+    ):
+        with pytest.raises(ShdError) as e:
+            ctx.call(name, *args)
+        assert e.value.code == SHD_ERR_ARG, name
+    ctx.sync()
