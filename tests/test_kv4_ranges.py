@@ -186,3 +186,19 @@ def test_queries_of_any_size(ctx, prompt, size):
     v = rng.standard_normal((n, HEADS, d)) * 2.0 ** rng.integers(-12, 13, (n, HEADS, 1))
     q = (queries(rng, u, 4) * size).astype(np.float32)
     run(ctx, k, v, q, prompt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("prompt", FORMS)
+@pytest.mark.parametrize("size", [0.0, 1e-6, 1.0, 65504.0])
+def test_rows_of_one_value(ctx, d, prompt, size):
+    """Value rows whose channels are all alike, so that every scale is 0: alone, and half of them beside ordinary rows."""
+    rng = np.random.default_rng(d + int(size))
+    n, u = 90, direction(rng, d)
+    k = rng.standard_normal((n, HEADS, d))
+    v = np.broadcast_to(size * rng.choice([-1.0, 1.0], (n, HEADS, 1)), (n, HEADS, d)).copy()
+    q = queries(rng, u, 4)
+    run(ctx, k, v, q, prompt)
+    v[::2] = rng.standard_normal((n // 2, HEADS, d))
+    run(ctx, k, v, q, prompt)
