@@ -305,7 +305,10 @@ int shd_kv4_read(shd_ctx* ctx, const shd_kv4_cache* cache, int slot, int pos0, i
  * pos[m] of slot[m] (device arrays) and its own K/V row is already written. The softmax is exact (no
  * clamp of the scores). pos[m] < 0 sees nothing and gives 0; a slot outside the cache, or a position
  * past the capacity whose window the ring does not hold, gives 0 and SHD_ERR_ARG at shd_sync. Output
- * [M][H * head_dim], reshared (attn - mask, mask); mask null: (attn, 0). */
+ * [M][H * head_dim], reshared (attn - mask, mask); mask null: (attn, 0). Products are formed from two f16 terms
+ * of an operand (22 bits) and summed in f32, under powers of two that follow what contributes, so that results are as
+ * near as f32's whatever the sizes of rows and queries; of a row's channel groups, one 2^-12 of the largest or
+ * smaller loses bits. */
 int shd_kv4_attn_decode(shd_ctx* ctx, const shd_kv4_cache* cache, const float* q, int ldq, int H,
                         const int32_t* slot, const int32_t* pos, int M, int window,
                         const float* mask, float* out_c, float* out_s);

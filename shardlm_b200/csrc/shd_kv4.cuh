@@ -122,6 +122,7 @@ inline int kv4_launch_positions(const Kv4View& c, int M, int G, int last, int ti
 // ------------------------------------------------------------------------------------------------
 constexpr float kKv4Never = -3.0e38f;  // running maximum before any row
 
+// the hardware's 2^x, to some 2^-22 of it and 0 below 2^-126: the rounding of an ordinary score moves a weight by more
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -8,10 +8,10 @@
 // is c * 2^-20), centred to (c - 7.5) * 2^-9, also exact, by one more: weights add up to 1 over many rows
 // whose values cancel, and sums of codes that are all positive would lose what cancels (measured
 // against 64 bits at 131000 positions: 5e-4 of the result). The other operand is split into two f16 terms
-// (22 bits, or 2^-37 of the largest beside them): the queries, scaled by a power of two of their head, and the
-// weights p_t s_tg, scaled by a running power of two of the largest of their head: the largest over rows
-// of weight times the row's largest scale, so that a row which weighs nothing has no say however large its values
-// are. A group whose scales are 2^-k of the row's largest loses bits from k = 15 on, to 2^-37 of that largest part.
+// (22 bits, or 2^-37 of the largest beside them): the queries and their group sums, scaled by powers of two
+// of their head, and the weights p_t s_tg, scaled by a running power of two of their head that follows
+// the largest weight times its row's largest scale, so that a row which weighs nothing has no say however
+// large its values are. A group whose scales are 2^-k of the row's largest loses bits from k = 15 on.
 // Sums are f32. Rows of the first product's A are the 8 heads' high terms and the 8 heads' low terms;
 // the second takes the two terms one after the other:
 //   S [8 + 8 heads x 8 rows]      += Q [16 x 16 channels] K^T   per group, then scaled by s
@@ -29,12 +29,12 @@
 // leaves partial results; the CTA that arrives last joins them in CTA order, so results do not depend on
 // timing.
 //
-// Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 41.7 us (2.0 TB/s of cache); 64
-// ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 73.5 us (2.3 TB/s); 8 at 1041 to 1280
-// positions 14.9 us; one at 554 positions 10.2 us. No pipe is full in the long ones (of the windowed batch's
+// Measured on a B200: one sequence at 131001 positions, 28 heads over 4, 42.1 us (2.0 TB/s of cache); 64
+// ragged ones under a window of 2048 and 4 sinks, 40 heads over 8, 73.1 us (2.3 TB/s); 8 at 1041 to 1280
+// positions 15.1 us; one at 554 positions 10.2 us. No pipe is full in the long ones (of the windowed batch's
 // time on the SMs the integer pipe is busy 38 %, tensor 23 %, issue slots 56 %, memory 27 %): a chunk of 16
 // rows is some 500 instructions of a warp in dependent steps, and the registers hold four warps a scheduler.
-// It takes 198 clocks of an SM, where its 215 integer and conversion instructions alone take 107. Short ones
+// It takes 196 clocks of an SM, where its 215 integer and conversion instructions alone take 107. Short ones
 // are bound by the chain of launch, plan, first rows from memory, combine and join, one after the other.
 #include <cmath>
 

@@ -5,7 +5,8 @@
 // share every unpacked row. It walks the rows that any of its positions sees, 64 at a time:
 //   S [128 x 64]       = Q [128 x HD] K^T      O [128 x HD] += P [128 x 64] V
 // Operands are f16 in two terms. The keys of 32 rows are divided by a power of two of theirs and
-// s (c - 7.5) is then exactly two terms (11 + 5 bits); queries, weights and minima keep 22 bits of theirs. Three of the
+// s (c - 7.5) is then exactly two terms (11 + 5 bits); queries, their group sums, weights and the values'
+// middles keep 22 bits of theirs, the keys' minima are exact. Three of the
 // four term products are formed (the fourth is below 2^-22 of the sum), accumulated in f32 in
 // tensor memory. Where the 32 rows' sizes are more than 2^6 apart, each row has a power of two of its own
 // and the softmax goes row by row (a large row that weighs nothing would else take the bits of the others).
@@ -34,12 +35,13 @@
 // values, reference, sum) in context scratch, and each CTA the place of the cut at its end, and a second
 // kernel joins them.
 //
-// Measured on a B200 (4 H HD FLOP a visible position): 512 positions after 8191, 40 heads over 8, 282 us,
-// 314 TFLOP/s; 512 from the start, 28 heads over 4, 32 us; 2000 under a window of 512, 12 heads over 2,
-// masked, 56 us. The three term products make the tensor work 3.1 times that. A 64-row step takes 3040
-// clocks of the softmax warps (scores to weights 1700, drains 690 on average, the rest waiting for the
-// tensor core, which is issued MMAs for 1970 of them); an item's queries and results take some 11000, which
-// is what bounds short prompts.
+// Measured on a B200 (4 H HD FLOP a visible position): 512 positions after 8191, 40 heads over 8, 292 us,
+// 303 TFLOP/s, over 100 launches, 302 to 319 us in long runs; 512 from the start, 28 heads over 4, 32.7 us; 2000 under
+// a window of 512, 12 heads over 2, masked, 57.3 us. Of these 9, 0.4 and 1.3 us are the price of telling rows of
+// unlike size apart. The three term products make the tensor work 3.1 times that. Before that a 64-row step took
+// 3040 clocks of the softmax warps (scores to weights 1700, drains 690 on average, the rest waiting for the
+// tensor core, which is issued MMAs for 1970 of them), now some 3 % more; an item's queries and results take some
+// 11000, which is what bounds short prompts.
 #include <cmath>
 
 #include "shd_kv4.cuh"
@@ -223,9 +225,9 @@ struct RowParams {
   }
 };
 
-// Where rows have their own powers of two, or scores may pass 2^23 and a reference that is rounded would be off by more
-// than the weights' room (here they are rounded as it is), seldom: score + e row by row, or out of sight, in the scores' place (apart
-// from the walk, whose code this would spread out)
+// Score + e row by row, or out of sight, in the scores' place: where rows have their own powers of two, or scores may
+// pass 2^23 and a reference that is rounded would be off by more than the weights' room (here the scores are
+// rounded as it is). Seldom, and so apart from the walk, whose code this would spread out.
 __device__ __noinline__ void own_scores(uint32_t t_s, const float* own, const int* rp, float4 of32, float rowf, int p) {
 #pragma unroll 1
   for (int y = 0; y < 32; y += 8) {
